@@ -40,6 +40,7 @@ typedef struct CUstream_st* lr_stream_t; /* == cudaStream_t */
 #define LR_DEVERR_PIPE_TIMEOUT 0x4   /* a GEMM pipeline wait ran out of time */
 #define LR_DEVERR_BAD_SEGMENT 0x8    /* a GEMM row segment outside the row range */
 #define LR_DEVERR_PEER_TIMEOUT 0x10  /* another rank's exchange flag did not arrive in time */
+#define LR_DEVERR_BAD_ADAPTER 0x20   /* an adapter number outside [-1, number of adapters) */
 
 const char* lr_status_string(int status);
 int lr_abi_version(void);
@@ -250,6 +251,89 @@ int lr_grouped_w4a16_gemm(const void* device_table, int E, int mode, int mat,
 int lr_quantized_matmul(const void* device_table, const void* A, int M, int K, int N,
                         int group_size, void* C, void* workspace, size_t workspace_bytes,
                         int32_t* err, lr_stream_t stream);
+
+/* ---- router training ------------------------------------------------------
+ * Gradients are computed without atomics: the same inputs give the same bits. */
+
+/* Top-k softmax gating with per-expert counts and the balance loss, from fp32
+ * logits (selection and weights as lr_topk_gating_dispatch, no dispatch):
+ *   expert_ids[S] int32, gate_weights[S] fp32, S = T*k;
+ *   counts[E + 1] int32: slots of each expert, then the number n of live tokens;
+ *   aux_loss[1] fp32 = load_balance_weight * E * sum_e (counts_e / (n k)) * mean_live(p_e).
+ * token_mask[T] (nullable; bytes, 0 = padding): a padded token keeps valid ids,
+ * gets weight 0 and enters neither counts nor loss, whatever its logits hold
+ * (NaN included).  n = 0 gives a loss of 0.  T = 0 is accepted.
+ * Limits: E <= 64, 1 <= k <= min(E, 8).                                    */
+size_t lr_balanced_gating_workspace_bytes(int num_tokens, int num_experts);
+int lr_balanced_gating(const float* logits, const uint8_t* token_mask, int T, int E, int k,
+                       float load_balance_weight, int32_t* expert_ids, float* gate_weights,
+                       int32_t* counts, float* aux_loss, void* workspace, size_t workspace_bytes,
+                       lr_stream_t stream);
+
+/* d_logits[T,E] from d_weights[S] and d_aux[1] (device; either may be NULL =
+ * zero).  counts is lr_balanced_gating's, or with counts_are_offsets != 0 the
+ * uncapped CSR offsets[E+1] of a dispatch without a token mask.  The counts
+ * are constants of the loss.  Padded tokens get zeros.                        */
+int lr_balanced_gating_backward(const float* logits, const uint8_t* token_mask,
+                                const int32_t* expert_ids, const int32_t* counts,
+                                int counts_are_offsets, const float* d_weights,
+                                const float* d_aux, int T, int E, int k,
+                                float load_balance_weight, float* d_logits, lr_stream_t stream);
+
+/* Gradients of lr_gate_logits: d_h[T,d] fp16 = d_logits . wg, d_wg[E,d] fp32 =
+ * d_logits^T . h, d_bias[E] fp32 = column sums (each nullable; d_bias needs
+ * d_wg).  d_logits[T,E] fp32 is not rounded.  Limits as lr_gate_logits; h, wg
+ * and d_h 16-byte aligned.                                                  */
+size_t lr_gate_backward_workspace_bytes(int num_tokens, int d_model, int num_experts);
+int lr_gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d, int E,
+                     void* d_h, float* d_wg, float* d_bias, void* workspace,
+                     size_t workspace_bytes, lr_stream_t stream);
+
+/* Gradient of the row dispatch: d_x[t,:] = fp16(sum_j d_permuted[slot_pos[t*k+j],:])
+ * over kept slots, fp32 in slot order.  d % 8 == 0.                           */
+int lr_dispatch_backward(const void* d_permuted, const int32_t* slot_pos, int T, int k, int d,
+                         void* d_x, lr_stream_t stream);
+
+/* Gradients of lr_combine over the T*k rows of a dispatch:
+ * d_y[slot_pos[s],:] = fp16(gate_weights[s] * d_out[t,:]), d_weights[s] =
+ * <d_out[t,:], y[slot_pos[s],:]> in fp32 (0 for a dropped slot); the rows of
+ * d_y that no slot keeps (past kept_counts in each segment of offsets) are
+ * zero.  d % 8 == 0.                                                        */
+int lr_combine_backward(const void* d_out, const void* y, const float* gate_weights,
+                        const int32_t* slot_pos, const int32_t* offsets,
+                        const int32_t* kept_counts, int T, int k, int d, int E, void* d_y,
+                        float* d_weights, lr_stream_t stream);
+
+/* ---- low-rank adapters of many requests -----------------------------------
+ * Row t of x (R x K fp16) uses adapter index[t] in [0, num_adapters), or none
+ * (-1; any other number is flagged LR_DEVERR_BAD_ADAPTER and taken as none).
+ * A bank holds a[num_adapters][rank][K] and b[num_adapters][N][rank], fp16, and
+ * scale[num_adapters] fp32 (NULL = 1).  x . a^T stays fp32; products are
+ * accumulated in fp32 and rounded once.
+ *   add:    out = base + scale (x a^T) b^T
+ *   swiglu: out = silu(gate + delta_gate) * (up + delta_up)
+ * out may be base (gate or up) itself: rows without an adapter are then left
+ * alone by add.  A row's result depends on its own adapter only.
+ * Limits: K, N and rank multiples of 8, rank <= 128; x, a, b, base, gate, up
+ * and out 16-byte aligned.  num_banks is 1 for add and 2 for swiglu.          */
+size_t lr_adapter_workspace_bytes(int num_rows, int rank, int num_banks);
+int lr_adapter_add(const void* x, int R, int K, const int32_t* index, int num_adapters,
+                   const void* a, const void* b, const float* scale, int rank, int N,
+                   const void* base, void* out, void* workspace, size_t workspace_bytes,
+                   int32_t* err, lr_stream_t stream);
+int lr_adapter_swiglu(const void* x, int R, int K, const int32_t* index, int num_adapters,
+                      const void* a_gate, const void* b_gate, const float* scale_gate,
+                      const void* a_up, const void* b_up, const float* scale_up, int rank, int N,
+                      const void* gate, const void* up, void* out, void* workspace,
+                      size_t workspace_bytes, int32_t* err, lr_stream_t stream);
+
+/* index[S] of a dispatch's rows for a bank with one entry per (adapter, expert),
+ * entry adapter * E + e: adapter_ids[T] in [-1, num_adapters) per token; dropped
+ * rows and tokens without an adapter get -1.                                 */
+int lr_adapter_rows(const int32_t* adapter_ids, int T, int num_adapters,
+                    const int32_t* source_idx, const int32_t* offsets,
+                    const int32_t* kept_counts, int S, int E, int32_t* index, int32_t* err,
+                    lr_stream_t stream);
 
 /* ---- expert-parallel exchange over NVLink peer memory --------------------
  * Replaces the all-GPU expert execution + host all-reduce of the reference's

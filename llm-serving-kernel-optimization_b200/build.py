@@ -29,7 +29,9 @@ CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 NVCC = str(CUDA_HOME / "bin" / "nvcc")
 
 CU_SOURCES = ["lr_capi.cu", "lr_routing.cu", "lr_w4a16_gemm.cu", "lr_w4a16_i8.cu",
-              "lr_w4a16_skinny.cu", "lr_w4a16_generic.cu", "lr_ep.cu"]
+              "lr_w4a16_skinny.cu", "lr_w4a16_generic.cu", "lr_ep.cu",
+              "lr_router_grad.cu", "lr_adapters.cu"]
+OPS_SOURCES = ["lr_torch_ops.cpp", "lr_adapt_ops.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -74,21 +76,31 @@ def build_kernels(force: bool = False, jobs: int = 4) -> Path:
     return KERNEL_LIB
 
 
-def build_torch_ops(force: bool = False) -> Path:
+def build_torch_ops(force: bool = False, jobs: int = 4) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    src = CSRC / "lr_torch_ops.cpp"
-    if not (force or _stale(OPS_LIB, [src, KERNEL_LIB] + _headers())):
-        return OPS_LIB
+    deps = _headers() + sorted(CSRC.glob("*.h"))
     inc = cpp_extension.include_paths() + [str(CUDA_HOME / "include"), str(INCLUDE),
                                            sysconfig.get_paths()["include"]]
     libdirs = cpp_extension.library_paths()
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           "-DTORCH_EXTENSION_NAME=_lr_torch_ops", str(src), "-o", str(OPS_LIB)]
-    for i in inc:
-        cmd += ["-I", i]
+    objs, todo = [], []
+    for name in OPS_SOURCES:
+        src = CSRC / name
+        o = OBJ_DIR / (src.stem + "_ops.o")
+        objs.append(o)
+        if force or _stale(o, [src] + deps):
+            cmd = ["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+                   "-DTORCH_EXTENSION_NAME=_lr_torch_ops", "-c", str(src), "-o", str(o)]
+            for i in inc:
+                cmd += ["-I", i]
+            todo.append(cmd)
+    with ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
+        list(ex.map(_run, todo))
+    if not (force or _stale(OPS_LIB, objs + [KERNEL_LIB])):
+        return OPS_LIB
+    cmd = ["g++", "-shared", *map(str, objs), "-o", str(OPS_LIB)]
     for d in libdirs:
         cmd += ["-L", d, f"-Wl,-rpath,{d}"]
     cmd += ["-L", str(LIB_DIR), "-l:liblr_kernels.so", "-Wl,-rpath,$ORIGIN",
@@ -99,7 +111,7 @@ def build_torch_ops(force: bool = False) -> Path:
 
 def build(force: bool = False, jobs: int = 4) -> None:
     build_kernels(force, jobs)
-    build_torch_ops(force)
+    build_torch_ops(force, jobs)
 
 
 if __name__ == "__main__":

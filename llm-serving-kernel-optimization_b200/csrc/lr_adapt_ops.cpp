@@ -1,0 +1,493 @@
+// lr_adapt_ops.cpp -- torch custom ops of the router's training path (with
+// their autograd formulas) and of the low-rank adapters.
+//
+// balanced_gating, gate_projection, dispatch_tokens and combine_tokens are
+// differentiable once: a backward pass that is itself recorded
+// (create_graph=True) is refused.
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <vector>
+
+#include "lr_ops_common.h"
+
+namespace {
+
+using namespace lr_ops;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = c10::optional<at::Tensor>;
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// Contiguous, 16-byte aligned, of type `type` (a copy only where it is not already).
+at::Tensor rows16(const at::Tensor& t, at::ScalarType type) {
+  at::Tensor r = t.detach().to(type).contiguous();
+  if (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15u) r = r.clone(at::MemoryFormat::Contiguous);
+  return r;
+}
+
+void check_same_device(const at::Tensor& t, const at::Tensor& like, const char* name) {
+  TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", expected ",
+              like.device());
+}
+
+void check_int32(const at::Tensor& t, const at::Tensor& like, int64_t n, const char* name) {
+  check_cuda(t, name);
+  check_same_device(t, like, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.numel() == n, name, ": ", n, " int32 expected");
+}
+
+void check_once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "lightning_router.", what,
+              " is differentiable once: backward with create_graph=True is not supported");
+}
+
+// ---------------------------------------------------------------------------
+// balanced gating
+// ---------------------------------------------------------------------------
+struct BalancedGating : public torch::autograd::Function<BalancedGating> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits_in,
+                               const OptTensor& mask_in, int64_t k, double lbw) {
+    TORCH_CHECK(logits_in.is_cuda(), "logits must be a CUDA tensor");
+    TORCH_CHECK(logits_in.dim() == 2 && logits_in.scalar_type() == at::kFloat,
+                "logits: (T,E) fp32");
+    c10::cuda::CUDAGuard g(logits_in.device());
+    const at::Tensor logits = logits_in.detach().contiguous();
+    const int64_t T = logits.size(0), E = logits.size(1);
+    TORCH_CHECK(E >= 1 && E <= 64 && k >= 1 && k <= 8 && k <= E,
+                "balanced_gating: 1 <= E <= 64 and 1 <= k <= min(E, 8) expected, got E=", E,
+                ", k=", k);
+    at::Tensor mask;
+    if (given(mask_in)) {
+      check_same_device(*mask_in, logits, "token_mask");
+      TORCH_CHECK(mask_in->scalar_type() == at::kBool && mask_in->numel() == T,
+                  "token_mask: (T,) bool");
+      mask = mask_in->reshape({-1}).contiguous();
+    }
+    auto ids = at::empty({T * k}, logits.options().dtype(at::kInt));
+    auto gw = at::empty({T * k}, logits.options());
+    auto stats = at::empty({E + 1}, logits.options().dtype(at::kInt));
+    auto aux = at::empty({}, logits.options());
+    auto ws = workspace(lr_balanced_gating_workspace_bytes(int(T), int(E)), logits);
+    check_status(lr_balanced_gating(logits.data_ptr<float>(),
+                                    mask.defined() ? static_cast<const uint8_t*>(mask.data_ptr())
+                                                   : nullptr,
+                                    int(T), int(E), int(k), float(lbw), ids.data_ptr<int32_t>(),
+                                    gw.data_ptr<float>(), stats.data_ptr<int32_t>(),
+                                    aux.data_ptr<float>(), ws.data_ptr(), size_t(ws.numel()),
+                                    cur_stream()),
+                 "balanced_gating");
+    ctx->mark_non_differentiable({ids, stats});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits_in, mask, ids, stats});
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["lbw"] = lbw;
+    return {ids, gw, stats, aux};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("balanced_gating");
+    const auto saved = ctx->get_saved_variables();
+    const int64_t k = ctx->saved_data["k"].toInt();
+    const double lbw = ctx->saved_data["lbw"].toDouble();
+    if (!grads[1].defined() && !grads[3].defined()) return {{}, {}, {}, {}};
+    c10::cuda::CUDAGuard g(saved[0].device());
+    const at::Tensor logits = saved[0].detach().contiguous();
+    const at::Tensor dw = grads[1].defined() ? grads[1].contiguous() : grads[1];
+    const at::Tensor da = grads[3].defined() ? grads[3].contiguous() : grads[3];
+    auto dl = at::empty_like(logits);
+    check_status(
+        lr_balanced_gating_backward(
+            logits.data_ptr<float>(),
+            saved[1].defined() ? static_cast<const uint8_t*>(saved[1].data_ptr()) : nullptr,
+            saved[2].data_ptr<int32_t>(), saved[3].data_ptr<int32_t>(), 0,
+            dw.defined() ? dw.data_ptr<float>() : nullptr,
+            da.defined() ? da.data_ptr<float>() : nullptr, int(logits.size(0)),
+            int(logits.size(1)), int(k), float(lbw), dl.data_ptr<float>(), cur_stream()),
+        "balanced_gating (backward)");
+    return {dl, {}, {}, {}};
+  }
+};
+
+std::vector<at::Tensor> balanced_gating(const at::Tensor& logits, const OptTensor& token_mask,
+                                        int64_t k, double lbw) {
+  return BalancedGating::apply(logits, token_mask, k, lbw);
+}
+
+// ---------------------------------------------------------------------------
+// gate projection
+// ---------------------------------------------------------------------------
+struct GateProjection : public torch::autograd::Function<GateProjection> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w,
+                            const OptTensor& bias) {
+    TORCH_CHECK(h.is_cuda() && w.is_cuda(), "hidden and gate_weight must be CUDA tensors");
+    TORCH_CHECK(h.dim() == 2 && w.dim() == 2 && h.size(1) == w.size(1),
+                "gate_projection: hidden (T,d) and gate_weight (E,d) expected");
+    TORCH_CHECK(at::isFloatingType(h.scalar_type()) && at::isFloatingType(w.scalar_type()),
+                "gate_projection: floating-point inputs expected");
+    check_same_device(w, h, "gate_weight");
+    c10::cuda::CUDAGuard g(h.device());
+    const int64_t T = h.size(0), d = h.size(1), E = w.size(0);
+    const at::Tensor hh = rows16(h, at::kHalf), wh = rows16(w, at::kHalf);
+    at::Tensor b;
+    if (given(bias)) {
+      check_same_device(*bias, h, "bias");
+      TORCH_CHECK(bias->numel() == E, "bias: (E,)");
+      b = bias->detach().to(at::kFloat).contiguous();
+    }
+    auto out = at::empty({T, E}, h.options().dtype(at::kFloat));
+    check_status(lr_gate_logits(hh.data_ptr(), wh.data_ptr(),
+                                b.defined() ? b.data_ptr<float>() : nullptr, int(T), int(d),
+                                int(E), out.data_ptr<float>(), cur_stream()),
+                 "gate_projection");
+    ctx->set_materialize_grads(false);
+    // an input that is used as it is goes in as the input, so that writing to it
+    // before the backward pass is noticed
+    ctx->save_for_backward({hh.is_same(h) || hh.data_ptr() == h.data_ptr() ? h : hh,
+                            wh.data_ptr() == w.data_ptr() ? w : wh});
+    ctx->saved_data["need_h"] = h.requires_grad();
+    ctx->saved_data["need_w"] = w.requires_grad();
+    ctx->saved_data["need_b"] = given(bias) && bias->requires_grad();
+    ctx->saved_data["h_type"] = int64_t(h.scalar_type());
+    ctx->saved_data["w_type"] = int64_t(w.scalar_type());
+    ctx->saved_data["b_type"] = int64_t(given(bias) ? bias->scalar_type() : at::kFloat);
+    ctx->saved_data["b_shape"] = given(bias) ? bias->sizes().vec() : std::vector<int64_t>{E};
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("gate_projection");
+    if (!grads[0].defined()) return {{}, {}, {}};
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor h = saved[0].detach(), w = saved[1].detach();
+    c10::cuda::CUDAGuard g(h.device());
+    const at::Tensor dl = grads[0].contiguous();
+    const int64_t T = h.size(0), d = h.size(1), E = w.size(0);
+    const bool need_h = ctx->saved_data["need_h"].toBool();
+    const bool need_b = ctx->saved_data["need_b"].toBool();
+    const bool need_w = ctx->saved_data["need_w"].toBool() || need_b;
+    const auto fopt = dl.options();
+    at::Tensor dh, dw, db;
+    if (need_h) dh = at::empty({T, d}, h.options());
+    if (need_w) dw = at::empty({E, d}, fopt);
+    if (need_b) db = at::empty({E}, fopt);
+    auto ws = workspace(need_w ? lr_gate_backward_workspace_bytes(int(T), int(d), int(E)) : 0, dl);
+    check_status(lr_gate_backward(h.data_ptr(), w.data_ptr(), dl.data_ptr<float>(), int(T), int(d),
+                                  int(E), need_h ? dh.data_ptr() : nullptr,
+                                  need_w ? dw.data_ptr<float>() : nullptr,
+                                  need_b ? db.data_ptr<float>() : nullptr, ws.data_ptr(),
+                                  size_t(ws.numel()), cur_stream()),
+                 "gate_projection (backward)");
+    if (need_h) dh = dh.to(at::ScalarType(ctx->saved_data["h_type"].toInt()));
+    if (need_w) dw = dw.to(at::ScalarType(ctx->saved_data["w_type"].toInt()));
+    if (need_b)
+      db = db.to(at::ScalarType(ctx->saved_data["b_type"].toInt()))
+               .view(ctx->saved_data["b_shape"].toIntVector());
+    return {dh, dw, db};
+  }
+};
+
+at::Tensor gate_projection(const at::Tensor& h, const at::Tensor& w, const OptTensor& bias) {
+  return GateProjection::apply(h, w, bias);
+}
+
+// ---------------------------------------------------------------------------
+// dispatch
+// ---------------------------------------------------------------------------
+using DispatchSig = std::vector<at::Tensor>(const OptTensor&, const at::Tensor&, int64_t, int64_t,
+                                            double, bool, bool, const OptTensor&);
+
+// Outputs as topk_gating_dispatch: ids 0, weights 1, tokens 2, offsets 3, kept 4,
+// aux 5, permuted 6, routing weights 7, sources 8, slot rows 9.
+struct DispatchTokens : public torch::autograd::Function<DispatchTokens> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& logits,
+                               int64_t k, int64_t capacity, double lbw, const OptTensor& err) {
+    TORCH_CHECK(x.is_cuda() && logits.is_cuda(), "x and logits must be CUDA tensors");
+    TORCH_CHECK(x.dim() == 2 && x.scalar_type() == at::kHalf, "x: (T,d) fp16");
+    TORCH_CHECK(logits.dim() == 2 && logits.scalar_type() == at::kFloat &&
+                    logits.size(0) == x.size(0),
+                "logits: (T,E) fp32");
+    check_same_device(logits, x, "logits");
+    c10::cuda::CUDAGuard g(x.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("lightning_router::topk_gating_dispatch", "")
+                               .typed<DispatchSig>();
+    auto out = op.call(rows16(x, at::kHalf), logits.detach().contiguous(), k, capacity, lbw, true,
+                       true, err);
+    ctx->mark_non_differentiable({out[0], out[2], out[3], out[4], out[7], out[8], out[9]});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, out[0], out[3], out[9]});
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["lbw"] = lbw;
+    ctx->saved_data["d"] = x.size(1);
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("dispatch_tokens");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor logits = saved[0].detach().contiguous();
+    c10::cuda::CUDAGuard g(logits.device());
+    const int64_t T = logits.size(0), E = logits.size(1);
+    const int64_t k = ctx->saved_data["k"].toInt(), d = ctx->saved_data["d"].toInt();
+    const double lbw = ctx->saved_data["lbw"].toDouble();
+    at::Tensor dx, dl;
+    if (grads[6].defined()) {
+      const at::Tensor dp = rows16(grads[6], at::kHalf);
+      dx = at::empty({T, d}, dp.options());
+      check_status(lr_dispatch_backward(dp.data_ptr(), saved[3].data_ptr<int32_t>(), int(T), int(k),
+                                        int(d), dx.data_ptr(), cur_stream()),
+                   "dispatch_tokens (backward)");
+    }
+    if (grads[1].defined() || grads[5].defined()) {
+      const at::Tensor dw = grads[1].defined() ? grads[1].contiguous() : grads[1];
+      const at::Tensor da = grads[5].defined() ? grads[5].contiguous() : grads[5];
+      dl = at::empty_like(logits);
+      check_status(lr_balanced_gating_backward(
+                       logits.data_ptr<float>(), nullptr, saved[1].data_ptr<int32_t>(),
+                       saved[2].data_ptr<int32_t>(), 1,
+                       dw.defined() ? dw.data_ptr<float>() : nullptr,
+                       da.defined() ? da.data_ptr<float>() : nullptr, int(T), int(E), int(k),
+                       float(lbw), dl.data_ptr<float>(), cur_stream()),
+                   "dispatch_tokens (backward)");
+    }
+    return {dx, dl, {}, {}, {}, {}};
+  }
+};
+
+std::vector<at::Tensor> dispatch_tokens(const at::Tensor& x, const at::Tensor& logits, int64_t k,
+                                        int64_t capacity, double lbw, const OptTensor& err) {
+  return DispatchTokens::apply(x, logits, k, capacity, lbw, err);
+}
+
+// ---------------------------------------------------------------------------
+// combine
+// ---------------------------------------------------------------------------
+struct CombineTokens : public torch::autograd::Function<CombineTokens> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& w,
+                            const at::Tensor& slot_pos, const at::Tensor& offsets,
+                            const at::Tensor& kept, int64_t k) {
+    TORCH_CHECK(y.is_cuda() && w.is_cuda(), "y and gate_weights must be CUDA tensors");
+    const int64_t S = slot_pos.numel();
+    TORCH_CHECK(k >= 1 && S % k == 0, "slot count must be T*k");
+    TORCH_CHECK(y.dim() == 2 && y.scalar_type() == at::kHalf && y.size(0) == S,
+                "y: one fp16 row per slot, (T*k, d)");
+    TORCH_CHECK(w.scalar_type() == at::kFloat && w.numel() == S, "gate_weights: (T*k,) fp32");
+    check_same_device(w, y, "gate_weights");
+    check_int32(slot_pos, y, S, "slot_pos");
+    const int64_t E = kept.numel();
+    check_int32(kept, y, E, "kept_counts");
+    check_int32(offsets, y, E + 1, "offsets");
+    c10::cuda::CUDAGuard g(y.device());
+    const at::Tensor yc = rows16(y, at::kHalf), wc = w.detach().contiguous();
+    const int64_t T = S / k, d = y.size(1);
+    auto out = at::empty({T, d}, yc.options());
+    check_status(lr_combine(yc.data_ptr(), wc.data_ptr<float>(), slot_pos.data_ptr<int32_t>(),
+                            int(T), int(k), int(d), out.data_ptr(), cur_stream()),
+                 "combine_tokens");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({yc.data_ptr() == y.data_ptr() ? y : yc, w, slot_pos, offsets, kept});
+    ctx->saved_data["k"] = k;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("combine_tokens");
+    if (!grads[0].defined()) return {{}, {}, {}, {}, {}, {}};
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor y = saved[0].detach(), w = saved[1].detach().contiguous();
+    c10::cuda::CUDAGuard g(y.device());
+    const int64_t k = ctx->saved_data["k"].toInt();
+    const int64_t S = y.size(0), d = y.size(1), E = saved[4].numel();
+    const at::Tensor dout = rows16(grads[0], at::kHalf);
+    auto dy = at::empty({S, d}, y.options());
+    auto dw = at::empty({S}, w.options());
+    check_status(lr_combine_backward(dout.data_ptr(), y.data_ptr(), w.data_ptr<float>(),
+                                     saved[2].data_ptr<int32_t>(), saved[3].data_ptr<int32_t>(),
+                                     saved[4].data_ptr<int32_t>(), int(S / k), int(k), int(d),
+                                     int(E), dy.data_ptr(), dw.data_ptr<float>(), cur_stream()),
+                 "combine_tokens (backward)");
+    return {dy, dw.view(w.sizes()), {}, {}, {}, {}};
+  }
+};
+
+at::Tensor combine_tokens(const at::Tensor& y, const at::Tensor& w, const at::Tensor& slot_pos,
+                          const at::Tensor& offsets, const at::Tensor& kept, int64_t k) {
+  return CombineTokens::apply(y, w, slot_pos, offsets, kept, k);
+}
+
+// ---------------------------------------------------------------------------
+// low-rank adapters
+// ---------------------------------------------------------------------------
+struct Bank {
+  const void* a;
+  const void* b;
+  const float* scale;
+  int64_t n, r, K, N;
+};
+
+Bank check_bank(const at::Tensor& a, const at::Tensor& b, const OptTensor& scale,
+                const at::Tensor& x) {
+  check_cuda(a, "adapter a");
+  check_cuda(b, "adapter b");
+  check_same_device(a, x, "adapter a");
+  check_same_device(b, x, "adapter b");
+  TORCH_CHECK(a.dim() == 3 && b.dim() == 3 && a.size(0) == b.size(0) && a.size(1) == b.size(2) &&
+                  a.scalar_type() == at::kHalf && b.scalar_type() == at::kHalf,
+              "adapters: a (n, rank, K) and b (n, N, rank) fp16 expected");
+  const int64_t n = a.size(0), r = a.size(1);
+  TORCH_CHECK(n >= 1, "adapters: an empty bank");
+  TORCH_CHECK(r >= 8 && r <= 128 && r % 8 == 0 && a.size(2) % 8 == 0 && b.size(1) % 8 == 0,
+              "adapters: rank (at most 128), K and N must be multiples of 8, got rank=", r,
+              ", K=", a.size(2), ", N=", b.size(1));
+  const float* s = nullptr;
+  if (given(scale)) {
+    check_cuda(*scale, "adapter scale");
+    check_same_device(*scale, x, "adapter scale");
+    TORCH_CHECK(scale->scalar_type() == at::kFloat && scale->numel() == n,
+                "adapter scale: (n,) fp32");
+    s = scale->data_ptr<float>();
+  }
+  TORCH_CHECK(x.size(1) == a.size(2), "adapters: x has ", x.size(1), " columns, a ", a.size(2));
+  return {a.data_ptr(), b.data_ptr(), s, n, r, a.size(2), b.size(1)};
+}
+
+void check_rows(const at::Tensor& t, const at::Tensor& x, int64_t N, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  check_same_device(t, x, name);
+  TORCH_CHECK(t.dim() == 2 && t.scalar_type() == at::kHalf && t.size(0) == x.size(0) &&
+                  t.size(1) == N,
+              name, ": (", x.size(0), ", ", N, ") fp16 expected");
+}
+
+// The result tensor: a new one, or `out`, which may share memory with the rows
+// it is computed from only as the very same tensor.
+at::Tensor result_rows(const OptTensor& out, const at::Tensor& x, int64_t N,
+                       std::initializer_list<at::Tensor> reads) {
+  if (!given(out)) return at::empty({x.size(0), N}, x.options());
+  check_rows(*out, x, N, "out");
+  TORCH_CHECK(out->is_contiguous() && (reinterpret_cast<uintptr_t>(out->data_ptr()) & 15u) == 0,
+              "out must be contiguous and 16-byte aligned");
+  const char* o0 = static_cast<const char*>(out->data_ptr());
+  const char* o1 = o0 + out->nbytes();
+  for (const at::Tensor& t : reads) {
+    const char* t0 = static_cast<const char*>(t.data_ptr());
+    const char* t1 = t0 + t.nbytes();
+    TORCH_CHECK(t0 == o0 || t1 <= o0 || o1 <= t0, "out overlaps an input at another offset");
+  }
+  return *out;
+}
+
+void check_index(const at::Tensor& index, const at::Tensor& x) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.scalar_type() == at::kHalf,
+              "x: a CUDA tensor (R,K) fp16 expected");
+  check_int32(index, x, x.size(0), "index");
+}
+
+at::Tensor adapter_add(const at::Tensor& x_in, const at::Tensor& index, const at::Tensor& a,
+                       const at::Tensor& b, const OptTensor& scale, const at::Tensor& base_in,
+                       const OptTensor& out_in, const OptTensor& err) {
+  check_index(index, x_in);
+  const Bank k = check_bank(a, b, scale, x_in);
+  check_rows(base_in, x_in, k.N, "base");
+  c10::cuda::CUDAGuard g(x_in.device());
+  const at::Tensor x = rows16(x_in, at::kHalf), base = rows16(base_in, at::kHalf);
+  at::Tensor out = result_rows(out_in, x, k.N, {base});
+  const int64_t R = x.size(0);
+  auto ws = workspace(lr_adapter_workspace_bytes(int(R), int(k.r), 1), x);
+  check_status(lr_adapter_add(x.data_ptr(), int(R), int(k.K), index.data_ptr<int32_t>(), int(k.n),
+                              k.a, k.b, k.scale, int(k.r), int(k.N), base.data_ptr(),
+                              out.data_ptr(), ws.data_ptr(), size_t(ws.numel()), err_ptr(err),
+                              cur_stream()),
+               "adapter_add");
+  return out;
+}
+
+at::Tensor adapter_swiglu(const at::Tensor& x_in, const at::Tensor& index, const at::Tensor& a_gate,
+                          const at::Tensor& b_gate, const OptTensor& scale_gate,
+                          const at::Tensor& a_up, const at::Tensor& b_up,
+                          const OptTensor& scale_up, const at::Tensor& gate_in,
+                          const at::Tensor& up_in, const OptTensor& out_in, const OptTensor& err) {
+  check_index(index, x_in);
+  const Bank kg = check_bank(a_gate, b_gate, scale_gate, x_in);
+  const Bank ku = check_bank(a_up, b_up, scale_up, x_in);
+  TORCH_CHECK(kg.n == ku.n && kg.r == ku.r && kg.N == ku.N,
+              "adapter_swiglu: the gate and up banks differ in size");
+  check_rows(gate_in, x_in, kg.N, "gate");
+  check_rows(up_in, x_in, kg.N, "up");
+  c10::cuda::CUDAGuard g(x_in.device());
+  const at::Tensor x = rows16(x_in, at::kHalf), gate = rows16(gate_in, at::kHalf),
+                   up = rows16(up_in, at::kHalf);
+  at::Tensor out = result_rows(out_in, x, kg.N, {gate, up});
+  const int64_t R = x.size(0);
+  auto ws = workspace(lr_adapter_workspace_bytes(int(R), int(kg.r), 2), x);
+  check_status(lr_adapter_swiglu(x.data_ptr(), int(R), int(kg.K), index.data_ptr<int32_t>(),
+                                 int(kg.n), kg.a, kg.b, kg.scale, ku.a, ku.b, ku.scale, int(kg.r),
+                                 int(kg.N), gate.data_ptr(), up.data_ptr(), out.data_ptr(),
+                                 ws.data_ptr(), size_t(ws.numel()), err_ptr(err), cur_stream()),
+               "adapter_swiglu");
+  return out;
+}
+
+at::Tensor adapter_rows(const at::Tensor& adapter_ids, const at::Tensor& source_idx,
+                        const at::Tensor& offsets, const at::Tensor& kept, int64_t num_adapters,
+                        const OptTensor& err) {
+  check_cuda(adapter_ids, "adapter_ids");
+  check_int32(adapter_ids, adapter_ids, adapter_ids.numel(), "adapter_ids");
+  const int64_t S = source_idx.numel(), E = kept.numel();
+  check_int32(source_idx, adapter_ids, S, "source_indices");
+  check_int32(kept, adapter_ids, E, "kept_counts");
+  check_int32(offsets, adapter_ids, E + 1, "offsets");
+  c10::cuda::CUDAGuard g(adapter_ids.device());
+  auto index = at::empty({S}, adapter_ids.options());
+  check_status(lr_adapter_rows(adapter_ids.data_ptr<int32_t>(), int(adapter_ids.numel()),
+                               int(num_adapters), source_idx.data_ptr<int32_t>(),
+                               offsets.data_ptr<int32_t>(), kept.data_ptr<int32_t>(), int(S),
+                               int(E), index.data_ptr<int32_t>(), err_ptr(err), cur_stream()),
+               "adapter_rows");
+  return index;
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(lightning_router, m) {
+  m.def("balanced_gating(Tensor logits, Tensor? token_mask, int k, float lbw) -> Tensor[]");
+  m.def("gate_projection(Tensor hidden, Tensor gate_weight, Tensor? bias) -> Tensor");
+  m.def(
+      "dispatch_tokens(Tensor x, Tensor logits, int k, int capacity, float lbw, Tensor? err) -> "
+      "Tensor[]");
+  m.def(
+      "combine_tokens(Tensor y, Tensor gate_weights, Tensor slot_pos, Tensor offsets, Tensor "
+      "kept_counts, int k) -> Tensor");
+  m.def(
+      "adapter_add(Tensor x, Tensor index, Tensor a, Tensor b, Tensor? scale, Tensor base, "
+      "Tensor? out, Tensor? err) -> Tensor");
+  m.def(
+      "adapter_swiglu(Tensor x, Tensor index, Tensor a_gate, Tensor b_gate, Tensor? scale_gate, "
+      "Tensor a_up, Tensor b_up, Tensor? scale_up, Tensor gate, Tensor up, Tensor? out, "
+      "Tensor? err) -> Tensor");
+  m.def(
+      "adapter_rows(Tensor adapter_ids, Tensor source_idx, Tensor offsets, Tensor kept_counts, "
+      "int num_adapters, Tensor? err) -> Tensor");
+}
+
+// The same functions below autograd (inference mode): apply() then records nothing.
+TORCH_LIBRARY_IMPL(lightning_router, CUDA, m) {
+  m.impl("balanced_gating", &balanced_gating);
+  m.impl("gate_projection", &gate_projection);
+  m.impl("dispatch_tokens", &dispatch_tokens);
+  m.impl("combine_tokens", &combine_tokens);
+  m.impl("adapter_add", &adapter_add);
+  m.impl("adapter_swiglu", &adapter_swiglu);
+  m.impl("adapter_rows", &adapter_rows);
+}
+
+TORCH_LIBRARY_IMPL(lightning_router, AutogradCUDA, m) {
+  m.impl("balanced_gating", &balanced_gating);
+  m.impl("gate_projection", &gate_projection);
+  m.impl("dispatch_tokens", &dispatch_tokens);
+  m.impl("combine_tokens", &combine_tokens);
+}

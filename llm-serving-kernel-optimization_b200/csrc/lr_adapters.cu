@@ -1,0 +1,601 @@
+// lr_adapters.cu -- low-rank adapters of many requests beside a shared projection (sm_100a).
+//
+// Row t of x carries an adapter number a = index[t] (-1: none):
+//   out_t = base_t + s_a (x_t A_a^T) B_a^T
+// or, beside a SwiGLU expert's two projections,
+//   out_t = silu(gate_t + D_gate) * (up_t + D_up).
+// Two launches: `shrink` writes v = x A^T (rank values per row, fp32), `expand`
+// adds v B^T to the base rows.  Rows are taken in windows of neighbours; a
+// window's rows are grouped by adapter inside the block (no sort of the batch,
+// no host involvement), and the block's 8 warps are dealt out to its groups:
+// one group (a prompt's rows) gets all warps, eight groups (decode) a warp each.
+// Work is bound by memory: a row costs 2 (K + 2N) bytes and 2 r (K + N)
+// operations, so mma.sync with fragments loaded straight into registers keeps
+// up and needs no staging through shared memory.
+#include "lr_common.cuh"
+
+namespace lr {
+
+constexpr int kAdWarps = 8;
+constexpr int kAdThreads = kAdWarps * 32;
+constexpr int kMaxRank = 128;
+
+LR_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                       uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+LR_DEVICE uint32_t cluster_ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+LR_DEVICE uint32_t cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+LR_DEVICE void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
+               ::: "memory");
+}
+LR_DEVICE float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+// Plain 16-byte read that leaves L1 alone (rows read once; may be written in place later).
+LR_DEVICE uint4 ld_row(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// a window's groups
+// ---------------------------------------------------------------------------
+struct Groups {
+  int32_t adapter[64];  // per row: its adapter, -1 none, -2 past the last row
+  int32_t group[64];    // per row: its group, -1 for no group
+  int32_t first[64];    // per group: its first row
+  int n;
+};
+
+// Warp 0 groups the W <= 64 rows from row0 by adapter.  Rows without one make
+// a group of their own when `with_none`.  The caller synchronises the block.
+template <int W>
+LR_DEVICE void group_rows(Groups& s, const int32_t* __restrict__ index, long row0, long R, int n,
+                          bool with_none, int32_t* err) {
+  const int lane = threadIdx.x & 31;
+  int a[2], lead[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = u * 32 + lane;
+    a[u] = -2;
+    if (t < W && row0 + t < R) {
+      a[u] = __ldg(index + row0 + t);
+      if (a[u] < -1 || a[u] >= n) {
+        report(err, LR_DEVERR_BAD_ADAPTER);
+        a[u] = -1;
+      }
+    }
+    const unsigned peers = __match_any_sync(0xffffffffu, a[u]);
+    lead[u] = u * 32 + __ffs(peers) - 1;
+  }
+  const int lowest = with_none ? -1 : 0;
+  unsigned la = __ballot_sync(0xffffffffu, lead[0] == lane && a[0] >= lowest);
+  if (W > 32) {  // a group of the upper rows may have started in the lower ones
+    for (unsigned m = la; m; m &= m - 1) {
+      const int r = __ffs(m) - 1;
+      const int ar = __shfl_sync(0xffffffffu, a[0], r);
+      if (a[1] == ar) lead[1] = r;
+    }
+  }
+  const unsigned lb = __ballot_sync(0xffffffffu, W > 32 && lead[1] == 32 + lane && a[1] >= lowest);
+  const unsigned long long leaders = la | (static_cast<unsigned long long>(lb) << 32);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = u * 32 + lane;
+    if (t < W) {
+      const int slot = __popcll(leaders & ((1ull << lead[u]) - 1));
+      s.adapter[t] = a[u];
+      s.group[t] = a[u] >= lowest ? slot : -1;
+      if (a[u] >= lowest && lead[u] == t) s.first[slot] = t;
+    }
+  }
+  if (lane == 0) s.n = __popcll(leaders);
+}
+
+// Warps per group (a power of two) when g groups share the block's warps.
+LR_DEVICE int warps_per_group(int g) { return g <= 1 ? 8 : g <= 2 ? 4 : g <= 4 ? 2 : 1; }
+
+// ---------------------------------------------------------------------------
+// shrink: v[row][r] = x[row] . A_a^T
+// ---------------------------------------------------------------------------
+// mma m16n8k16 with the rank as M (RB blocks of 16) and the window's rows as N
+// (NT tiles of 8).  A lane's 16-byte loads hold 8 neighbouring k of a row; the
+// k axis of the product is taken in that order for both operands, so 32 k are
+// two mma steps with no shuffle.  K is split over the cluster's blocks and over
+// the warps of a group; the parts are added in a fixed order through
+// (distributed) shared memory.
+struct ShrinkArgs {
+  const __half* x;
+  const __half* a[2];
+  const int32_t* index;
+  float* v;  // [bank][R][r]
+  long R;
+  int K, n, r;
+  int32_t* err;
+};
+
+template <int RB, int NT>
+__global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p, int rank_groups) {
+  constexpr int W = 8 * NT;
+  constexpr int RK = 16 * RB;
+  constexpr int PITCH = W + 2;
+  extern __shared__ float s_part[];  // [kAdWarps][RK][PITCH]
+  __shared__ Groups s;
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const int cs = int(cluster_nctarank()), cr = int(cluster_ctarank());
+  const long row0 = long(blockIdx.x / cs) * W;
+  const int bank = blockIdx.y / rank_groups, rank0 = (blockIdx.y % rank_groups) * RK;
+  if (warp == 0) group_rows<W>(s, p.index, row0, p.R, p.n, false, bank == 0 ? p.err : nullptr);
+  __syncthreads();
+  const int nb = (p.K + 31) / 32;
+  for (int base = 0; base < s.n; base += kAdWarps) {
+    const int ng = min(kAdWarps, s.n - base);
+    const int wpg = warps_per_group(ng);
+    const int grp = warp / wpg, sub = warp % wpg;
+    float acc[RB][NT][4];
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+    if (grp < ng) {
+      const int slot = base + grp;
+      const int ad = s.adapter[s.first[slot]];
+      const __half* ap = (bank ? p.a[1] : p.a[0]) + size_t(ad) * p.r * p.K;
+      const __half* arow[2 * RB];
+      bool aok[2 * RB];
+#pragma unroll
+      for (int i = 0; i < 2 * RB; ++i) {
+        const int rk = rank0 + i * 8 + g;
+        aok[i] = rk < p.r;
+        arow[i] = ap + size_t(aok[i] ? rk : 0) * p.K + tq * 8;
+      }
+      bool xok[NT], any[NT];
+      const __half* xrow = p.x + size_t(row0 + g) * p.K + tq * 8;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        xok[j] = s.group[j * 8 + g] == slot;
+        any[j] = __any_sync(0xffffffffu, xok[j]);
+      }
+      const int part = cr * wpg + sub, parts = cs * wpg;
+      const int kb0 = int(long(nb) * part / parts), kb1 = int(long(nb) * (part + 1) / parts);
+#pragma unroll(RB * NT == 1 ? 4 : NT == 1 ? 2 : 1)
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const int k = kb * 32;
+        const bool kok = k + tq * 8 < p.K;
+        uint4 av[2 * RB], xv[NT];
+#pragma unroll
+        for (int i = 0; i < 2 * RB; ++i) {
+          av[i] = make_uint4(0, 0, 0, 0);
+          if (aok[i] && kok) av[i] = __ldg(reinterpret_cast<const uint4*>(arow[i] + k));
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          xv[j] = make_uint4(0, 0, 0, 0);
+          if (xok[j] && kok)
+            xv[j] = ld_row(reinterpret_cast<const uint4*>(xrow + size_t(j) * 8 * p.K + k));
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          if (any[j]) {
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+              mma_f16(acc[i][j], av[2 * i].x, av[2 * i + 1].x, av[2 * i].y, av[2 * i + 1].y,
+                      xv[j].x, xv[j].y);
+              mma_f16(acc[i][j], av[2 * i].z, av[2 * i + 1].z, av[2 * i].w, av[2 * i + 1].w,
+                      xv[j].z, xv[j].w);
+            }
+          }
+        }
+      }
+    }
+    float* mine = s_part + size_t(warp) * RK * PITCH;
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<float2*>(mine + (i * 16 + g + 8 * c) * PITCH + j * 8 + 2 * tq) =
+              make_float2(acc[i][j][2 * c], acc[i][j][2 * c + 1]);
+    cluster_sync();
+    for (int o = cr * kAdThreads + threadIdx.x; o < W * RK; o += cs * kAdThreads) {
+      const int t = o / RK, i = o % RK;
+      const int gt = s.group[t] - base;
+      if (gt >= 0 && gt < ng && rank0 + i < p.r) {
+        float sum = 0.f;
+        for (int c = 0; c < cs; ++c)
+          for (int u = 0; u < wpg; ++u)
+            sum += ld_cluster_f32(smem_u32(s_part + (size_t(gt * wpg + u) * RK + i) * PITCH + t), c);
+        p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
+      }
+    }
+    cluster_sync();  // the parts stay until every block of the cluster has read them
+  }
+}
+
+// ---------------------------------------------------------------------------
+// expand: out[row] = base[row] + s_a v[row] . B_a^T   (or the SwiGLU of two)
+// ---------------------------------------------------------------------------
+// mma m16n8k16 with the window's rows as M (MT tiles of 16) and output columns
+// as N.  v enters as two fp16 terms of the row scaled by a power of two to
+// [2^14, 2^15) (value and remainder: 2^-22 of the row's largest, no overflow),
+// so v is not rounded to fp16.  n-tile j, column c stands for output column
+// (c >> 1) * 8 + 2 j + (c & 1) of the warp's 32: a lane ends with 8 neighbouring
+// columns of its two rows, one 16-byte load of the base and one store each.
+struct ExpandArgs {
+  const float* v;       // [bank][R][r]
+  const __half* b[2];
+  const float* scale[2];
+  const int32_t* index;
+  const __half* base[2];  // the base rows; gate and up rows for SwiGLU
+  __half* out;
+  long R;
+  int N, n, r;
+  int groups_per_chunk;  // 32-column groups of a block
+  bool in_place;
+};
+
+template <int MT, bool SWIGLU>
+__global__ void __launch_bounds__(kAdThreads) adapter_expand_kernel(ExpandArgs p) {
+  constexpr int W = 16 * MT;
+  constexpr int BANKS = SWIGLU ? 2 : 1;
+  extern __shared__ __align__(16) unsigned char s_dyn[];  // [bank][hi, lo][W][pitch] fp16
+  __shared__ Groups s;
+  __shared__ float s_fac[BANKS][W];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const long row0 = long(blockIdx.x) * W;
+  const int r32 = (p.r + 31) & ~31;
+  const int pitch = r32 + 8;
+  __half* s_v = reinterpret_cast<__half*>(s_dyn);
+  if (warp == 0) group_rows<W>(s, p.index, row0, p.R, p.n, !p.in_place, nullptr);
+  __syncthreads();
+  {  // v: fp32 -> scaled (value, remainder) pairs
+    constexpr int LPR = kAdThreads / W;  // lanes per row (4 or 16)
+    const int t = threadIdx.x / LPR, q = threadIdx.x % LPR;
+    const int ad = s.adapter[t];
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk) {
+      const float* row = p.v + (size_t(bk) * p.R + row0 + t) * p.r;
+      float m = 0.f;
+      if (ad >= 0)
+        for (int i = q; i < p.r; i += LPR) m = fmaxf(m, fabsf(__ldcg(row + i)));
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      int ex = 0;
+      if (m > 0.f && m < INFINITY) ex = max(-100, min(100, 14 - ilogbf(m)));
+      __half* hi = s_v + size_t(2 * bk) * W * pitch + size_t(t) * pitch;
+      __half* lo = hi + size_t(W) * pitch;
+      for (int i = q; i < r32; i += LPR) {
+        const float val = (ad >= 0 && i < p.r) ? ldexpf(__ldcg(row + i), ex) : 0.f;
+        const __half h = __float2half_rn(val);
+        const float hf = __half2float(h);
+        hi[i] = h;
+        lo[i] = __float2half_rn(fabsf(hf) < INFINITY ? val - hf : 0.f);
+      }
+      if (q == 0)
+        s_fac[bk][t] =
+            ad >= 0 ? ldexpf(p.scale[bk] ? __ldg(p.scale[bk] + ad) : 1.f, -ex) : 0.f;
+    }
+  }
+  __syncthreads();
+  const int cg0 = blockIdx.y * p.groups_per_chunk;
+  const int cg1 = min(cg0 + p.groups_per_chunk, (p.N + 31) / 32);
+  for (int base = 0; base < s.n; base += kAdWarps) {
+    const int ng = min(kAdWarps, s.n - base);
+    const int wpg = warps_per_group(ng);
+    const int grp = warp / wpg, sub = warp % wpg;
+    if (grp >= ng) continue;
+    const int slot = base + grp;
+    const int ad = s.adapter[s.first[slot]];
+    unsigned rows_ok = 0, tiles = 0;  // this lane's member rows, the warp's used m-tiles
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (s.group[m * 16 + g + 8 * h] == slot) rows_ok |= 1u << (2 * m + h);
+      if (__any_sync(0xffffffffu, (rows_ok >> (2 * m)) & 3u)) tiles |= 1u << m;
+    }
+    for (int cg = cg0 + sub; cg < cg1; cg += wpg) {
+      const int n0 = cg * 32;
+      const int nc = n0 + tq * 8;
+      uint4 bs[BANKS][MT][2];
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (((rows_ok >> (2 * m + h)) & 1u) && nc < p.N)
+              bs[bk][m][h] = ld_row(reinterpret_cast<const uint4*>(
+                  p.base[bk] + size_t(row0 + m * 16 + g + 8 * h) * p.N + nc));
+      float acc[BANKS][MT][4][4];
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[bk][m][j][c] = 0.f;
+      if (ad >= 0) {
+#pragma unroll
+        for (int bk = 0; bk < BANKS; ++bk) {
+          const int nr = n0 + (g >> 1) * 8 + (g & 1);
+          const __half* bp = p.b[bk] + (size_t(ad) * p.N + nr) * p.r + tq * 8;
+          const bool nok = n0 + (g >> 1) * 8 < p.N;
+          const __half* vp = s_v + size_t(2 * bk) * W * pitch + tq * 8;
+          for (int rk = 0; rk < p.r; rk += 32) {
+            uint4 bv[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              bv[j] = make_uint4(0, 0, 0, 0);
+              if (nok && rk + tq * 8 < p.r)
+                bv[j] = __ldg(reinterpret_cast<const uint4*>(bp + size_t(2 * j) * p.r + rk));
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              if ((tiles >> m) & 1u) {
+#pragma unroll
+                for (int term = 0; term < 2; ++term) {
+                  const __half* vr = vp + size_t(term) * W * pitch + size_t(m * 16 + g) * pitch + rk;
+                  const uint4 a0 = *reinterpret_cast<const uint4*>(vr);
+                  const uint4 a1 = *reinterpret_cast<const uint4*>(vr + size_t(8) * pitch);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    mma_f16(acc[bk][m][j], a0.x, a1.x, a0.y, a1.y, bv[j].x, bv[j].y);
+                    mma_f16(acc[bk][m][j], a0.z, a1.z, a0.w, a1.w, bv[j].z, bv[j].w);
+                  }
+                }
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!((rows_ok >> (2 * m + h)) & 1u) || nc >= p.N) continue;
+          const int t = m * 16 + g + 8 * h;
+          float o[BANKS][8];
+#pragma unroll
+          for (int bk = 0; bk < BANKS; ++bk) {
+            const __half2* bh = reinterpret_cast<const __half2*>(&bs[bk][m][h]);
+            const float f = s_fac[bk][t];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float2 b2 = __half22float2(bh[j]);
+              o[bk][2 * j] = ad >= 0 ? fmaf(acc[bk][m][j][2 * h], f, b2.x) : b2.x;
+              o[bk][2 * j + 1] = ad >= 0 ? fmaf(acc[bk][m][j][2 * h + 1], f, b2.y) : b2.y;
+            }
+          }
+          if (SWIGLU) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[0][i] = silu_f32(o[0][i]) * o[BANKS - 1][i];
+          }
+          *reinterpret_cast<uint4*>(p.out + size_t(row0 + t) * p.N + nc) = pack_half8(o[0]);
+        }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// adapter numbers of the expert rows
+// ---------------------------------------------------------------------------
+// Row r of expert e's segment from token t uses the bank's entry adapter[t] * E + e;
+// rows past the segment's kept slots and tokens without an adapter get -1.
+__global__ void __launch_bounds__(256)
+    adapter_rows_kernel(const int32_t* __restrict__ adapter, int T, int n,
+                        const int32_t* __restrict__ source_idx,
+                        const int32_t* __restrict__ offsets,
+                        const int32_t* __restrict__ kept_counts, long S, int E,
+                        int32_t* __restrict__ index, int32_t* err) {
+  pdl_wait();
+  pdl_trigger();
+  const long r = long(blockIdx.x) * 256 + threadIdx.x;
+  if (r >= S) return;
+  int lo = 0, hi = E;  // the last e with offsets[e] <= r
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(offsets + mid) <= r) lo = mid; else hi = mid;
+  }
+  int out = -1;
+  if (r < long(__ldg(offsets + lo)) + __ldg(kept_counts + lo)) {
+    const int t = __ldg(source_idx + r);
+    if (t < 0 || t >= T) {
+      report(err, LR_DEVERR_BAD_TOKEN);
+    } else {
+      const int a = __ldg(adapter + t);
+      if (a < -1 || a >= n)
+        report(err, LR_DEVERR_BAD_ADAPTER);
+      else if (a >= 0)
+        out = a * E + lo;
+    }
+  }
+  index[r] = out;
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Launch with a cluster of `cluster` blocks along x, programmatic as launch_pdl.
+template <typename... KArgs, typename... Args>
+static int launch_cluster(void (*kern)(KArgs...), dim3 grid, unsigned cluster, size_t smem,
+                          cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kAdThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &cs) != cudaSuccess) cs = cudaStreamCaptureStatusNone;
+  cfg.numAttrs = cs == cudaStreamCaptureStatusNone ? 2 : 1;
+  LR_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
+  return 0;
+}
+
+constexpr long kSmallRows = 256;  // up to here windows of 8 (shrink) and 16 rows (expand)
+constexpr long kTargetBlocks = 148;
+
+template <int RB, int NT>
+static int launch_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
+  constexpr int W = 8 * NT, RK = 16 * RB;
+  constexpr int smem = kAdWarps * RK * (W + 2) * int(sizeof(float));
+  auto kern = adapter_shrink_kernel<RB, NT>;
+  static unsigned long long configured = 0;
+  if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
+  const long windows = (p.R + W - 1) / W;
+  const int rank_groups = (p.r + RK - 1) / RK;
+  unsigned cs = 1;
+  while (cs < 8 && windows * rank_groups * banks * cs < kTargetBlocks) cs *= 2;
+  if (windows * cs > 0x7fffffffL) return LR_ERR_INVALID_ARGUMENT;
+  return launch_cluster(kern, dim3(unsigned(windows * cs), rank_groups * banks), cs, smem, stream,
+                        p, rank_groups);
+}
+
+template <int MT, bool SWIGLU>
+static int launch_expand(ExpandArgs p, cudaStream_t stream) {
+  constexpr int W = 16 * MT;
+  const int r32 = (p.r + 31) & ~31;
+  const int per = 2 * W * 2 * (SWIGLU ? 2 : 1);
+  auto kern = adapter_expand_kernel<MT, SWIGLU>;
+  static unsigned long long configured = 0;
+  if (const int rc = set_dyn_smem_once(kern, per * (kMaxRank + 8), configured)) return rc;
+  const long windows = (p.R + W - 1) / W;
+  const int cgs = (p.N + 31) / 32;
+  // 256 columns per block, more while the grid stays above eight blocks per SM
+  int gpc = 8;
+  while (gpc < 64 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
+  p.groups_per_chunk = gpc;
+  if (windows > 0x7fffffffL) return LR_ERR_INVALID_ARGUMENT;
+  return launch_pdl(kern, dim3(unsigned(windows), (cgs + gpc - 1) / gpc), dim3(kAdThreads),
+                    size_t(per) * (r32 + 8), stream, p);
+}
+
+static int run_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
+  const bool small = p.R <= kSmallRows;
+  if (p.r <= 16)
+    return small ? launch_shrink<1, 1>(p, banks, stream) : launch_shrink<1, 8>(p, banks, stream);
+  if (p.r <= 32)
+    return small ? launch_shrink<2, 1>(p, banks, stream) : launch_shrink<2, 8>(p, banks, stream);
+  return small ? launch_shrink<4, 1>(p, banks, stream) : launch_shrink<4, 8>(p, banks, stream);
+}
+
+static int check_adapter_args(const void* x, long R, int K, const int32_t* index, int n, int r,
+                              int N) {
+  if (R < 0 || R > 0x7fffffffL || K <= 0 || K % 8 != 0 || N <= 0 || N % 8 != 0 || n < 1 || r < 8 ||
+      r > kMaxRank || r % 8 != 0)
+    return LR_ERR_INVALID_ARGUMENT;
+  if (R > 0 && (!x || !index || !aligned16(x))) return LR_ERR_INVALID_ARGUMENT;
+  return LR_OK;
+}
+
+static bool bank_ok(const void* a, const void* b) { return a && b && aligned16(a) && aligned16(b); }
+
+}  // namespace lr
+
+// ===========================================================================
+// C ABI
+// ===========================================================================
+using namespace lr;
+
+extern "C" size_t lr_adapter_workspace_bytes(int num_rows, int rank, int num_banks) {
+  if (num_rows < 1 || rank < 1 || num_banks < 1) return 0;
+  return size_t(num_rows) * rank * num_banks * sizeof(float);
+}
+
+extern "C" int lr_adapter_add(const void* x, int R, int K, const int32_t* index, int num_adapters,
+                              const void* a, const void* b, const float* scale, int rank, int N,
+                              const void* base, void* out, void* workspace, size_t workspace_bytes,
+                              int32_t* err, lr_stream_t stream) {
+  if (const int rc = check_adapter_args(x, R, K, index, num_adapters, rank, N)) return rc;
+  if (R == 0) return LR_OK;
+  if (!bank_ok(a, b) || !base || !out || !aligned16(base) || !aligned16(out))
+    return LR_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < lr_adapter_workspace_bytes(R, rank, 1))
+    return LR_ERR_WORKSPACE;
+  ShrinkArgs sp{static_cast<const __half*>(x), {static_cast<const __half*>(a), nullptr}, index,
+                static_cast<float*>(workspace), R, K, num_adapters, rank, err};
+  if (const int rc = run_shrink(sp, 1, stream)) return rc;
+  ExpandArgs ep{sp.v, {static_cast<const __half*>(b), nullptr}, {scale, nullptr}, index,
+                {static_cast<const __half*>(base), nullptr}, static_cast<__half*>(out), R, N,
+                num_adapters, rank, 0, base == out};
+  return R <= kSmallRows ? launch_expand<1, false>(ep, stream) : launch_expand<4, false>(ep, stream);
+}
+
+extern "C" int lr_adapter_swiglu(const void* x, int R, int K, const int32_t* index,
+                                 int num_adapters, const void* a_gate, const void* b_gate,
+                                 const float* scale_gate, const void* a_up, const void* b_up,
+                                 const float* scale_up, int rank, int N, const void* gate,
+                                 const void* up, void* out, void* workspace,
+                                 size_t workspace_bytes, int32_t* err, lr_stream_t stream) {
+  if (const int rc = check_adapter_args(x, R, K, index, num_adapters, rank, N)) return rc;
+  if (R == 0) return LR_OK;
+  if (!bank_ok(a_gate, b_gate) || !bank_ok(a_up, b_up) || !gate || !up || !out ||
+      !aligned16(gate) || !aligned16(up) || !aligned16(out))
+    return LR_ERR_INVALID_ARGUMENT;
+  if (!workspace || workspace_bytes < lr_adapter_workspace_bytes(R, rank, 2))
+    return LR_ERR_WORKSPACE;
+  ShrinkArgs sp{static_cast<const __half*>(x),
+                {static_cast<const __half*>(a_gate), static_cast<const __half*>(a_up)}, index,
+                static_cast<float*>(workspace), R, K, num_adapters, rank, err};
+  if (const int rc = run_shrink(sp, 2, stream)) return rc;
+  ExpandArgs ep{sp.v, {static_cast<const __half*>(b_gate), static_cast<const __half*>(b_up)},
+                {scale_gate, scale_up}, index,
+                {static_cast<const __half*>(gate), static_cast<const __half*>(up)},
+                static_cast<__half*>(out), R, N, num_adapters, rank, 0, false};
+  return R <= kSmallRows ? launch_expand<1, true>(ep, stream) : launch_expand<2, true>(ep, stream);
+}
+
+extern "C" int lr_adapter_rows(const int32_t* adapter_ids, int T, int num_adapters,
+                               const int32_t* source_idx, const int32_t* offsets,
+                               const int32_t* kept_counts, int S, int E, int32_t* index,
+                               int32_t* err, lr_stream_t stream) {
+  if (T < 0 || S < 0 || E < 1 || num_adapters < 1 || long(num_adapters) * E > 0x7fffffffL)
+    return LR_ERR_INVALID_ARGUMENT;
+  if (S == 0) return LR_OK;
+  if (!adapter_ids || !source_idx || !offsets || !kept_counts || !index)
+    return LR_ERR_INVALID_ARGUMENT;
+  return launch_pdl(adapter_rows_kernel, dim3((unsigned(S) + 255) / 256), dim3(256), 0, stream,
+                    adapter_ids, T, num_adapters, source_idx, offsets, kept_counts, long(S), E,
+                    index, err);
+}

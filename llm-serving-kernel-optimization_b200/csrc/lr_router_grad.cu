@@ -1,0 +1,851 @@
+// lr_router_grad.cu -- the router's training path (sm_100a): top-k gating with
+// the balance loss and per-expert counts, and the gradients of the gate
+// projection, the dispatch and the weighted combine.
+//
+// With p = softmax(l_t), the selected set s_t (k largest logits, ties towards
+// the lowest expert), q = sum_{s_t} p + 1e-9, w_j = p_j / q, counts c_e and the
+// n live tokens:
+//   loss   = lbw * E * sum_e f_e P_e,  f_e = c_e / (n k),  P_e = sum_t p_te / n
+//   dp_e   = [e in s_t] (dw_e - sum_j dw_j w_j) / q  +  dloss * lbw * E * f_e / n
+//   dl_e   = p_e (dp_e - sum_i p_i dp_i)              (f is a constant, as in the loss)
+//   dW     = dl^T h,  dh = dl W,  db = sum_t dl
+//   dy_row = w dout_t,  dw = <dout_t, y_row>,  dx_t = sum_j dpermuted[row_j]
+#include "lr_common.cuh"
+
+namespace lr {
+
+// ---------------------------------------------------------------------------
+// top-k gating + balance loss + counts
+// ---------------------------------------------------------------------------
+// A token's logits are spread over LPT lanes, 8 per lane in two float4 pieces
+// (lane l holds experts c*4*LPT + 4l + r, c < 2, r < 4), so a warp reads whole
+// rows.  Selection is k rounds of a maximum over (ordered logit, lowest expert
+// first) keys.  Probability sums and counts stay in registers over a lane's
+// tokens, go through shuffles and shared memory to one partial per block and
+// expert, and are summed over blocks in double in block order: no atomics.
+constexpr int kGateThreads = 512;
+constexpr int kGateBlocksMax = 296;  // 2 per SM
+
+struct GatingParts {
+  double* psum;    // [E][B]
+  int32_t* count;  // [E + 1][B], row E: live tokens
+};
+
+// Larger key = larger logit, then lower expert; NaN below every number.
+LR_DEVICE unsigned long long select_key(float v, int e) {
+  uint32_t u = __float_as_uint(v + 0.f);  // -0 -> +0: they tie
+  u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  if (v != v) u = 0u;
+  return (static_cast<unsigned long long>(u) << 32) | (0xffffffffu - unsigned(e));
+}
+
+template <int LPT>
+LR_DEVICE float group_sum(float v) {
+#pragma unroll
+  for (int o = 1; o < LPT; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <int LPT>
+LR_DEVICE float group_max(float v) {
+#pragma unroll
+  for (int o = 1; o < LPT; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// This lane's 8 logits of row t (-inf past E) and their softmax.
+template <int LPT>
+LR_DEVICE void row_softmax(const float* __restrict__ logits, int t, bool valid, int E, bool vec,
+                           int l, float (&v)[8], float (&p)[8]) {
+  const float* row = logits + size_t(valid ? t : 0) * E;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int e0 = c * 4 * LPT + 4 * l;
+    if (vec) {
+      float4 q = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (valid && e0 < E) q = __ldg(reinterpret_cast<const float4*>(row + e0));
+      v[4 * c] = q.x;
+      v[4 * c + 1] = q.y;
+      v[4 * c + 2] = q.z;
+      v[4 * c + 3] = q.w;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        v[4 * c + r] = (valid && e0 + r < E) ? __ldg(row + e0 + r) : -INFINITY;
+    }
+  }
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
+  m = group_max<LPT>(m);
+  float z = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = (i >> 2) * 4 * LPT + 4 * l + (i & 3);
+    p[i] = e < E ? expf(v[i] - m) : 0.f;
+    z += p[i];
+  }
+  z = group_sum<LPT>(z);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] = p[i] / z;
+}
+
+// counts[0..E), counts[E] = live tokens, and the loss, from totals in double.
+LR_DEVICE void write_gating_stats(int E, int k, float lbw, const double* s_p, const int32_t* s_c,
+                                  int32_t* __restrict__ counts, float* __restrict__ aux) {
+  if (threadIdx.x == 0) {
+    const int n = s_c[E];
+    double a = 0.0;
+    for (int e = 0; e < E; ++e) {
+      counts[e] = s_c[e];
+      if (n > 0) a += (double(s_c[e]) / (double(n) * k)) * (s_p[e] / n);
+    }
+    counts[E] = n;
+    aux[0] = static_cast<float>(double(lbw) * E * a);
+  }
+}
+
+template <int LPT>
+__global__ void __launch_bounds__(kGateThreads)
+    balanced_gating_kernel(const float* __restrict__ logits, const uint8_t* __restrict__ mask,
+                           int T, int E, int k, float lbw, bool vec,
+                           int32_t* __restrict__ expert_ids, float* __restrict__ gate_w,
+                           int32_t* __restrict__ counts, float* __restrict__ aux,
+                           GatingParts parts) {
+  constexpr int kW = kGateThreads / 32;
+  __shared__ float s_p[kW][8 * LPT];
+  __shared__ int32_t s_c[kW][8 * LPT + 1];
+  __shared__ double s_tp[8 * LPT];
+  __shared__ int32_t s_tc[8 * LPT + 1];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int l = lane % LPT;
+  const int per_warp = 32 / LPT;
+  float psum[8];
+  int cnt[8];
+  int live_n = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    psum[i] = 0.f;
+    cnt[i] = 0;
+  }
+  const long stride = long(gridDim.x) * kW * per_warp;
+  for (long tb = (long(blockIdx.x) * kW + warp) * per_warp; tb < T; tb += stride) {
+    const int t = int(tb) + lane / LPT;
+    const bool valid = t < T;
+    const bool live = valid && (mask == nullptr || mask[t] != 0);
+    float v[8], p[8];
+    row_softmax<LPT>(logits, t, valid, E, vec, l, v, p);
+    unsigned taken = 0;  // this lane's selected experts
+    int ids[kMaxTopK];
+    float ps[kMaxTopK];
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < kMaxTopK; ++j) {
+      if (j < k) {
+        unsigned long long best = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int e = (i >> 2) * 4 * LPT + 4 * l + (i & 3);
+          const unsigned long long key = select_key(v[i], e);
+          if (e < E && !((taken >> i) & 1u) && key > best) best = key;
+        }
+#pragma unroll
+        for (int o = 1; o < LPT; o <<= 1) {
+          const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+          if (other > best) best = other;
+        }
+        const int e = int(0xffffffffu - unsigned(best));
+        const int owner = (e >> 2) % LPT, i = (e >> 2) / LPT * 4 + (e & 3);
+        if (owner == l) taken |= 1u << i;
+        float pe = 0.f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (x == i) pe = p[x];
+        pe = __shfl_sync(0xffffffffu, pe, (lane & ~(LPT - 1)) + owner);
+        ids[j] = e;
+        ps[j] = pe;
+        q += pe;
+      }
+    }
+    const float denom = q + 1e-9f;
+    if (valid) {
+#pragma unroll
+      for (int j = 0; j < kMaxTopK; ++j) {
+        if (j < k && j % LPT == l) {
+          const size_t s = size_t(t) * k + j;
+          expert_ids[s] = ids[j];
+          gate_w[s] = live ? ps[j] / denom : 0.f;
+        }
+      }
+    }
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        psum[i] += p[i];
+        cnt[i] += (taken >> i) & 1u;
+      }
+      live_n += l == 0;
+    }
+  }
+  // lanes with the same experts, then warps, then blocks
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int o = LPT; o < 32; o <<= 1) {
+      psum[i] += __shfl_xor_sync(0xffffffffu, psum[i], o);
+      cnt[i] += __shfl_xor_sync(0xffffffffu, cnt[i], o);
+    }
+    if (lane < LPT) {
+      const int e = (i >> 2) * 4 * LPT + 4 * l + (i & 3);
+      s_p[warp][e] = psum[i];
+      s_c[warp][e] = cnt[i];
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) live_n += __shfl_xor_sync(0xffffffffu, live_n, o);
+  if (lane == 0) s_c[warp][8 * LPT] = live_n;
+  __syncthreads();
+  for (int e = threadIdx.x; e <= 8 * LPT; e += kGateThreads) {
+    double ps = 0.0;
+    int c = 0;
+    for (int w = 0; w < kW; ++w) {
+      if (e < 8 * LPT) ps += double(s_p[w][e]);
+      c += s_c[w][e];
+    }
+    const int row = e == 8 * LPT ? E : e;  // the live count moves up to row E
+    if (gridDim.x == 1) {
+      if (e < E) s_tp[e] = ps;
+      if (e < E || e == 8 * LPT) s_tc[row] = c;
+    } else if (e < E || e == 8 * LPT) {
+      if (e < E) parts.psum[size_t(e) * gridDim.x + blockIdx.x] = ps;
+      parts.count[size_t(row) * gridDim.x + blockIdx.x] = c;
+    }
+  }
+  if (gridDim.x > 1) return;
+  __syncthreads();
+  write_gating_stats(E, k, lbw, s_tp, s_tc, counts, aux);
+}
+
+// One block: totals over the B blocks' partials, a warp per expert.
+__global__ void __launch_bounds__(1024)
+    gating_stats_kernel(GatingParts parts, int B, int E, int k, float lbw,
+                        int32_t* __restrict__ counts, float* __restrict__ aux) {
+  __shared__ double s_tp[64];
+  __shared__ int32_t s_tc[65];
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  for (int e = threadIdx.x >> 5; e <= E; e += 32) {
+    double ps = 0.0;
+    int c = 0;
+    for (int b = lane; b < B; b += 32) {
+      if (e < E) ps += parts.psum[size_t(e) * B + b];
+      c += parts.count[size_t(e) * B + b];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ps += __shfl_xor_sync(0xffffffffu, ps, o);
+      c += __shfl_xor_sync(0xffffffffu, c, o);
+    }
+    if (lane == 0) {
+      if (e < E) s_tp[e] = ps;
+      s_tc[e] = c;
+    }
+  }
+  __syncthreads();
+  write_gating_stats(E, k, lbw, s_tp, s_tc, counts, aux);
+}
+
+// The gradient in the logits: the softmax is taken again from the logits (one
+// read, nothing kept from the forward but the ids), one launch, no reductions
+// across tokens.  With `csr` the counts are the differences of CSR offsets and
+// every token is live.
+template <int LPT>
+__global__ void __launch_bounds__(kGateThreads)
+    balanced_gating_backward_kernel(const float* __restrict__ logits,
+                                    const uint8_t* __restrict__ mask,
+                                    const int32_t* __restrict__ expert_ids,
+                                    const int32_t* __restrict__ counts, int csr,
+                                    const float* __restrict__ d_w, const float* __restrict__ d_aux,
+                                    int T, int E, int k, float lbw, bool vec,
+                                    float* __restrict__ d_logits) {
+  constexpr int kW = kGateThreads / 32;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int l = lane % LPT;
+  const int per_warp = 32 / LPT;
+  const int n = csr ? T : counts[E];
+  float bal[8];  // the loss' gradient in p_e
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = (i >> 2) * 4 * LPT + 4 * l + (i & 3);
+    bal[i] = 0.f;
+    if (d_aux && e < E && n > 0) {
+      const int c = csr ? counts[e + 1] - counts[e] : counts[e];
+      bal[i] = d_aux[0] * float(double(lbw) * E * (double(c) / (double(n) * k)) / n);
+    }
+  }
+  const long stride = long(gridDim.x) * kW * per_warp;
+  for (long tb = (long(blockIdx.x) * kW + warp) * per_warp; tb < T; tb += stride) {
+    const int t = int(tb) + lane / LPT;
+    const bool valid = t < T;
+    const bool live = valid && (mask == nullptr || mask[t] != 0);
+    float v[8], p[8], dw[8];
+    row_softmax<LPT>(logits, t, valid, E, vec, l, v, p);
+    unsigned taken = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dw[i] = 0.f;
+    if (d_w && valid) {
+#pragma unroll
+      for (int j = 0; j < kMaxTopK; ++j) {
+        if (j < k) {
+          const size_t s = size_t(t) * k + j;
+          const int e = __ldg(expert_ids + s);
+          const float g = __ldg(d_w + s);
+          if ((e >> 2) % LPT == l) {
+            const int i = (e >> 2) / LPT * 4 + (e & 3);
+            taken |= 1u << i;
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              if (x == i) dw[x] = g;
+          }
+        }
+      }
+    }
+    float q = 0.f, c = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if ((taken >> i) & 1u) {
+        q += p[i];
+        c = fmaf(dw[i], p[i], c);
+      }
+    }
+    q = group_sum<LPT>(q) + 1e-9f;
+    c = group_sum<LPT>(c) / q;
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      dw[i] = bal[i] + (((taken >> i) & 1u) ? (dw[i] - c) / q : 0.f);
+      dot = fmaf(p[i], dw[i], dot);
+    }
+    dot = group_sum<LPT>(dot);
+    if (!valid) continue;  // the loop bound is the same for the whole warp
+    float* row = d_logits + size_t(t) * E;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e0 = h * 4 * LPT + 4 * l;
+      float g[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) g[r] = live ? p[4 * h + r] * (dw[4 * h + r] - dot) : 0.f;
+      if (vec) {
+        if (e0 < E) *reinterpret_cast<float4*>(row + e0) = make_float4(g[0], g[1], g[2], g[3]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (e0 + r < E) row[e0 + r] = g[r];
+      }
+    }
+  }
+}
+
+static int gating_blocks(int T, int E) {
+  const int lpt = E <= 8 ? 1 : E <= 16 ? 2 : E <= 32 ? 4 : 8;
+  const long per_block = kGateThreads / lpt;
+  const long b = (T + per_block - 1) / per_block;
+  return int(b < 1 ? 1 : b > kGateBlocksMax ? kGateBlocksMax : b);
+}
+
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+
+// ---------------------------------------------------------------------------
+// gate projection: gradients
+// ---------------------------------------------------------------------------
+// fp32 gradients meet fp16 rows and weights on mma.sync m16n8k8 tf32: an fp16
+// value is a tf32 value, and the fp32 one goes in as two tf32 terms (rounded,
+// and rounded remainder: 2^-22 relative), so no rounding beyond fp32's is added.
+LR_DEVICE void split_tf32(float v, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
+  const float h = __uint_as_float(hi);
+  const float r = fabsf(h) < INFINITY ? v - h : 0.f;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
+}
+
+LR_DEVICE void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+LR_DEVICE void half8_bits(const uint4& v, uint32_t (&f)[8]) {
+  const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = __half22float2(h[i]);
+    f[2 * i] = __float_as_uint(x.x);
+    f[2 * i + 1] = __float_as_uint(x.y);
+  }
+}
+
+// dW[E,d] = dl^T h.  A block owns 64 columns of h and a token range that its 8
+// warps split; rows are the k axis.  A lane's 16-byte load holds 8 neighbouring
+// columns of one row; column g*8 + 2m (+1) is row g (g + 8) of m-tile m, so the
+// fragments need no shuffle.  A warp adds at most 256 rows in one accumulator
+// chain; warps are joined in shared memory, token ranges by a second launch,
+// both in a fixed order.
+constexpr int kDwWarps = 8;
+constexpr int kDwChain = 256;
+
+template <int ET>
+__global__ void __launch_bounds__(kDwWarps * 32)
+    gate_dw_kernel(const __half* __restrict__ h, const float* __restrict__ dl, int T, int d, int E,
+                   int tokens_per_warp, float* __restrict__ part, float* __restrict__ part_b) {
+  __shared__ float red[kDwWarps][8][65];
+  __shared__ float red_b[kDwWarps][8 * ET];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const int d0 = blockIdx.x * 64, e0 = blockIdx.z * 64;
+  const long tb = (long(blockIdx.y) * kDwWarps + warp) * tokens_per_warp;
+  const long te = min(long(T), tb + tokens_per_warp);
+  const bool dok = d0 + g * 8 < d;
+  float acc[4][ET][4];
+  float bsum[ET];
+#pragma unroll
+  for (int n = 0; n < ET; ++n) {
+    bsum[n] = 0.f;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+  }
+#pragma unroll 2
+  for (long t0 = tb; t0 < te; t0 += 8) {
+    uint32_t x[2][8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const long t = t0 + tq + 4 * u;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (t < te && dok) v = ld_stream(reinterpret_cast<const uint4*>(h + size_t(t) * d + d0 + g * 8));
+      half8_bits(v, x[u]);
+    }
+#pragma unroll
+    for (int n = 0; n < ET; ++n) {
+      if (e0 + n * 8 < E) {
+        const int e = e0 + n * 8 + g;
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const long t = t0 + tq + 4 * u;
+          const float v = (t < te && e < E) ? __ldg(dl + size_t(t) * E + e) : 0.f;
+          bsum[n] += v;
+          split_tf32(v, hi[u], lo[u]);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const uint32_t a[4] = {x[0][2 * m], x[0][2 * m + 1], x[1][2 * m], x[1][2 * m + 1]};
+          mma_tf32(acc[m][n], a, hi[0], hi[1]);
+          mma_tf32(acc[m][n], a, lo[0], lo[1]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < ET; ++n) {
+    if (e0 + n * 8 < E) {  // the same for the whole block
+      __syncthreads();
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          red[warp][2 * tq + (i & 1)][g * 8 + 2 * m + (i >> 1)] = acc[m][n][i];
+      __syncthreads();
+      for (int o = threadIdx.x; o < 8 * 64; o += kDwWarps * 32) {
+        const int r = o >> 6, c = o & 63;
+        const int e = e0 + n * 8 + r;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kDwWarps; ++w) s += red[w][r][c];
+        if (e < E && d0 + c < d) part[(size_t(blockIdx.y) * E + e) * d + d0 + c] = s;
+      }
+    }
+  }
+  if (part_b && blockIdx.x == 0) {
+#pragma unroll
+    for (int n = 0; n < ET; ++n) {
+      float s = bsum[n];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (tq == 0) red_b[warp][n * 8 + g] = s;
+    }
+    __syncthreads();
+    for (int o = threadIdx.x; o < 8 * ET; o += kDwWarps * 32) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kDwWarps; ++w) s += red_b[w][o];
+      if (e0 + o < E) part_b[size_t(blockIdx.y) * E + e0 + o] = s;
+    }
+  }
+}
+
+// out[i] = sum over the token ranges of part[s][i], in range order.
+__global__ void __launch_bounds__(256)
+    sum_parts_kernel(const float* __restrict__ part, long n, const float* __restrict__ part_b,
+                     int nb, int splits, float* __restrict__ out, float* __restrict__ out_b) {
+  pdl_wait();
+  pdl_trigger();
+  const long i = long(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) {
+    float s = 0.f;
+    for (int p = 0; p < splits; ++p) s += part[size_t(p) * n + i];
+    out[i] = s;
+  }
+  if (out_b && i < nb) {
+    float s = 0.f;
+    for (int p = 0; p < splits; ++p) s += part_b[size_t(p) * nb + i];
+    out_b[i] = s;
+  }
+}
+
+// dh[T,d] = dl W, fp16 out.  A warp owns MT*16 tokens x 64 columns; experts are
+// the k axis.  n-tile j takes column g*8 + j of the lane's 16-byte weight load,
+// so a lane ends with 16 neighbouring columns of its rows.
+template <int MT>
+__global__ void __launch_bounds__(256)
+    gate_dh_kernel(const float* __restrict__ dl, const __half* __restrict__ wg, int T, int d, int E,
+                   __half* __restrict__ dh) {
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const int t0 = blockIdx.x * (16 * MT);
+  const int d0 = (blockIdx.y * 8 + warp) * 64;
+  if (d0 >= d) return;
+  const bool dok = d0 + g * 8 < d;
+  float acc[MT][8][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
+  for (int e0 = 0; e0 < E; e0 += 8) {
+    uint32_t b[2][8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int e = e0 + tq + 4 * u;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (e < E && dok) v = __ldg(reinterpret_cast<const uint4*>(wg + size_t(e) * d + d0 + g * 8));
+      half8_bits(v, b[u]);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + m * 16 + g + 8 * (i & 1);
+        const int e = e0 + tq + 4 * (i >> 1);
+        split_tf32((t < T && e < E) ? __ldg(dl + size_t(t) * E + e) : 0.f, hi[i], lo[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        mma_tf32(acc[m][j], hi, b[0][j], b[1][j]);
+        mma_tf32(acc[m][j], lo, b[0][j], b[1][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int t = t0 + m * 16 + g + 8 * r;
+      if (t >= T) continue;
+#pragma unroll
+      for (int half_i = 0; half_i < 2; ++half_i) {  // columns (2tq) * 8 .. and (2tq + 1) * 8 ..
+        const int c = d0 + (2 * tq + half_i) * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = acc[m][j][2 * r + half_i];
+        if (c < d) *reinterpret_cast<uint4*>(dh + size_t(t) * d + c) = pack_half8(v);
+      }
+    }
+}
+
+struct DwPlan {
+  int tokens_per_warp, splits;
+};
+
+// Token ranges of the weight gradient: chains of at most kDwChain rows per warp,
+// shorter ones while the grid has fewer than two blocks per SM.
+static DwPlan dw_plan(int T, int d, int E) {
+  const long cols = long((d + 63) / 64) * ((E + 63) / 64);
+  int tpw = kDwChain;
+  while (tpw > 16 && cols * ((T + long(tpw) * kDwWarps - 1) / (long(tpw) * kDwWarps)) < 296)
+    tpw /= 2;
+  return {tpw, int((T + long(tpw) * kDwWarps - 1) / (long(tpw) * kDwWarps))};
+}
+
+// ---------------------------------------------------------------------------
+// weighted combine: gradients
+// ---------------------------------------------------------------------------
+// WPT warps share a token's row: the row of dout is read once, each kept slot's
+// y row once, dy written once; the dot products are summed over lanes and warps
+// in a fixed order.  Rows no slot keeps (the tail of an over-full expert's
+// segment) are zero-filled by the warps of the tokens with the same numbers.
+template <int WPT>
+__global__ void __launch_bounds__(256)
+    combine_backward_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ y,
+                            const float* __restrict__ gate_w, const int32_t* __restrict__ slot_pos,
+                            const int32_t* __restrict__ offsets,
+                            const int32_t* __restrict__ kept_counts, int E, int T, int k, int d8,
+                            uint4* __restrict__ dy, float* __restrict__ d_w) {
+  constexpr int kTok = 8 / WPT;
+  __shared__ float s_dot[8][kMaxTopK];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = warp % WPT;
+  const long t = long(blockIdx.x) * kTok + warp / WPT;
+  const bool valid = t < T;
+  int my_pos = -1;
+  float my_w = 0.f;
+  if (valid && lane < k) {
+    my_pos = __ldg(slot_pos + size_t(t) * k + lane);
+    my_w = __ldg(gate_w + size_t(t) * k + lane);
+  }
+  int pos[kMaxTopK];
+  float w[kMaxTopK], dot[kMaxTopK];
+#pragma unroll
+  for (int j = 0; j < kMaxTopK; ++j) {
+    pos[j] = __shfl_sync(0xffffffffu, my_pos, j);
+    w[j] = __shfl_sync(0xffffffffu, my_w, j);
+    dot[j] = 0.f;
+  }
+  if (valid) {
+    constexpr int U = 2;
+    for (int c0 = part * 32 * U; c0 < d8; c0 += WPT * 32 * U) {
+      uint4 g[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u * 32 + lane;
+        if (c < d8) g[u] = ld_stream(dout + size_t(t) * d8 + c);
+      }
+#pragma unroll
+      for (int j = 0; j < kMaxTopK; ++j) {
+        if (j < k && pos[j] >= 0) {
+          uint4 v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * 32 + lane;
+            if (c < d8) v[u] = ld_stream(y + size_t(pos[j]) * d8 + c);
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * 32 + lane;
+            if (c < d8) {
+              const __half2* gh = reinterpret_cast<const __half2*>(&g[u]);
+              const __half2* vh = reinterpret_cast<const __half2*>(&v[u]);
+              float o[8];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 a = __half22float2(gh[i]), b = __half22float2(vh[i]);
+                dot[j] = fmaf(a.x, b.x, dot[j]);
+                dot[j] = fmaf(a.y, b.y, dot[j]);
+                o[2 * i] = w[j] * a.x;
+                o[2 * i + 1] = w[j] * a.y;
+              }
+              dy[size_t(pos[j]) * d8 + c] = pack_half8(o);
+            }
+          }
+        }
+      }
+    }
+    // rows that no slot keeps
+    for (int j = 0; j < k; ++j) {
+      const long r = t * k + j;
+      bool drop = false;
+      for (int e = lane; e < E; e += 32)
+        drop = drop || (r >= long(__ldg(offsets + e)) + __ldg(kept_counts + e) &&
+                        r < __ldg(offsets + e + 1));
+      if (__any_sync(0xffffffffu, drop)) {
+        for (int c = part * 32 + lane; c < d8; c += WPT * 32)
+          dy[size_t(r) * d8 + c] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kMaxTopK; ++j) {
+    if (j < k) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+      if (lane == 0) s_dot[warp][j] = dot[j];
+    }
+  }
+  __syncthreads();
+  if (valid && part == 0 && lane < k) {
+    float s = 0.f;
+#pragma unroll
+    for (int p = 0; p < WPT; ++p) s += s_dot[warp + p][lane];
+    d_w[size_t(t) * k + lane] = s;
+  }
+}
+
+}  // namespace lr
+
+// ===========================================================================
+// C ABI
+// ===========================================================================
+using namespace lr;
+
+static bool gating_args_ok(int T, int E, int k) {
+  return T >= 0 && E >= 1 && E <= 64 && k >= 1 && k <= kMaxTopK && k <= E;
+}
+
+extern "C" size_t lr_balanced_gating_workspace_bytes(int num_tokens, int num_experts) {
+  if (num_tokens < 1 || num_experts < 1) return 0;
+  const size_t B = gating_blocks(num_tokens, num_experts);
+  if (B == 1) return 0;
+  return align256(B * num_experts * sizeof(double)) + B * (num_experts + 1) * sizeof(int32_t);
+}
+
+extern "C" int lr_balanced_gating(const float* logits, const uint8_t* token_mask, int T, int E,
+                                  int k, float load_balance_weight, int32_t* expert_ids,
+                                  float* gate_weights, int32_t* counts, float* aux_loss,
+                                  void* workspace, size_t workspace_bytes, lr_stream_t stream) {
+  if (!gating_args_ok(T, E, k) || !counts || !aux_loss) return LR_ERR_INVALID_ARGUMENT;
+  if (T == 0) {
+    LR_CUDA_TRY(cudaMemsetAsync(counts, 0, (E + 1) * sizeof(int32_t), stream));
+    LR_CUDA_TRY(cudaMemsetAsync(aux_loss, 0, sizeof(float), stream));
+    return LR_OK;
+  }
+  if (!logits || !expert_ids || !gate_weights) return LR_ERR_INVALID_ARGUMENT;
+  const int B = gating_blocks(T, E);
+  GatingParts parts{nullptr, nullptr};
+  if (B > 1) {
+    if (!workspace || workspace_bytes < lr_balanced_gating_workspace_bytes(T, E))
+      return LR_ERR_WORKSPACE;
+    parts.psum = static_cast<double*>(workspace);
+    parts.count = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) +
+                                             align256(size_t(B) * E * sizeof(double)));
+  }
+  const bool vec = E % 4 == 0 && aligned16(logits);
+  auto run = [&](auto kern) {
+    return launch_pdl(kern, dim3(B), dim3(kGateThreads), 0, stream, logits, token_mask, T, E, k,
+                      load_balance_weight, vec, expert_ids, gate_weights, counts, aux_loss, parts);
+  };
+  const int rc = E <= 8    ? run(balanced_gating_kernel<1>)
+                 : E <= 16 ? run(balanced_gating_kernel<2>)
+                 : E <= 32 ? run(balanced_gating_kernel<4>)
+                           : run(balanced_gating_kernel<8>);
+  if (rc != LR_OK || B == 1) return rc;
+  return launch_pdl(gating_stats_kernel, dim3(1), dim3(1024), 0, stream, parts, B, E, k,
+                    load_balance_weight, counts, aux_loss);
+}
+
+extern "C" int lr_balanced_gating_backward(const float* logits, const uint8_t* token_mask,
+                                           const int32_t* expert_ids, const int32_t* counts,
+                                           int counts_are_offsets, const float* d_weights,
+                                           const float* d_aux, int T, int E, int k,
+                                           float load_balance_weight, float* d_logits,
+                                           lr_stream_t stream) {
+  if (!gating_args_ok(T, E, k)) return LR_ERR_INVALID_ARGUMENT;
+  if (T == 0) return LR_OK;
+  if (!logits || !counts || !d_logits || (d_weights && !expert_ids))
+    return LR_ERR_INVALID_ARGUMENT;
+  if (counts_are_offsets && token_mask) return LR_ERR_INVALID_ARGUMENT;
+  const bool vec = E % 4 == 0 && aligned16(logits) && aligned16(d_logits);
+  const int B = gating_blocks(T, E);
+  auto run = [&](auto kern) {
+    return launch_pdl(kern, dim3(B), dim3(kGateThreads), 0, stream, logits, token_mask, expert_ids,
+                      counts, counts_are_offsets, d_weights, d_aux, T, E, k, load_balance_weight,
+                      vec, d_logits);
+  };
+  return E <= 8    ? run(balanced_gating_backward_kernel<1>)
+         : E <= 16 ? run(balanced_gating_backward_kernel<2>)
+         : E <= 32 ? run(balanced_gating_backward_kernel<4>)
+                   : run(balanced_gating_backward_kernel<8>);
+}
+
+extern "C" size_t lr_gate_backward_workspace_bytes(int num_tokens, int d_model, int num_experts) {
+  if (num_tokens < 1 || d_model < 1 || num_experts < 1) return 0;
+  const DwPlan p = dw_plan(num_tokens, d_model, num_experts);
+  if (p.splits == 1) return 0;
+  return size_t(p.splits) * num_experts * (size_t(d_model) + 1) * sizeof(float);
+}
+
+extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d,
+                                int E, void* d_h, float* d_wg, float* d_bias, void* workspace,
+                                size_t workspace_bytes, lr_stream_t stream) {
+  if (T < 0 || d <= 0 || d % 16 != 0 || E < 1 || E > 256) return LR_ERR_INVALID_ARGUMENT;
+  if (d_bias && !d_wg) return LR_ERR_INVALID_ARGUMENT;
+  if (T == 0) {
+    if (d_wg) LR_CUDA_TRY(cudaMemsetAsync(d_wg, 0, size_t(E) * d * sizeof(float), stream));
+    if (d_bias) LR_CUDA_TRY(cudaMemsetAsync(d_bias, 0, size_t(E) * sizeof(float), stream));
+    return LR_OK;
+  }
+  if (!d_logits || (d_h && !wg) || (d_wg && !h)) return LR_ERR_INVALID_ARGUMENT;
+  if (!aligned16(h) || !aligned16(wg) || !aligned16(d_h)) return LR_ERR_INVALID_ARGUMENT;
+  if (d_wg) {
+    const DwPlan p = dw_plan(T, d, E);
+    float* part = d_wg;
+    float* part_b = d_bias;
+    if (p.splits > 1) {
+      if (!workspace || workspace_bytes < lr_gate_backward_workspace_bytes(T, d, E))
+        return LR_ERR_WORKSPACE;
+      part = static_cast<float*>(workspace);
+      part_b = d_bias ? part + size_t(p.splits) * E * d : nullptr;
+    }
+    if (p.splits > 65535) return LR_ERR_INVALID_ARGUMENT;
+    const dim3 grid((d + 63) / 64, p.splits, (E + 63) / 64);
+    auto run = [&](auto kern) {
+      return launch_pdl(kern, grid, dim3(kDwWarps * 32), 0, stream,
+                        static_cast<const __half*>(h), d_logits, T, d, E, p.tokens_per_warp, part,
+                        part_b);
+    };
+    const int rc = E <= 8    ? run(gate_dw_kernel<1>)
+                   : E <= 16 ? run(gate_dw_kernel<2>)
+                   : E <= 32 ? run(gate_dw_kernel<4>)
+                             : run(gate_dw_kernel<8>);
+    if (rc != LR_OK) return rc;
+    if (p.splits > 1) {
+      const long n = long(E) * d;
+      const int rc2 =
+          launch_pdl(sum_parts_kernel, dim3(unsigned((n + 255) / 256)), dim3(256), 0, stream,
+                     static_cast<const float*>(part), n, static_cast<const float*>(part_b), E,
+                     p.splits, d_wg, d_bias);
+      if (rc2 != LR_OK) return rc2;
+    }
+  }
+  if (d_h) {
+    constexpr int MT = 2;
+    const dim3 grid((T + 16 * MT - 1) / (16 * MT), (d + 511) / 512);
+    return launch_pdl(gate_dh_kernel<MT>, grid, dim3(256), 0, stream, d_logits,
+                      static_cast<const __half*>(wg), T, d, E, static_cast<__half*>(d_h));
+  }
+  return LR_OK;
+}
+
+extern "C" int lr_combine_backward(const void* d_out, const void* y, const float* gate_weights,
+                                   const int32_t* slot_pos, const int32_t* offsets,
+                                   const int32_t* kept_counts, int T, int k, int d, int E,
+                                   void* d_y, float* d_weights, lr_stream_t stream) {
+  if (T < 0 || k < 1 || k > kMaxTopK || d <= 0 || d % 8 != 0 || E < 1)
+    return LR_ERR_INVALID_ARGUMENT;
+  if (T == 0) return LR_OK;
+  if (!d_out || !y || !gate_weights || !slot_pos || !offsets || !kept_counts || !d_y || !d_weights)
+    return LR_ERR_INVALID_ARGUMENT;
+  if (!aligned16(d_out) || !aligned16(y) || !aligned16(d_y)) return LR_ERR_INVALID_ARGUMENT;
+  const int d8 = d / 8;
+  auto run = [&](auto kern, int wpt) {
+    const int per = 8 / wpt;
+    return launch_pdl(kern, dim3((T + per - 1) / per), dim3(256), 0, stream,
+                      static_cast<const uint4*>(d_out), static_cast<const uint4*>(y), gate_weights,
+                      slot_pos, offsets, kept_counts, E, T, k, d8, static_cast<uint4*>(d_y),
+                      d_weights);
+  };
+  return T < 2368 ? run(combine_backward_kernel<8>, 8) : run(combine_backward_kernel<1>, 1);
+}

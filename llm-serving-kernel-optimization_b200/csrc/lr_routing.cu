@@ -792,7 +792,9 @@ __global__ void __launch_bounds__(256)
 
 // ---------------------------------------------------------------------------
 // combine: one warp per (token, 1/parts of the row), fp32 accumulation in
-// slot order (the split only spreads small batches over more warps)
+// slot order (the split only spreads small batches over more warps).  Without
+// weights (gate_w null) the rows are added as they are: the gradient of the
+// dispatch.
 // ---------------------------------------------------------------------------
 constexpr int kCombUnroll = 4;
 
@@ -820,7 +822,7 @@ __global__ void __launch_bounds__(256)
   float my_w = 0.f;
   if (lane < k) {
     my_pos = __ldg(slot_pos + size_t(t) * k + lane);
-    my_w = __ldg(gate_w + size_t(t) * k + lane);
+    my_w = gate_w ? __ldg(gate_w + size_t(t) * k + lane) : 1.f;
   }
   int pos[kMaxTopK];
   float w[kMaxTopK];
@@ -1211,6 +1213,19 @@ extern "C" int lr_combine(const void* y, const float* gate_weights, const int32_
                                slot_pos, T, k, d / 8, parts, static_cast<uint4*>(out)))
     return rc;
   return LR_OK;
+}
+
+extern "C" int lr_dispatch_backward(const void* d_permuted, const int32_t* slot_pos, int T, int k,
+                                    int d, void* d_x, lr_stream_t stream) {
+  if (T < 0 || k < 1 || k > kMaxTopK || d <= 0 || d % 8 != 0) return LR_ERR_INVALID_ARGUMENT;
+  if (T == 0) return LR_OK;
+  if (!d_permuted || !slot_pos || !d_x || !aligned16(d_permuted) || !aligned16(d_x))
+    return LR_ERR_INVALID_ARGUMENT;
+  const int parts = row_parts(T, d / 8);
+  return launch_pdl(combine_kernel, dim3(unsigned((long(T) * parts + 7) / 8)), dim3(256), 0,
+                    stream, static_cast<const uint4*>(d_permuted),
+                    static_cast<const float*>(nullptr), slot_pos, T, k, d / 8, parts,
+                    static_cast<uint4*>(d_x));
 }
 
 extern "C" size_t lr_gather_workspace_bytes(int num_rows, int num_tokens) {

@@ -2,9 +2,6 @@
 // torch custom ops (namespace `lightning_router`).  Tensors are validated here,
 // outputs and workspaces come from the caching allocator on the current
 // stream, and a non-zero LR_* status raises a RuntimeError.
-#include <ATen/ATen.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -12,35 +9,11 @@
 #include <tuple>
 #include <vector>
 
-#include "../../include/lightning_router.h"
+#include "lr_ops_common.h"
 
 namespace {
 
-void check_status(int rc, const char* what) {
-  TORCH_CHECK(rc == LR_OK, "lightning_router.", what, " failed: ", lr_status_string(rc), " (",
-              rc, ")");
-}
-
-lr_stream_t cur_stream() {
-  return reinterpret_cast<lr_stream_t>(at::cuda::getCurrentCUDAStream().stream());
-}
-
-void check_cuda(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
-  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
-}
-
-int32_t* err_ptr(const c10::optional<at::Tensor>& err) {
-  if (!err.has_value() || !err->defined()) return nullptr;
-  TORCH_CHECK(err->is_cuda() && err->scalar_type() == at::kInt && err->numel() >= 1,
-              "err must be a CUDA int32 tensor");
-  return err->data_ptr<int32_t>();
-}
-
-at::Tensor workspace(size_t bytes, const at::Tensor& like) {
-  return at::empty({static_cast<int64_t>(bytes < 16 ? 16 : bytes)},
-                   like.options().dtype(at::kByte));
-}
+using namespace lr_ops;
 
 // ---------------------------------------------------------------------------
 at::Tensor gate_logits(const at::Tensor& h, const at::Tensor& wg,

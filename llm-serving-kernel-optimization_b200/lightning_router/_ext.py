@@ -31,6 +31,10 @@ C_ABI_SYMBOLS = (
     "lr_weight_table_bytes", "lr_encode_weight_table",
     "lr_grouped_gemm_workspace_bytes", "lr_grouped_w4a16_workspace_bytes",
     "lr_grouped_w4a16_gemm", "lr_quantized_matmul",
+    "lr_balanced_gating_workspace_bytes", "lr_balanced_gating", "lr_balanced_gating_backward",
+    "lr_gate_backward_workspace_bytes", "lr_gate_backward",
+    "lr_dispatch_backward", "lr_combine_backward",
+    "lr_adapter_workspace_bytes", "lr_adapter_add", "lr_adapter_swiglu", "lr_adapter_rows",
     "lr_ep_plan_size", "lr_ep_plan", "lr_ep_plan_tokens", "lr_ep_publish", "lr_ep_plan_wait",
     "lr_ep_signal", "lr_ep_gather", "lr_ep_combine",
     "lr_ipc_export", "lr_ipc_import", "lr_ipc_close",
@@ -57,7 +61,8 @@ def clib() -> ctypes.CDLL:
     for name in ("lr_route_workspace_bytes", "lr_dispatch_workspace_bytes",
                  "lr_gate_dispatch_workspace_bytes",
                  "lr_gather_workspace_bytes", "lr_weight_table_bytes",
-                 "lr_grouped_gemm_workspace_bytes"):
+                 "lr_grouped_gemm_workspace_bytes", "lr_balanced_gating_workspace_bytes",
+                 "lr_gate_backward_workspace_bytes", "lr_adapter_workspace_bytes"):
         getattr(lib, name).restype = ctypes.c_size_t
     return lib
 
@@ -99,6 +104,7 @@ DEVERR_BITS = {
     0x4: "GEMM pipeline wait timed out",
     0x8: "GEMM row segment outside the row range",
     0x10: "another rank's expert-parallel exchange flag did not arrive in time",
+    0x20: "adapter number outside [-1, number of adapters)",
 }
 
 
