@@ -18,6 +18,7 @@ The operators (``op``):
               (form ``swiglu``).
 """
 
+import functools
 import math
 import sys
 from pathlib import Path
@@ -30,8 +31,9 @@ LBW = 0.01
 EPS = 1e-9
 
 
+@functools.lru_cache(maxsize=None)
 def _package():
-    """The framework's modules (its package directory goes on sys.path first, as for any of its users)."""
+    """The framework's modules, imported once (its package directory goes on sys.path, as for any user)."""
     where = str(Path(__file__).resolve().parents[1] / "llm-serving-kernel-optimization_b200")
     if where not in sys.path:
         sys.path.insert(0, where)
