@@ -142,6 +142,8 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
   constexpr int W = 8 * NT;
   constexpr int RK = 16 * RB;
   constexpr int PITCH = W + 2;
+  // k-blocks whose loads are in flight together: 12 to 16 16-byte loads per lane
+  constexpr int U = NT == 1 ? (RB == 1 ? 4 : RB == 2 ? 3 : 2) : (RB == 4 ? 1 : 2);
   extern __shared__ float s_part[];  // [kAdWarps][RK][PITCH]
   __shared__ Groups s;
   pdl_wait();
@@ -150,11 +152,12 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
   const int cs = int(cluster_nctarank()), cr = int(cluster_ctarank());
   const long row0 = long(blockIdx.x / cs) * W;
   const int bank = blockIdx.y / rank_groups, rank0 = (blockIdx.y % rank_groups) * RK;
+  const int per_round = kAdWarps / gridDim.z;  // groups a block takes at a time
   if (warp == 0) group_rows<W>(s, p.index, row0, p.R, p.n, false, bank == 0 ? p.err : nullptr);
   __syncthreads();
   const int nb = (p.K + 31) / 32;
-  for (int base = 0; base < s.n; base += kAdWarps) {
-    const int ng = min(kAdWarps, s.n - base);
+  for (int base = blockIdx.z * per_round; base < s.n; base += kAdWarps) {
+    const int ng = min(per_round, s.n - base);
     const int wpg = warps_per_group(ng);
     const int grp = warp / wpg, sub = warp % wpg;
     float acc[RB][NT][4];
@@ -167,15 +170,7 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
     if (grp < ng) {
       const int slot = base + grp;
       const int ad = s.adapter[s.first[slot]];
-      const __half* ap = (bank ? p.a[1] : p.a[0]) + size_t(ad) * p.r * p.K;
-      const __half* arow[2 * RB];
-      bool aok[2 * RB];
-#pragma unroll
-      for (int i = 0; i < 2 * RB; ++i) {
-        const int rk = rank0 + i * 8 + g;
-        aok[i] = rk < p.r;
-        arow[i] = ap + size_t(aok[i] ? rk : 0) * p.K + tq * 8;
-      }
+      const __half* ap = (bank ? p.a[1] : p.a[0]) + size_t(ad) * p.r * p.K + tq * 8;
       bool xok[NT], any[NT];
       const __half* xrow = p.x + size_t(row0 + g) * p.K + tq * 8;
 #pragma unroll
@@ -185,31 +180,38 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
       }
       const int part = cr * wpg + sub, parts = cs * wpg;
       const int kb0 = int(long(nb) * part / parts), kb1 = int(long(nb) * (part + 1) / parts);
-#pragma unroll(RB * NT == 1 ? 4 : NT == 1 ? 2 : 1)
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int k = kb * 32;
-        const bool kok = k + tq * 8 < p.K;
-        uint4 av[2 * RB], xv[NT];
+      for (int kb = kb0; kb < kb1; kb += U) {
+        uint4 av[U][2 * RB], xv[U][NT];
 #pragma unroll
-        for (int i = 0; i < 2 * RB; ++i) {
-          av[i] = make_uint4(0, 0, 0, 0);
-          if (aok[i] && kok) av[i] = __ldg(reinterpret_cast<const uint4*>(arow[i] + k));
+        for (int u = 0; u < U; ++u) {
+          const int k = (kb + u) * 32;
+          const bool kok = kb + u < kb1 && k + tq * 8 < p.K;
+#pragma unroll
+          for (int i = 0; i < 2 * RB; ++i) {
+            const int rk = rank0 + i * 8 + g;
+            av[u][i] = make_uint4(0, 0, 0, 0);
+            if (kok && rk < p.r)
+              av[u][i] = __ldg(reinterpret_cast<const uint4*>(ap + size_t(rk) * p.K + k));
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            xv[u][j] = make_uint4(0, 0, 0, 0);
+            if (kok && xok[j])
+              xv[u][j] = ld_row(reinterpret_cast<const uint4*>(xrow + size_t(j) * 8 * p.K + k));
+          }
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          xv[j] = make_uint4(0, 0, 0, 0);
-          if (xok[j] && kok)
-            xv[j] = ld_row(reinterpret_cast<const uint4*>(xrow + size_t(j) * 8 * p.K + k));
-        }
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if (any[j]) {
+          for (int j = 0; j < NT; ++j) {
+            if (any[j]) {
+              const uint4 x = xv[u][j];
 #pragma unroll
-            for (int i = 0; i < RB; ++i) {
-              mma_f16(acc[i][j], av[2 * i].x, av[2 * i + 1].x, av[2 * i].y, av[2 * i + 1].y,
-                      xv[j].x, xv[j].y);
-              mma_f16(acc[i][j], av[2 * i].z, av[2 * i + 1].z, av[2 * i].w, av[2 * i + 1].w,
-                      xv[j].z, xv[j].w);
+              for (int i = 0; i < RB; ++i) {
+                const uint4 lo = av[u][2 * i], hi = av[u][2 * i + 1];
+                mma_f16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+                mma_f16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+              }
             }
           }
         }
@@ -224,19 +226,41 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
         for (int c = 0; c < 2; ++c)
           *reinterpret_cast<float2*>(mine + (i * 16 + g + 8 * c) * PITCH + j * 8 + 2 * tq) =
               make_float2(acc[i][j][2 * c], acc[i][j][2 * c + 1]);
-    cluster_sync();
-    for (int o = cr * kAdThreads + threadIdx.x; o < W * RK; o += cs * kAdThreads) {
+    __syncthreads();
+    // warps of a group, then blocks of the cluster, in order
+    for (int o = threadIdx.x; o < W * RK; o += kAdThreads) {
       const int t = o / RK, i = o % RK;
       const int gt = s.group[t] - base;
-      if (gt >= 0 && gt < ng && rank0 + i < p.r) {
+      if (s.group[t] < 0 || gt < 0 || gt >= ng || rank0 + i >= p.r) continue;
+      float* at = s_part + (size_t(gt * wpg) * RK + i) * PITCH + t;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < kAdWarps; ++u)
+        if (u < wpg) sum += at[u * RK * PITCH];
+      if (cs == 1)
+        p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
+      else
+        *at = sum;
+    }
+    if (cs > 1) {
+      cluster_sync();
+      for (int o = cr * kAdThreads + threadIdx.x; o < W * RK; o += cs * kAdThreads) {
+        const int t = o / RK, i = o % RK;
+        const int gt = s.group[t] - base;
+        if (s.group[t] < 0 || gt < 0 || gt >= ng || rank0 + i >= p.r) continue;
+        const uint32_t at = smem_u32(s_part + (size_t(gt * wpg) * RK + i) * PITCH + t);
+        float q[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) q[c] = c < cs ? ld_cluster_f32(at, c) : 0.f;
         float sum = 0.f;
-        for (int c = 0; c < cs; ++c)
-          for (int u = 0; u < wpg; ++u)
-            sum += ld_cluster_f32(smem_u32(s_part + (size_t(gt * wpg + u) * RK + i) * PITCH + t), c);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) sum += q[c];
         p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
       }
+      cluster_sync();  // the parts stay until every block of the cluster has read them
+    } else {
+      __syncthreads();
     }
-    cluster_sync();  // the parts stay until every block of the cluster has read them
   }
 }
 
@@ -262,48 +286,121 @@ struct ExpandArgs {
   bool in_place;
 };
 
-template <int MT, bool SWIGLU>
-__global__ void __launch_bounds__(kAdThreads) adapter_expand_kernel(ExpandArgs p) {
+// The weights of a warp's 32 columns stay in registers while its row tiles pass.
+// RV is the rank rounded up to 16 (8-byte loads: one mma step), 32, 64 or 128
+// (16-byte loads: two steps per 32).
+template <int RV>
+struct RankTile {
+  static constexpr int kPer = RV == 16 ? 4 : 8;     // rank values of a lane's load
+  static constexpr int kLoads = RV == 16 ? 1 : RV / 32;
+  static constexpr int kWords = kPer / 2;
+  uint32_t w[kLoads][4][kWords];
+
+  // Columns n0 + (g >> 1) * 8 + 2 j + (g & 1); bp points at (that column for j = 0, tq * kPer).
+  LR_DEVICE void load(const __half* __restrict__ bp, int r, bool ok, int tq) {
+#pragma unroll
+    for (int b = 0; b < kLoads; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = ok && b * 32 + tq * kPer < r;
+        const __half* q = bp + size_t(2 * j) * r + b * 32;
+        if (RV == 16) {
+          uint2 v = make_uint2(0, 0);
+          if (in) v = __ldg(reinterpret_cast<const uint2*>(q));
+          w[b][j][0] = v.x;
+          w[b][j][1] = v.y;
+        } else {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (in) v = __ldg(reinterpret_cast<const uint4*>(q));
+          w[b][j][0] = v.x;
+          w[b][j][1] = v.y;
+          w[b][j][kWords - 2] = v.z;
+          w[b][j][kWords - 1] = v.w;
+        }
+      }
+  }
+
+  // acc += rows (two fp16 terms, `lo` after `hi`) . weights; hi points at (row g, tq * kPer).
+  LR_DEVICE void multiply(float (&acc)[4][4], const __half* hi, const __half* lo, int pitch) const {
+#pragma unroll
+    for (int b = 0; b < kLoads; ++b)
+#pragma unroll
+      for (int term = 0; term < 2; ++term) {
+        const __half* q = (term ? lo : hi) + b * 32;
+        if (RV == 16) {
+          const uint2 a0 = *reinterpret_cast<const uint2*>(q);
+          const uint2 a1 = *reinterpret_cast<const uint2*>(q + 8 * pitch);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            mma_f16(acc[j], a0.x, a1.x, a0.y, a1.y, w[b][j][0], w[b][j][1]);
+        } else {
+          const uint4 a0 = *reinterpret_cast<const uint4*>(q);
+          const uint4 a1 = *reinterpret_cast<const uint4*>(q + 8 * pitch);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            mma_f16(acc[j], a0.x, a1.x, a0.y, a1.y, w[b][j][0], w[b][j][1]);
+            mma_f16(acc[j], a0.z, a1.z, a0.w, a1.w, w[b][j][kWords - 2], w[b][j][kWords - 1]);
+          }
+        }
+      }
+  }
+};
+
+template <int RV, int MT, bool SWIGLU>
+__global__ void __launch_bounds__(kAdThreads, RV <= 64 && !SWIGLU ? 2 : 1)
+    adapter_expand_kernel(ExpandArgs p) {
   constexpr int W = 16 * MT;
   constexpr int BANKS = SWIGLU ? 2 : 1;
-  extern __shared__ __align__(16) unsigned char s_dyn[];  // [bank][hi, lo][W][pitch] fp16
+  constexpr int PITCH = RV + 8;
+  // column groups of a warp whose loads are in flight together (one row tile only)
+  constexpr int UC = MT > 1 || RV > 64 ? 1 : (RV <= 32 && !SWIGLU ? 4 : 2);
+  extern __shared__ __align__(16) __half s_v[];  // [bank][hi, lo][W][PITCH]
   __shared__ Groups s;
   __shared__ float s_fac[BANKS][W];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const long row0 = long(blockIdx.x) * W;
-  const int r32 = (p.r + 31) & ~31;
-  const int pitch = r32 + 8;
-  __half* s_v = reinterpret_cast<__half*>(s_dyn);
   if (warp == 0) group_rows<W>(s, p.index, row0, p.R, p.n, !p.in_place, nullptr);
   __syncthreads();
   {  // v: fp32 -> scaled (value, remainder) pairs
-    constexpr int LPR = kAdThreads / W;  // lanes per row (4 or 16)
+    constexpr int LPR = kAdThreads / W;  // lanes of a row
+    constexpr int EL = (RV + LPR - 1) / LPR;
     const int t = threadIdx.x / LPR, q = threadIdx.x % LPR;
     const int ad = s.adapter[t];
 #pragma unroll
     for (int bk = 0; bk < BANKS; ++bk) {
       const float* row = p.v + (size_t(bk) * p.R + row0 + t) * p.r;
+      float val[EL];
       float m = 0.f;
-      if (ad >= 0)
-        for (int i = q; i < p.r; i += LPR) m = fmaxf(m, fabsf(__ldcg(row + i)));
+#pragma unroll
+      for (int i = 0; i < EL; ++i) {
+        const int c = i * LPR + q;
+        val[i] = ad >= 0 && c < p.r ? __ldcg(row + c) : 0.f;
+        m = fmaxf(m, fabsf(val[i]));
+      }
 #pragma unroll
       for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      // 2^ex takes the row's largest into [2^14, 2^15); both powers are normal numbers
       int ex = 0;
-      if (m > 0.f && m < INFINITY) ex = max(-100, min(100, 14 - ilogbf(m)));
-      __half* hi = s_v + size_t(2 * bk) * W * pitch + size_t(t) * pitch;
-      __half* lo = hi + size_t(W) * pitch;
-      for (int i = q; i < r32; i += LPR) {
-        const float val = (ad >= 0 && i < p.r) ? ldexpf(__ldcg(row + i), ex) : 0.f;
-        const __half h = __float2half_rn(val);
-        const float hf = __half2float(h);
-        hi[i] = h;
-        lo[i] = __float2half_rn(fabsf(hf) < INFINITY ? val - hf : 0.f);
+      if (m > 0.f && m < INFINITY) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
+      const float up = __uint_as_float(unsigned(127 + ex) << 23);
+      const float down = __uint_as_float(unsigned(127 - ex) << 23);
+      __half* hi = s_v + (2 * bk * W + t) * PITCH;
+      __half* lo = hi + W * PITCH;
+#pragma unroll
+      for (int i = 0; i < EL; ++i) {
+        const int c = i * LPR + q;
+        if (c < RV) {
+          const float x = val[i] * up;
+          const __half h = __float2half_rn(x);
+          const float hf = __half2float(h);
+          hi[c] = h;
+          lo[c] = __float2half_rn(fabsf(hf) < INFINITY ? x - hf : 0.f);
+        }
       }
       if (q == 0)
-        s_fac[bk][t] =
-            ad >= 0 ? ldexpf(p.scale[bk] ? __ldg(p.scale[bk] + ad) : 1.f, -ex) : 0.f;
+        s_fac[bk][t] = ad >= 0 ? (p.scale[bk] ? __ldg(p.scale[bk] + ad) : 1.f) * down : 0.f;
     }
   }
   __syncthreads();
@@ -316,7 +413,7 @@ __global__ void __launch_bounds__(kAdThreads) adapter_expand_kernel(ExpandArgs p
     if (grp >= ng) continue;
     const int slot = base + grp;
     const int ad = s.adapter[s.first[slot]];
-    unsigned rows_ok = 0, tiles = 0;  // this lane's member rows, the warp's used m-tiles
+    unsigned rows_ok = 0, tiles = 0;  // this lane's member rows, the warp's used row tiles
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -324,86 +421,73 @@ __global__ void __launch_bounds__(kAdThreads) adapter_expand_kernel(ExpandArgs p
         if (s.group[m * 16 + g + 8 * h] == slot) rows_ok |= 1u << (2 * m + h);
       if (__any_sync(0xffffffffu, (rows_ok >> (2 * m)) & 3u)) tiles |= 1u << m;
     }
-    for (int cg = cg0 + sub; cg < cg1; cg += wpg) {
-      const int n0 = cg * 32;
-      const int nc = n0 + tq * 8;
-      uint4 bs[BANKS][MT][2];
+    for (int cg = cg0 + sub; cg < cg1; cg += wpg * UC) {
+      uint4 bs[UC][BANKS][MT][2];
+      RankTile<RV> wt[UC][BANKS];
 #pragma unroll
-      for (int bk = 0; bk < BANKS; ++bk)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (((rows_ok >> (2 * m + h)) & 1u) && nc < p.N)
-              bs[bk][m][h] = ld_row(reinterpret_cast<const uint4*>(
-                  p.base[bk] + size_t(row0 + m * 16 + g + 8 * h) * p.N + nc));
-      float acc[BANKS][MT][4][4];
-#pragma unroll
-      for (int bk = 0; bk < BANKS; ++bk)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[bk][m][j][c] = 0.f;
-      if (ad >= 0) {
+      for (int uc = 0; uc < UC; ++uc) {
+        const int c = cg + uc * wpg;
+        const int n0 = c * 32, nc = n0 + tq * 8;
+        const bool cok = c < cg1;
+        const int nr = n0 + (g >> 1) * 8;
 #pragma unroll
         for (int bk = 0; bk < BANKS; ++bk) {
-          const int nr = n0 + (g >> 1) * 8 + (g & 1);
-          const __half* bp = p.b[bk] + (size_t(ad) * p.N + nr) * p.r + tq * 8;
-          const bool nok = n0 + (g >> 1) * 8 < p.N;
-          const __half* vp = s_v + size_t(2 * bk) * W * pitch + tq * 8;
-          for (int rk = 0; rk < p.r; rk += 32) {
-            uint4 bv[4];
+          if (ad >= 0)
+            wt[uc][bk].load(
+                p.b[bk] + (size_t(ad) * p.N + nr + (g & 1)) * p.r + tq * RankTile<RV>::kPer, p.r,
+                cok && nr < p.N, tq);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              bv[j] = make_uint4(0, 0, 0, 0);
-              if (nok && rk + tq * 8 < p.r)
-                bv[j] = __ldg(reinterpret_cast<const uint4*>(bp + size_t(2 * j) * p.r + rk));
-            }
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              if ((tiles >> m) & 1u) {
-#pragma unroll
-                for (int term = 0; term < 2; ++term) {
-                  const __half* vr = vp + size_t(term) * W * pitch + size_t(m * 16 + g) * pitch + rk;
-                  const uint4 a0 = *reinterpret_cast<const uint4*>(vr);
-                  const uint4 a1 = *reinterpret_cast<const uint4*>(vr + size_t(8) * pitch);
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    mma_f16(acc[bk][m][j], a0.x, a1.x, a0.y, a1.y, bv[j].x, bv[j].y);
-                    mma_f16(acc[bk][m][j], a0.z, a1.z, a0.w, a1.w, bv[j].z, bv[j].w);
-                  }
-                }
-              }
-            }
-          }
+            for (int h = 0; h < 2; ++h)
+              if (cok && ((rows_ok >> (2 * m + h)) & 1u) && nc < p.N)
+                bs[uc][bk][m][h] = ld_row(reinterpret_cast<const uint4*>(
+                    p.base[bk] + size_t(row0 + m * 16 + g + 8 * h) * p.N + nc));
         }
       }
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int uc = 0; uc < UC; ++uc) {
+        const int c = cg + uc * wpg;
+        const int nc = c * 32 + tq * 8;
+        if (c >= cg1) break;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!((rows_ok >> (2 * m + h)) & 1u) || nc >= p.N) continue;
-          const int t = m * 16 + g + 8 * h;
-          float o[BANKS][8];
+        for (int m = 0; m < MT; ++m) {
+          if (!((tiles >> m) & 1u)) continue;
+          float acc[BANKS][4][4];
 #pragma unroll
           for (int bk = 0; bk < BANKS; ++bk) {
-            const __half2* bh = reinterpret_cast<const __half2*>(&bs[bk][m][h]);
-            const float f = s_fac[bk][t];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float2 b2 = __half22float2(bh[j]);
-              o[bk][2 * j] = ad >= 0 ? fmaf(acc[bk][m][j][2 * h], f, b2.x) : b2.x;
-              o[bk][2 * j + 1] = ad >= 0 ? fmaf(acc[bk][m][j][2 * h + 1], f, b2.y) : b2.y;
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[bk][j][i] = 0.f;
+            const __half* hi =
+                s_v + (2 * bk * W + m * 16 + g) * PITCH + tq * RankTile<RV>::kPer;
+            if (ad >= 0) wt[uc][bk].multiply(acc[bk], hi, hi + W * PITCH, PITCH);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!((rows_ok >> (2 * m + h)) & 1u) || nc >= p.N) continue;
+            const int t = m * 16 + g + 8 * h;
+            float o[BANKS][8];
+#pragma unroll
+            for (int bk = 0; bk < BANKS; ++bk) {
+              const __half2* bh = reinterpret_cast<const __half2*>(&bs[uc][bk][m][h]);
+              const float f = s_fac[bk][t];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 b2 = __half22float2(bh[j]);
+                o[bk][2 * j] = ad >= 0 ? fmaf(acc[bk][j][2 * h], f, b2.x) : b2.x;
+                o[bk][2 * j + 1] = ad >= 0 ? fmaf(acc[bk][j][2 * h + 1], f, b2.y) : b2.y;
+              }
             }
-          }
-          if (SWIGLU) {
+            if (SWIGLU) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[0][i] = silu_f32(o[0][i]) * o[BANKS - 1][i];
+              for (int i = 0; i < 8; ++i) o[0][i] = silu_f32(o[0][i]) * o[BANKS - 1][i];
+            }
+            *reinterpret_cast<uint4*>(p.out + size_t(row0 + t) * p.N + nc) = pack_half8(o[0]);
           }
-          *reinterpret_cast<uint4*>(p.out + size_t(row0 + t) * p.N + nc) = pack_half8(o[0]);
         }
+      }
     }
   }
 }
@@ -485,21 +569,22 @@ static int launch_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
   if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
   const long windows = (p.R + W - 1) / W;
   const int rank_groups = (p.r + RK - 1) / RK;
-  unsigned cs = 1;
+  // fill the SMs by splitting K over a cluster, then a window's groups over blocks
+  unsigned cs = 1, gs = 1;
   while (cs < 8 && windows * rank_groups * banks * cs < kTargetBlocks) cs *= 2;
+  while (gs < 4 && gs < p.R && windows * rank_groups * banks * cs * gs < kTargetBlocks) gs *= 2;
   if (windows * cs > 0x7fffffffL) return LR_ERR_INVALID_ARGUMENT;
-  return launch_cluster(kern, dim3(unsigned(windows * cs), rank_groups * banks), cs, smem, stream,
-                        p, rank_groups);
+  return launch_cluster(kern, dim3(unsigned(windows * cs), rank_groups * banks, gs), cs, smem,
+                        stream, p, rank_groups);
 }
 
-template <int MT, bool SWIGLU>
+template <int RV, int MT, bool SWIGLU>
 static int launch_expand(ExpandArgs p, cudaStream_t stream) {
   constexpr int W = 16 * MT;
-  const int r32 = (p.r + 31) & ~31;
-  const int per = 2 * W * 2 * (SWIGLU ? 2 : 1);
-  auto kern = adapter_expand_kernel<MT, SWIGLU>;
+  constexpr int smem = (SWIGLU ? 4 : 2) * W * (RV + 8) * int(sizeof(__half));
+  auto kern = adapter_expand_kernel<RV, MT, SWIGLU>;
   static unsigned long long configured = 0;
-  if (const int rc = set_dyn_smem_once(kern, per * (kMaxRank + 8), configured)) return rc;
+  if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
   const long windows = (p.R + W - 1) / W;
   const int cgs = (p.N + 31) / 32;
   // 256 columns per block, more while the grid stays above eight blocks per SM
@@ -507,17 +592,30 @@ static int launch_expand(ExpandArgs p, cudaStream_t stream) {
   while (gpc < 64 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
   p.groups_per_chunk = gpc;
   if (windows > 0x7fffffffL) return LR_ERR_INVALID_ARGUMENT;
-  return launch_pdl(kern, dim3(unsigned(windows), (cgs + gpc - 1) / gpc), dim3(kAdThreads),
-                    size_t(per) * (r32 + 8), stream, p);
+  return launch_pdl(kern, dim3(unsigned(windows), (cgs + gpc - 1) / gpc), dim3(kAdThreads), smem,
+                    stream, p);
 }
 
 static int run_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
   const bool small = p.R <= kSmallRows;
   if (p.r <= 16)
-    return small ? launch_shrink<1, 1>(p, banks, stream) : launch_shrink<1, 8>(p, banks, stream);
+    return small ? launch_shrink<1, 1>(p, banks, stream) : launch_shrink<1, 4>(p, banks, stream);
   if (p.r <= 32)
-    return small ? launch_shrink<2, 1>(p, banks, stream) : launch_shrink<2, 8>(p, banks, stream);
-  return small ? launch_shrink<4, 1>(p, banks, stream) : launch_shrink<4, 8>(p, banks, stream);
+    return small ? launch_shrink<2, 1>(p, banks, stream) : launch_shrink<2, 4>(p, banks, stream);
+  return small ? launch_shrink<4, 1>(p, banks, stream) : launch_shrink<4, 4>(p, banks, stream);
+}
+
+template <bool SWIGLU>
+static int run_expand(const ExpandArgs& p, cudaStream_t stream) {
+  constexpr int MT = SWIGLU ? 2 : 4;
+  const bool small = p.R <= kSmallRows;
+  if (p.r <= 16)
+    return small ? launch_expand<16, 1, SWIGLU>(p, stream) : launch_expand<16, MT, SWIGLU>(p, stream);
+  if (p.r <= 32)
+    return small ? launch_expand<32, 1, SWIGLU>(p, stream) : launch_expand<32, MT, SWIGLU>(p, stream);
+  if (p.r <= 64)
+    return small ? launch_expand<64, 1, SWIGLU>(p, stream) : launch_expand<64, MT, SWIGLU>(p, stream);
+  return small ? launch_expand<128, 1, SWIGLU>(p, stream) : launch_expand<128, MT, SWIGLU>(p, stream);
 }
 
 static int check_adapter_args(const void* x, long R, int K, const int32_t* index, int n, int r,
@@ -559,7 +657,7 @@ extern "C" int lr_adapter_add(const void* x, int R, int K, const int32_t* index,
   ExpandArgs ep{sp.v, {static_cast<const __half*>(b), nullptr}, {scale, nullptr}, index,
                 {static_cast<const __half*>(base), nullptr}, static_cast<__half*>(out), R, N,
                 num_adapters, rank, 0, base == out};
-  return R <= kSmallRows ? launch_expand<1, false>(ep, stream) : launch_expand<4, false>(ep, stream);
+  return run_expand<false>(ep, stream);
 }
 
 extern "C" int lr_adapter_swiglu(const void* x, int R, int K, const int32_t* index,
@@ -583,7 +681,7 @@ extern "C" int lr_adapter_swiglu(const void* x, int R, int K, const int32_t* ind
                 {scale_gate, scale_up}, index,
                 {static_cast<const __half*>(gate), static_cast<const __half*>(up)},
                 static_cast<__half*>(out), R, N, num_adapters, rank, 0, false};
-  return R <= kSmallRows ? launch_expand<1, true>(ep, stream) : launch_expand<2, true>(ep, stream);
+  return run_expand<true>(ep, stream);
 }
 
 extern "C" int lr_adapter_rows(const int32_t* adapter_ids, int T, int num_adapters,
