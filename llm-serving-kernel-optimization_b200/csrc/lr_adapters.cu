@@ -60,6 +60,29 @@ LR_DEVICE uint4 ld_row(const uint4* p) {
   return v;
 }
 
+LR_DEVICE void cp_async_16(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem)
+               : "memory");
+}
+LR_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+LR_DEVICE void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// silu(gate) * up of eight fp16 values
+LR_DEVICE uint4 swiglu8(const uint4& gate, const uint4& up) {
+  const __half2* a = reinterpret_cast<const __half2*>(&gate);
+  const __half2* b = reinterpret_cast<const __half2*>(&up);
+  float o[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = __half22float2(a[i]), y = __half22float2(b[i]);
+    o[2 * i] = silu_f32(x.x) * y.x;
+    o[2 * i + 1] = silu_f32(x.y) * y.y;
+  }
+  return pack_half8(o);
+}
+
 // ---------------------------------------------------------------------------
 // a window's groups
 // ---------------------------------------------------------------------------
@@ -170,51 +193,59 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
     if (grp < ng) {
       const int slot = base + grp;
       const int ad = s.adapter[s.first[slot]];
+      // Rank rows past r and rows of other groups read a valid row instead: their
+      // products land in values that nobody takes.
       const __half* ap = (bank ? p.a[1] : p.a[0]) + size_t(ad) * p.r * p.K + tq * 8;
-      bool xok[NT], any[NT];
-      const __half* xrow = p.x + size_t(row0 + g) * p.K + tq * 8;
+      const __half* arow[2 * RB];
+#pragma unroll
+      for (int i = 0; i < 2 * RB; ++i) {
+        const int rk = rank0 + i * 8 + g;
+        arow[i] = ap + size_t(rk < p.r ? rk : 0) * p.K;
+      }
+      const __half* xrow[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        xok[j] = s.group[j * 8 + g] == slot;
-        any[j] = __any_sync(0xffffffffu, xok[j]);
+        const int t = s.group[j * 8 + g] == slot ? j * 8 + g : s.first[slot];
+        xrow[j] = p.x + size_t(row0 + t) * p.K + tq * 8;
       }
+      auto load = [&](uint4(&av)[2 * RB], uint4(&xv)[NT], int kb) {
+#pragma unroll
+        for (int i = 0; i < 2 * RB; ++i)
+          av[i] = __ldg(reinterpret_cast<const uint4*>(arow[i] + kb * 32));
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          xv[j] = ld_row(reinterpret_cast<const uint4*>(xrow[j] + kb * 32));
+      };
+      auto multiply = [&](const uint4(&av)[2 * RB], const uint4(&xv)[NT]) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < RB; ++i) {
+            const uint4 lo = av[2 * i], hi = av[2 * i + 1], x = xv[j];
+            mma_f16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+            mma_f16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+          }
+      };
       const int part = cr * wpg + sub, parts = cs * wpg;
       const int kb0 = int(long(nb) * part / parts), kb1 = int(long(nb) * (part + 1) / parts);
-      for (int kb = kb0; kb < kb1; kb += U) {
+      const int kfull = min(kb1, p.K / 32);  // a last block of fewer than 32 k comes apart
+      int kb = kb0;
+      for (; kb + U <= kfull; kb += U) {
         uint4 av[U][2 * RB], xv[U][NT];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int k = (kb + u) * 32;
-          const bool kok = kb + u < kb1 && k + tq * 8 < p.K;
+        for (int u = 0; u < U; ++u) load(av[u], xv[u], kb + u);
 #pragma unroll
-          for (int i = 0; i < 2 * RB; ++i) {
-            const int rk = rank0 + i * 8 + g;
-            av[u][i] = make_uint4(0, 0, 0, 0);
-            if (kok && rk < p.r)
-              av[u][i] = __ldg(reinterpret_cast<const uint4*>(ap + size_t(rk) * p.K + k));
-          }
+        for (int u = 0; u < U; ++u) multiply(av[u], xv[u]);
+      }
+      for (; kb < kb1; ++kb) {
+        uint4 av[2 * RB], xv[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            xv[u][j] = make_uint4(0, 0, 0, 0);
-            if (kok && xok[j])
-              xv[u][j] = ld_row(reinterpret_cast<const uint4*>(xrow + size_t(j) * 8 * p.K + k));
-          }
-        }
+        for (int i = 0; i < 2 * RB; ++i) av[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if (any[j]) {
-              const uint4 x = xv[u][j];
-#pragma unroll
-              for (int i = 0; i < RB; ++i) {
-                const uint4 lo = av[u][2 * i], hi = av[u][2 * i + 1];
-                mma_f16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
-                mma_f16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
-              }
-            }
-          }
-        }
+        for (int j = 0; j < NT; ++j) xv[j] = make_uint4(0, 0, 0, 0);
+        if (kb * 32 + tq * 8 < p.K) load(av, xv, kb);
+        __syncwarp();
+        multiply(av, xv);
       }
     }
     float* mine = s_part + size_t(warp) * RK * PITCH;
@@ -346,15 +377,25 @@ struct RankTile {
   }
 };
 
+// Base rows in flight per warp: a ring over column groups, or (one row tile) as
+// many column groups at once as their weights' registers allow.
+template <int RV, int MT, bool SWIGLU>
+constexpr int expand_stages() {
+  return MT > 1 ? (RV <= 32 ? 3 : 2) : RV == 16 ? (SWIGLU ? 4 : 8) : RV == 32 ? (SWIGLU ? 2 : 4) : RV == 64 && !SWIGLU ? 2 : 1;
+}
+
 template <int RV, int MT, bool SWIGLU>
 __global__ void __launch_bounds__(kAdThreads, RV <= 64 && !SWIGLU ? 2 : 1)
     adapter_expand_kernel(ExpandArgs p) {
   constexpr int W = 16 * MT;
   constexpr int BANKS = SWIGLU ? 2 : 1;
   constexpr int PITCH = RV + 8;
-  // column groups of a warp whose loads are in flight together (one row tile only)
-  constexpr int UC = MT > 1 || RV > 64 ? 1 : (RV <= 32 && !SWIGLU ? 4 : 2);
-  extern __shared__ __align__(16) __half s_v[];  // [bank][hi, lo][W][PITCH]
+  constexpr int S = expand_stages<RV, MT, SWIGLU>();
+  constexpr bool AHEAD = RV <= 64 && !SWIGLU;
+  extern __shared__ __align__(16) unsigned char s_dyn[];
+  uint4* s_ring = reinterpret_cast<uint4*>(s_dyn);  // [warp][S][bank][2 MT][lane]
+  __half* s_v = reinterpret_cast<__half*>(s_ring + kAdWarps * S * BANKS * MT * 2 * 32);
+  // s_v: [bank][hi, lo][W][PITCH]
   __shared__ Groups s;
   __shared__ float s_fac[BANKS][W];
   pdl_wait();
@@ -421,73 +462,125 @@ __global__ void __launch_bounds__(kAdThreads, RV <= 64 && !SWIGLU ? 2 : 1)
         if (s.group[m * 16 + g + 8 * h] == slot) rows_ok |= 1u << (2 * m + h);
       if (__any_sync(0xffffffffu, (rows_ok >> (2 * m)) & 3u)) tiles |= 1u << m;
     }
-    for (int cg = cg0 + sub; cg < cg1; cg += wpg * UC) {
-      uint4 bs[UC][BANKS][MT][2];
-      RankTile<RV> wt[UC][BANKS];
+    // This lane's rows: (m, h) is 16 m + 8 h rows below the first.
+    const size_t row_off = size_t(row0 + g) * p.N;
+    const auto at = [&](int m, int h) { return size_t(unsigned(16 * m + 8 * h) * unsigned(p.N)); };
+    if (ad < 0) {  // no adapter: the base rows as they are
+      for (int c = cg0 + sub; c < cg1; c += wpg) {
+        const int nc = c * 32 + tq * 8;
 #pragma unroll
-      for (int uc = 0; uc < UC; ++uc) {
-        const int c = cg + uc * wpg;
-        const int n0 = c * 32, nc = n0 + tq * 8;
-        const bool cok = c < cg1;
-        const int nr = n0 + (g >> 1) * 8;
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int bk = 0; bk < BANKS; ++bk) {
-          if (ad >= 0)
-            wt[uc][bk].load(
-                p.b[bk] + (size_t(ad) * p.N + nr + (g & 1)) * p.r + tq * RankTile<RV>::kPer, p.r,
-                cok && nr < p.N, tq);
+          for (int h = 0; h < 2; ++h) {
+            if (!((rows_ok >> (2 * m + h)) & 1u) || nc >= p.N) continue;
+            uint4 v = ld_row(reinterpret_cast<const uint4*>(p.base[0] + row_off + at(m, h) + nc));
+            if (SWIGLU)
+              v = swiglu8(v, ld_row(reinterpret_cast<const uint4*>(p.base[BANKS - 1] + row_off +
+                                                                    at(m, h) + nc)));
+            *reinterpret_cast<uint4*>(p.out + row_off + at(m, h) + nc) = v;
+          }
+      }
+      continue;
+    }
+    // Column group c's base rows go to stage st of this lane's own slots.
+    uint4* slots = s_ring + warp * (S * BANKS * MT * 2 * 32) + lane;
+    const auto fetch = [&](int c, int st) {
+      const int nc = c * 32 + tq * 8;
+      if (c < cg1 && nc < p.N) {
+#pragma unroll
+        for (int bk = 0; bk < BANKS; ++bk)
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              if (cok && ((rows_ok >> (2 * m + h)) & 1u) && nc < p.N)
-                bs[uc][bk][m][h] = ld_row(reinterpret_cast<const uint4*>(
-                    p.base[bk] + size_t(row0 + m * 16 + g + 8 * h) * p.N + nc));
-        }
+              if ((rows_ok >> (2 * m + h)) & 1u)
+                cp_async_16(slots + ((st * BANKS + bk) * MT * 2 + 2 * m + h) * 32,
+                            p.base[bk] + row_off + at(m, h) + nc);
       }
+      cp_async_commit();
+    };
+    const auto weights = [&](RankTile<RV>(&wt)[BANKS], int c) {
+      const int nr = c * 32 + (g >> 1) * 8;
 #pragma unroll
-      for (int uc = 0; uc < UC; ++uc) {
-        const int c = cg + uc * wpg;
-        const int nc = c * 32 + tq * 8;
-        if (c >= cg1) break;
+      for (int bk = 0; bk < BANKS; ++bk)
+        wt[bk].load(p.b[bk] + (size_t(ad) * p.N + nr + (g & 1)) * p.r + tq * RankTile<RV>::kPer,
+                    p.r, c < cg1 && nr < p.N, tq);
+    };
+    const auto finish = [&](const RankTile<RV>(&wt)[BANKS], int c, int st) {
+      const int nc = c * 32 + tq * 8;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if (!((tiles >> m) & 1u)) continue;
-          float acc[BANKS][4][4];
+      for (int m = 0; m < MT; ++m) {
+        if (!((tiles >> m) & 1u)) continue;
+        float acc[BANKS][4][4];
+#pragma unroll
+        for (int bk = 0; bk < BANKS; ++bk) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[bk][j][i] = 0.f;
+          const __half* hi = s_v + (2 * bk * W + m * 16 + g) * PITCH + tq * RankTile<RV>::kPer;
+          wt[bk].multiply(acc[bk], hi, hi + W * PITCH, PITCH);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!((rows_ok >> (2 * m + h)) & 1u) || nc >= p.N) continue;
+          float o[BANKS][8];
 #pragma unroll
           for (int bk = 0; bk < BANKS; ++bk) {
+            const uint4 bs = slots[((st * BANKS + bk) * MT * 2 + 2 * m + h) * 32];
+            const __half2* bh = reinterpret_cast<const __half2*>(&bs);
+            const float f = s_fac[bk][m * 16 + g + 8 * h];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[bk][j][i] = 0.f;
-            const __half* hi =
-                s_v + (2 * bk * W + m * 16 + g) * PITCH + tq * RankTile<RV>::kPer;
-            if (ad >= 0) wt[uc][bk].multiply(acc[bk], hi, hi + W * PITCH, PITCH);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (!((rows_ok >> (2 * m + h)) & 1u) || nc >= p.N) continue;
-            const int t = m * 16 + g + 8 * h;
-            float o[BANKS][8];
-#pragma unroll
-            for (int bk = 0; bk < BANKS; ++bk) {
-              const __half2* bh = reinterpret_cast<const __half2*>(&bs[uc][bk][m][h]);
-              const float f = s_fac[bk][t];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 b2 = __half22float2(bh[j]);
-                o[bk][2 * j] = ad >= 0 ? fmaf(acc[bk][j][2 * h], f, b2.x) : b2.x;
-                o[bk][2 * j + 1] = ad >= 0 ? fmaf(acc[bk][j][2 * h + 1], f, b2.y) : b2.y;
-              }
+            for (int j = 0; j < 4; ++j) {
+              const float2 b2 = __half22float2(bh[j]);
+              o[bk][2 * j] = fmaf(acc[bk][j][2 * h], f, b2.x);
+              o[bk][2 * j + 1] = fmaf(acc[bk][j][2 * h + 1], f, b2.y);
             }
-            if (SWIGLU) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) o[0][i] = silu_f32(o[0][i]) * o[BANKS - 1][i];
-            }
-            *reinterpret_cast<uint4*>(p.out + size_t(row0 + t) * p.N + nc) = pack_half8(o[0]);
           }
+          if (SWIGLU) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[0][i] = silu_f32(o[0][i]) * o[BANKS - 1][i];
+          }
+          *reinterpret_cast<uint4*>(p.out + row_off + at(m, h) + nc) = pack_half8(o[0]);
         }
       }
+    };
+    if (MT == 1) {  // S column groups at a time, all their loads in flight
+      for (int c0 = cg0 + sub; c0 < cg1; c0 += wpg * S) {
+        RankTile<RV> wt[S][BANKS];
+#pragma unroll
+        for (int u = 0; u < S; ++u) {
+          fetch(c0 + u * wpg, u);
+          weights(wt[u], c0 + u * wpg);
+        }
+        cp_async_wait<0>();
+#pragma unroll
+        for (int u = 0; u < S; ++u)
+          if (c0 + u * wpg < cg1) finish(wt[u], c0 + u * wpg, u);
+      }
+    } else {  // a ring of S stages of base rows, the next group's weights in registers
+      RankTile<RV> wt[BANKS];
+      int c = cg0 + sub, st = 0;
+#pragma unroll
+      for (int u = 0; u < S - 1; ++u) fetch(c + u * wpg, u);
+      if (AHEAD) weights(wt, c);
+      for (; c < cg1; c += wpg) {
+        fetch(c + (S - 1) * wpg, st == 0 ? S - 1 : st - 1);
+        if (AHEAD) {
+          RankTile<RV> next[BANKS];
+          weights(next, c + wpg);
+          cp_async_wait<S - 1>();
+          finish(wt, c, st);
+#pragma unroll
+          for (int bk = 0; bk < BANKS; ++bk) wt[bk] = next[bk];
+        } else {
+          weights(wt, c);
+          cp_async_wait<S - 1>();
+          finish(wt, c, st);
+        }
+        st = st == S - 1 ? 0 : st + 1;
+      }
+      cp_async_wait<0>();
     }
   }
 }
@@ -581,7 +674,9 @@ static int launch_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
 template <int RV, int MT, bool SWIGLU>
 static int launch_expand(ExpandArgs p, cudaStream_t stream) {
   constexpr int W = 16 * MT;
-  constexpr int smem = (SWIGLU ? 4 : 2) * W * (RV + 8) * int(sizeof(__half));
+  constexpr int banks = SWIGLU ? 2 : 1;
+  constexpr int smem = kAdWarps * expand_stages<RV, MT, SWIGLU>() * banks * MT * 2 * 32 * 16 +
+                       banks * 2 * W * (RV + 8) * int(sizeof(__half));
   auto kern = adapter_expand_kernel<RV, MT, SWIGLU>;
   static unsigned long long configured = 0;
   if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
