@@ -1,0 +1,655 @@
+// lr_lowrank.cuh -- rows times a short inner dimension (up to 128), added to or
+// combined with base rows: the second half of the low-rank adapters and the row
+// gradient of the gate projection.
+#pragma once
+
+#include "lr_common.cuh"
+
+namespace lr {
+
+constexpr int kAdWarps = 8;
+constexpr int kAdThreads = kAdWarps * 32;
+constexpr int kMaxRank = 128;
+
+LR_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                       uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with a zero accumulator.
+LR_DEVICE void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+LR_DEVICE uint32_t cluster_ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+LR_DEVICE uint32_t cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+LR_DEVICE void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
+               ::: "memory");
+}
+LR_DEVICE float ld_cluster_f32(uint32_t saddr, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+// Plain 16-byte read that leaves L1 alone (rows read once; may be written in place later).
+LR_DEVICE uint4 ld_row(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
+LR_DEVICE void cp_async_16(void* smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem)
+               : "memory");
+}
+LR_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// silu(gate) * up of eight fp16 values
+LR_DEVICE uint4 swiglu8(const uint4& gate, const uint4& up) {
+  const __half2* a = reinterpret_cast<const __half2*>(&gate);
+  const __half2* b = reinterpret_cast<const __half2*>(&up);
+  float o[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = __half22float2(a[i]), y = __half22float2(b[i]);
+    o[2 * i] = silu_f32(x.x) * y.x;
+    o[2 * i + 1] = silu_f32(x.y) * y.y;
+  }
+  return pack_half8(o);
+}
+
+// ---------------------------------------------------------------------------
+// a window's groups
+// ---------------------------------------------------------------------------
+struct Groups {
+  int32_t adapter[64];  // per row: its adapter, -1 none, -2 past the last row
+  int32_t group[64];    // per row: its group, -1 for no group
+  int32_t first[64];    // per group: its first row
+  int n;
+  int uniform;          // every row has the same adapter
+};
+
+// Warp 0 groups the W <= 64 rows from row0 by adapter.  Rows without one make
+// a group of their own when `with_none`.  The caller synchronises the block.
+template <int W>
+LR_DEVICE void group_rows(Groups& s, const int32_t* __restrict__ index, long row0, long R, int n,
+                          bool with_none, int32_t* err) {
+  const int lane = threadIdx.x & 31;
+  int a[2], lead[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = u * 32 + lane;
+    a[u] = -2;
+    if (t < W && row0 + t < R) {
+      a[u] = __ldg(index + row0 + t);
+      if (a[u] < -1 || a[u] >= n) {
+        report(err, LR_DEVERR_BAD_ADAPTER);
+        a[u] = -1;
+      }
+    }
+    const unsigned peers = __match_any_sync(0xffffffffu, a[u]);
+    lead[u] = u * 32 + __ffs(peers) - 1;
+  }
+  const int lowest = with_none ? -1 : 0;
+  unsigned la = __ballot_sync(0xffffffffu, lead[0] == lane && a[0] >= lowest);
+  if (W > 32) {  // a group of the upper rows may have started in the lower ones
+    for (unsigned m = la; m; m &= m - 1) {
+      const int r = __ffs(m) - 1;
+      const int ar = __shfl_sync(0xffffffffu, a[0], r);
+      if (a[1] == ar) lead[1] = r;
+    }
+  }
+  const unsigned lb = __ballot_sync(0xffffffffu, W > 32 && lead[1] == 32 + lane && a[1] >= lowest);
+  const unsigned long long leaders = la | (static_cast<unsigned long long>(lb) << 32);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = u * 32 + lane;
+    if (t < W) {
+      const int slot = __popcll(leaders & ((1ull << lead[u]) - 1));
+      s.adapter[t] = a[u];
+      s.group[t] = a[u] >= lowest ? slot : -1;
+      if (a[u] >= lowest && lead[u] == t) s.first[slot] = t;
+    }
+  }
+  const int a0 = __shfl_sync(0xffffffffu, a[0], 0);
+  const bool same = __all_sync(0xffffffffu, (a[0] == a0 || a[0] == -2) && (a[1] == a0 || a[1] == -2));
+  if (lane == 0) {
+    s.n = __popcll(leaders);
+    s.uniform = same && a0 >= 0;
+  }
+}
+
+// Warps per group (a power of two) when g groups share the block's warps.
+LR_DEVICE int warps_per_group(int g) { return g <= 1 ? 8 : g <= 2 ? 4 : g <= 4 ? 2 : 1; }
+
+// ---------------------------------------------------------------------------
+// expand: out[row] = base[row] + s_a v[row] . B_a^T   (or the SwiGLU of two)
+// ---------------------------------------------------------------------------
+// mma m16n8k16 with the window's rows as M (MT tiles of 16) and output columns
+// as N.  v enters as two fp16 terms of the row scaled by a power of two to
+// [2^14, 2^15) (value and remainder: 2^-22 of the row's largest, no overflow),
+// so v is not rounded to fp16.  The terms are written to shared memory in
+// fragment order: one 16-byte read is a lane's A operand.  n-tile j, column c
+// stands for output column (c >> 1) * 8 + 2 j + (c & 1) of the warp's 32: a lane
+// ends with 8 neighbouring columns of its two rows, one 16-byte read of the base
+// and one store each.
+constexpr uint64_t kCopyWaitNs = 1000000000ull;  // bound of every wait for a copy
+
+enum ExpandMode : int {
+  kExpandAdd = 0,      // base + delta
+  kExpandSwiglu = 1,   // silu(base + delta) * (base2 + delta2)
+  kExpandProduct = 2,  // delta alone, every row with entry 0 of b (no index)
+};
+
+struct ExpandArgs {
+  const float* v;  // [bank][R][r]
+  const __half* b[2];  // [n][N][ldb], zero past r
+  const float* scale[2];
+  const int32_t* index;
+  const __half* base[2];  // the base rows; gate and up rows for SwiGLU
+  __half* out;
+  long R;
+  int N, n, r, ldb;
+  int groups_per_chunk;  // 32-column groups of a block
+  bool in_place;
+  int32_t* err;
+};
+
+// The weights of a warp's 32 columns stay in registers while its row tiles pass.
+// RV is the rank rounded up to 16 (8-byte loads: one mma step), 32, 64 or 128
+// (16-byte loads: two steps per 32).
+template <int RV>
+struct RankTile {
+  static constexpr int kPer = RV == 16 ? 4 : 8;     // rank values of a lane's load
+  static constexpr int kLoads = RV == 16 ? 1 : RV / 32;
+  static constexpr int kSteps = RV / 16;            // mma steps
+  uint32_t w[kSteps][4][2];
+
+  // Columns n0 + (g >> 1) * 8 + 2 j + (g & 1); bp points at (that column for j = 0, tq * kPer).
+  LR_DEVICE void load(const __half* __restrict__ bp, int ldb, bool ok, int tq) {
+#pragma unroll
+    for (int b = 0; b < kLoads; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = ok && b * 32 + tq * kPer < ldb;
+        const __half* q = bp + (unsigned(2 * j) * unsigned(ldb) + b * 32);
+        if (RV == 16) {
+          uint2 v = make_uint2(0, 0);
+          if (in) v = __ldg(reinterpret_cast<const uint2*>(q));
+          w[0][j][0] = v.x;
+          w[0][j][1] = v.y;
+        } else {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (in) v = __ldg(reinterpret_cast<const uint4*>(q));
+          w[2 * b][j][0] = v.x;
+          w[2 * b][j][1] = v.y;
+          w[(2 * b + 1) % kSteps][j][0] = v.z;
+          w[(2 * b + 1) % kSteps][j][1] = v.w;
+        }
+      }
+  }
+
+  // acc = the row tile's two terms (`lo` after `hi`: [step][lane]) . weights
+  LR_DEVICE void multiply(float (&acc)[4][4], const uint4* hi, const uint4* lo) const {
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      const uint4 a = hi[t * 32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (t == 0)
+          mma_f16_first(acc[j], a.x, a.y, a.z, a.w, w[t][j][0], w[t][j][1]);
+        else
+          mma_f16(acc[j], a.x, a.y, a.z, a.w, w[t][j][0], w[t][j][1]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      const uint4 a = lo[t * 32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mma_f16(acc[j], a.x, a.y, a.z, a.w, w[t][j][0], w[t][j][1]);
+    }
+  }
+};
+
+// Place of rank values (c, c + 1), c even, of row t among a window's fragments
+// [row tile][step][lane][4 words]: the words of a lane are (row g, first k),
+// (row g + 8, first k), (row g, second k), (row g + 8, second k).
+template <int RV>
+LR_DEVICE int fragment_word(int t, int c) {
+  const int m = t >> 4, h = (t >> 3) & 1, g = t & 7;
+  int step, tq, kh;
+  if (RV == 16) {
+    step = 0;
+    tq = c >> 2;
+    kh = (c >> 1) & 1;
+  } else {
+    step = (c >> 5) * 2 + ((c >> 2) & 1);
+    tq = (c >> 3) & 3;
+    kh = (c >> 1) & 1;
+  }
+  return ((m * (RV / 16) + step) * 32 + g * 4 + tq) * 4 + kh * 2 + h;
+}
+
+// One row tile: column groups of a warp whose loads are in flight together.
+template <int RV, int MODE>
+constexpr int expand_ahead() {
+  return RV == 16 ? (MODE == kExpandSwiglu ? 4 : 8)
+                  : RV == 32 ? (MODE == kExpandSwiglu ? 2 : 4)
+                             : RV == 64 && MODE != kExpandSwiglu ? 2 : 1;
+}
+
+// Larger windows stream the base rows: stages of the window's rows x 256 columns
+// by bulk copies of a producer warp, a consumer warp per 32 columns.
+constexpr int kTileCols = 256;
+constexpr int kTileGroups = kTileCols / 32;
+constexpr int kTilePitch = kTileCols * 2 + 64;  // bytes; neighbouring rows in different banks
+constexpr int kTileStages = 2;
+
+template <int RV, int MT, int MODE>
+constexpr int expand_base_bytes() {
+  return MODE == kExpandProduct ? 0
+         : MT == 1 ? kAdWarps * expand_ahead<RV, MODE>() * (MODE == kExpandSwiglu ? 2 : 1) * 2 * 512
+                   : kTileStages * (MODE == kExpandSwiglu ? 2 : 1) * MT * 16 * kTilePitch;
+}
+
+template <int RV, int MT, int MODE>
+constexpr int expand_smem_bytes() {
+  return expand_base_bytes<RV, MT, MODE>() + (MODE == kExpandSwiglu ? 2 : 1) * 2 * MT * 16 * RV * 2;
+}
+
+template <int MT, int MODE>
+constexpr int expand_threads() {
+  return kAdThreads + (MT > 1 && MODE != kExpandProduct ? 32 : 0);
+}
+
+// Nine warps leave 96 registers a thread to two blocks on an SM: enough up to rank 32.
+template <int RV, int MT, int MODE>
+constexpr int expand_min_blocks() {
+  return MODE == kExpandSwiglu || RV > 64 ? 1 : RV > 32 && MT > 1 && MODE == kExpandAdd ? 1 : 2;
+}
+
+// Eight results of a row: base (and base2) with the scaled sums of both banks.
+template <int MODE, int BANKS>
+LR_DEVICE uint4 expand_epilogue(const float (&acc)[BANKS][4][4], int h, const float (&fac)[BANKS],
+                                const uint4 (&base)[BANKS]) {
+  float o[BANKS][8];
+#pragma unroll
+  for (int bk = 0; bk < BANKS; ++bk) {
+    const __half2* bh = reinterpret_cast<const __half2*>(&base[bk]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 b2 = MODE == kExpandProduct ? make_float2(0.f, 0.f) : __half22float2(bh[j]);
+      o[bk][2 * j] = fmaf(acc[bk][j][2 * h], fac[bk], b2.x);
+      o[bk][2 * j + 1] = fmaf(acc[bk][j][2 * h + 1], fac[bk], b2.y);
+    }
+  }
+  if (MODE == kExpandSwiglu) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[0][i] = silu_f32(o[0][i]) * o[BANKS - 1][i];
+  }
+  return pack_half8(o[0]);
+}
+
+template <int RV, int MT, int MODE>
+__global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<RV, MT, MODE>())
+    expand_kernel(ExpandArgs p) {
+  constexpr int W = 16 * MT;
+  constexpr int BANKS = MODE == kExpandSwiglu ? 2 : 1;
+  constexpr int kTerm = W * RV / 8;  // uint4 of one term of v
+  extern __shared__ __align__(128) unsigned char s_dyn[];  // base rows, then v
+  uint4* s_v = reinterpret_cast<uint4*>(s_dyn + expand_base_bytes<RV, MT, MODE>());
+  // s_v: [bank][hi, lo][row tile][step][lane]
+  __shared__ uint64_t s_full[kTileStages], s_empty[kTileStages];
+  __shared__ int s_abort;
+  __shared__ Groups s;
+  __shared__ float s_fac[BANKS][W];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const long row0 = long(blockIdx.x) * W;
+  const int nrows = int(min(long(W), p.R - row0));
+  const int cg0 = blockIdx.y * p.groups_per_chunk;
+  const int cg1 = min(cg0 + p.groups_per_chunk, (p.N + 31) / 32);
+  if (MODE != kExpandProduct && warp == 0)
+    group_rows<W>(s, p.index, row0, p.R, p.n, !p.in_place, nullptr);
+  if (MT > 1 && MODE != kExpandProduct && threadIdx.x == 32) {
+    for (int i = 0; i < kTileStages; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(s_empty + i, kAdWarps);
+    }
+    s_abort = 0;
+    fence_mbarrier_init();
+  }
+  __syncthreads();
+  const bool stream = MT > 1 && MODE != kExpandProduct && s.uniform;
+
+  // Producer: tiles [first, last) of the base rows as bulk copies, each as soon as
+  // its stage has been read.  The first stages start ahead of everything else.
+  const int n_tiles = (cg1 - cg0 + kTileGroups - 1) / kTileGroups;
+  const auto produce = [&](int first, int last) {
+    for (int i = first; i < last; ++i) {
+      const int st = i % kTileStages, round = i / kTileStages, cg = cg0 + i * kTileGroups;
+      if (round > 0 &&
+          !mbar_wait_bounded(s_empty + st, (round - 1) & 1, &s_abort, p.err, kCopyWaitNs))
+        return i;
+      __syncwarp();
+      const unsigned bytes = unsigned(min(kTileCols, p.N - cg * 32)) * 2u;
+      if (lane == 0) mbar_arrive_expect_tx(s_full + st, bytes * nrows * BANKS);
+      __syncwarp();
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk)
+        for (int t = lane; t < nrows; t += 32)
+          bulk_load(s_dyn + ((st * BANKS + bk) * W + t) * kTilePitch,
+                    p.base[bk] + size_t(row0 + t) * p.N + cg * 32, bytes, s_full + st);
+    }
+    return last;
+  };
+  if (stream && warp == kAdWarps) produce(0, min(n_tiles, kTileStages));
+  if (threadIdx.x < kAdThreads) {  // v: fp32 -> scaled (value, remainder) pairs in fragment order
+    constexpr int LPR = kAdThreads / W;               // lanes of a row
+    constexpr int EL = (RV / 2 + LPR - 1) / LPR;      // pairs of a lane
+    const int t = threadIdx.x / LPR, q = threadIdx.x % LPR;
+    const int ad = MODE == kExpandProduct ? (t < nrows ? 0 : -1) : s.adapter[t];
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk) {
+      const float* row = p.v + (size_t(bk) * p.R + row0 + t) * p.r;
+      float val[EL][2];
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < EL; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = 2 * (i * LPR + q) + e;
+          val[i][e] = ad >= 0 && c < p.r ? __ldcg(row + c) : 0.f;
+          m = fmaxf(m, fabsf(val[i][e]));
+        }
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      // 2^ex takes the row's largest into [2^14, 2^15); both powers are normal numbers
+      int ex = 0;
+      if (m > 0.f && m < INFINITY) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
+      const float up = __uint_as_float(unsigned(127 + ex) << 23);
+      const float down = __uint_as_float(unsigned(127 - ex) << 23);
+      uint32_t* hi = reinterpret_cast<uint32_t*>(s_v + 2 * bk * kTerm);
+      uint32_t* lo = hi + 4 * kTerm;
+#pragma unroll
+      for (int i = 0; i < EL; ++i) {
+        const int c = 2 * (i * LPR + q);
+        if (c < RV) {
+          __half h[2], l[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = val[i][e] * up;
+            h[e] = __float2half_rn(x);
+            const float hf = __half2float(h[e]);
+            l[e] = __float2half_rn(fabsf(hf) < INFINITY ? x - hf : 0.f);
+          }
+          const int at = fragment_word<RV>(t, c);
+          hi[at] = __half_as_ushort(h[0]) | (uint32_t(__half_as_ushort(h[1])) << 16);
+          lo[at] = __half_as_ushort(l[0]) | (uint32_t(__half_as_ushort(l[1])) << 16);
+        }
+      }
+      if (q == 0)
+        s_fac[bk][t] = ad >= 0 ? (p.scale[bk] ? __ldg(p.scale[bk] + ad) : 1.f) * down : 0.f;
+    }
+  }
+  __syncthreads();
+
+  const unsigned n8 = 8u * unsigned(p.N);
+  if (MT > 1 && (stream || MODE == kExpandProduct)) {
+    // One entry of b for the whole window (a prompt's rows): a warp takes every
+    // eighth column group for all rows.
+    if (warp == kAdWarps) {
+      const int issued = produce(min(n_tiles, kTileStages), n_tiles);
+      // the last copies arrive before the block's shared memory goes
+      int none = 0;
+      for (int i = max(0, issued - kTileStages); i < issued; ++i)
+        mbar_wait_bounded(s_full + i % kTileStages, (i / kTileStages) & 1, &none, p.err,
+                          kCopyWaitNs);
+      return;
+    }
+    const int ad = MODE == kExpandProduct ? 0 : s.adapter[0];
+    const __half* wp[BANKS];
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk)
+      wp[bk] = p.b[bk] +
+               (size_t(ad) * p.N + (cg0 + warp) * 32 + (g >> 1) * 8 + (g & 1)) * p.ldb +
+               tq * RankTile<RV>::kPer;
+    const size_t wstep = size_t(kTileCols) * p.ldb;
+    float fac[2 * MT][BANKS];
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk)
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) fac[i][bk] = s_fac[bk][g + 8 * i];
+    __half* out = p.out + size_t(row0 + g) * p.N + (cg0 + warp) * 32 + tq * 8;
+    const unsigned char* bp = s_dyn + g * kTilePitch + warp * 64 + tq * 16;
+    const uint4* vp = s_v + lane;
+    unsigned st = 0, parity = 0;
+
+    const auto weights = [&](RankTile<RV>(&wt)[BANKS], int c) {
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk) {
+        wt[bk].load(wp[bk], p.ldb, c < cg1 && c * 32 + (g >> 1) * 8 < p.N, tq);
+        wp[bk] += wstep;
+      }
+    };
+    const auto tile = [&](const RankTile<RV>(&wt)[BANKS], int c) {
+      if (MODE != kExpandProduct &&
+          !mbar_wait_bounded(s_full + st, parity, &s_abort, p.err, kCopyWaitNs))
+        return false;
+      const bool cok = c < cg1 && c * 32 + tq * 8 < p.N;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        uint4 bs[2][BANKS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int bk = 0; bk < BANKS; ++bk)
+            if (MODE != kExpandProduct)
+              bs[h][bk] = *reinterpret_cast<const uint4*>(
+                  bp + ((st * BANKS + bk) * W + 16 * m + 8 * h) * kTilePitch);
+        if (m == MT - 1 && MODE != kExpandProduct) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_empty + st);
+        }
+        float acc[BANKS][4][4];
+#pragma unroll
+        for (int bk = 0; bk < BANKS; ++bk) {
+          const uint4* hi = vp + 2 * bk * kTerm + m * (RV / 16) * 32;
+          wt[bk].multiply(acc[bk], hi, hi + kTerm);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 o = expand_epilogue<MODE, BANKS>(acc, h, fac[2 * m + h], bs[h]);
+          if (cok && g + 16 * m + 8 * h < nrows)
+            *reinterpret_cast<uint4*>(out + size_t(unsigned(2 * m + h) * n8)) = o;
+        }
+      }
+      out += kTileCols;
+      if (++st == kTileStages) {
+        st = 0;
+        parity ^= 1;
+      }
+      return true;
+    };
+    // the next column group's weights load while one is multiplied
+    RankTile<RV> w0[BANKS], w1[BANKS];
+    int c = cg0 + warp;
+    const int end = cg0 + warp + n_tiles * kTileGroups;
+    if (RV <= 64 && MODE != kExpandSwiglu) {
+      weights(w0, c);
+      while (true) {
+        weights(w1, c + kTileGroups);
+        if (!tile(w0, c) || (c += kTileGroups) >= end) break;
+        weights(w0, c + kTileGroups);
+        if (!tile(w1, c) || (c += kTileGroups) >= end) break;
+      }
+    } else {
+      for (; c < end; c += kTileGroups) {
+        weights(w0, c);
+        if (!tile(w0, c)) break;
+      }
+    }
+    return;
+  }
+
+  // Mixed windows and small batches: the warps are dealt out to the groups.
+  if (warp >= kAdWarps) return;
+  constexpr int S = MT == 1 ? expand_ahead<RV, MODE>() : 1;
+  const int n_groups = MODE == kExpandProduct ? 1 : s.n;
+  for (int base = 0; base < n_groups; base += kAdWarps) {
+    const int ng = min(kAdWarps, n_groups - base);
+    const int wpg = warps_per_group(ng);
+    const int grp = warp / wpg, sub = warp % wpg;
+    if (grp >= ng) continue;
+    const int slot = base + grp;
+    const int ad = MODE == kExpandProduct ? 0 : s.adapter[s.first[slot]];
+    unsigned rows_ok = 0, tiles = 0;  // this lane's member rows, the warp's used row tiles
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int t = m * 16 + g + 8 * h;
+        if (MODE == kExpandProduct ? t < nrows : s.group[t] == slot) rows_ok |= 1u << (2 * m + h);
+      }
+      if (__any_sync(0xffffffffu, (rows_ok >> (2 * m)) & 3u)) tiles |= 1u << m;
+    }
+    // This lane's element offsets from the window's first row: row g + 8 i, column nc.
+    const unsigned row_n = unsigned(g) * unsigned(p.N) + tq * 8;
+    const size_t window = size_t(row0) * p.N;
+    const __half* base0 = MODE == kExpandProduct ? nullptr : p.base[0] + window;
+    const __half* base1 = MODE == kExpandProduct ? nullptr : p.base[BANKS - 1] + window;
+    __half* out = p.out + window;
+    if (ad < 0) {  // no adapter: the base rows as they are
+      for (int c = cg0 + sub; c < cg1; c += wpg) {
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {
+          if (!((rows_ok >> i) & 1u) || c * 32 + tq * 8 >= p.N) continue;
+          const unsigned o = row_n + c * 32 + i * n8;
+          uint4 v = ld_row(reinterpret_cast<const uint4*>(base0 + o));
+          if (MODE == kExpandSwiglu)
+            v = swiglu8(v, ld_row(reinterpret_cast<const uint4*>(base1 + o)));
+          *reinterpret_cast<uint4*>(out + o) = v;
+        }
+      }
+      continue;
+    }
+    // The base rows go through this lane's own slots of shared memory.
+    uint4* slots = reinterpret_cast<uint4*>(s_dyn) + warp * (S * BANKS * MT * 2 * 32) + lane;
+    for (int c0 = cg0 + sub; c0 < cg1; c0 += wpg * S) {  // all loads of S groups in flight
+      RankTile<RV> wt[S][BANKS];
+#pragma unroll
+      for (int u = 0; u < S; ++u) {
+        const int c = c0 + u * wpg;
+        const bool cin = c < cg1;
+        const int nr = c * 32 + (g >> 1) * 8;
+        const unsigned o = row_n + c * 32;
+#pragma unroll
+        for (int bk = 0; bk < BANKS; ++bk) {
+          if (MODE != kExpandProduct && cin && c * 32 + tq * 8 < p.N) {
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i)
+              if ((rows_ok >> i) & 1u)
+                cp_async_16(slots + ((u * BANKS + bk) * MT * 2 + i) * 32,
+                            (bk ? base1 : base0) + (o + i * n8));
+          }
+          wt[u][bk].load(p.b[bk] + (size_t(ad) * p.N + nr + (g & 1)) * p.ldb +
+                             tq * RankTile<RV>::kPer,
+                         p.ldb, cin && nr < p.N, tq);
+        }
+      }
+      cp_async_wait_all();
+#pragma unroll
+      for (int u = 0; u < S; ++u) {
+        const int c = c0 + u * wpg;
+        if (c >= cg1) break;
+        const bool cok = c * 32 + tq * 8 < p.N;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (!((tiles >> m) & 1u)) continue;
+          float acc[BANKS][4][4];
+#pragma unroll
+          for (int bk = 0; bk < BANKS; ++bk) {
+            const uint4* hi = s_v + lane + 2 * bk * kTerm + m * (RV / 16) * 32;
+            wt[u][bk].multiply(acc[bk], hi, hi + kTerm);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int i = 2 * m + h;
+            if (!((rows_ok >> i) & 1u) || !cok) continue;
+            uint4 bs[BANKS];
+            float fac[BANKS];
+#pragma unroll
+            for (int bk = 0; bk < BANKS; ++bk) {
+              if (MODE != kExpandProduct) bs[bk] = slots[((u * BANKS + bk) * MT * 2 + i) * 32];
+              fac[bk] = s_fac[bk][g + 8 * i];
+            }
+            *reinterpret_cast<uint4*>(out + (row_n + c * 32 + i * n8)) =
+                expand_epilogue<MODE, BANKS>(acc, h, fac, bs);
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+constexpr long kTargetBlocks = 148;
+
+template <int RV, int MT, int MODE>
+static int launch_expand(ExpandArgs p, cudaStream_t stream) {
+  constexpr int W = 16 * MT;
+  constexpr int smem = expand_smem_bytes<RV, MT, MODE>();
+  auto kern = expand_kernel<RV, MT, MODE>;
+  static unsigned long long configured = 0;
+  if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
+  const long windows = (p.R + W - 1) / W;
+  const int cgs = (p.N + 31) / 32;
+  // 256 columns per block, more while the grid stays above eight blocks per SM
+  int gpc = kTileGroups;
+  while (gpc < 64 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
+  p.groups_per_chunk = gpc;
+  if (windows > 0x7fffffffL || (cgs + gpc - 1) / gpc > 65535) return LR_ERR_INVALID_ARGUMENT;
+  return launch_pdl(kern, dim3(unsigned(windows), (cgs + gpc - 1) / gpc),
+                    dim3(expand_threads<MT, MODE>()), smem, stream, p);
+}
+
+// Row windows of 16 up to `small_rows` rows, else of 64 (32 for SwiGLU).
+template <int MODE>
+static int run_expand(const ExpandArgs& p, long small_rows, cudaStream_t stream) {
+  constexpr int MT = MODE == kExpandSwiglu ? 2 : 4;
+  const bool small = p.R <= small_rows;
+  if (p.r <= 16)
+    return small ? launch_expand<16, 1, MODE>(p, stream) : launch_expand<16, MT, MODE>(p, stream);
+  if (p.r <= 32)
+    return small ? launch_expand<32, 1, MODE>(p, stream) : launch_expand<32, MT, MODE>(p, stream);
+  if (p.r <= 64)
+    return small ? launch_expand<64, 1, MODE>(p, stream) : launch_expand<64, MT, MODE>(p, stream);
+  return small ? launch_expand<128, 1, MODE>(p, stream) : launch_expand<128, MT, MODE>(p, stream);
+}
+
+}  // namespace lr
