@@ -282,8 +282,8 @@ int lr_balanced_gating_backward(const float* logits, const uint8_t* token_mask,
 
 /* Gradients of lr_gate_logits: d_h[T,d] fp16 = d_logits . wg, d_wg[E,d] fp32 =
  * d_logits^T . h, d_bias[E] fp32 = column sums (each nullable; d_bias needs
- * d_wg).  d_logits[T,E] fp32 is not rounded.  Limits as lr_gate_logits; h, wg
- * and d_h 16-byte aligned.                                                  */
+ * d_wg).  d_logits[T,E] fp32 is not rounded.  Limits as lr_gate_logits; h, wg,
+ * d_h, d_wg and the workspace 16-byte aligned.                               */
 size_t lr_gate_backward_workspace_bytes(int num_tokens, int d_model, int num_experts);
 int lr_gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d, int E,
                      void* d_h, float* d_wg, float* d_bias, void* workspace,

@@ -173,7 +173,7 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     if (need_h) dh = at::empty({T, d}, h.options());
     if (need_w) dw = at::empty({E, d}, fopt);
     if (need_b) db = at::empty({E}, fopt);
-    auto ws = workspace(need_w ? lr_gate_backward_workspace_bytes(int(T), int(d), int(E)) : 0, dl);
+    auto ws = workspace(lr_gate_backward_workspace_bytes(int(T), int(d), int(E)), dl);
     check_status(lr_gate_backward(h.data_ptr(), w.data_ptr(), dl.data_ptr<float>(), int(T), int(d),
                                   int(E), need_h ? dh.data_ptr() : nullptr,
                                   need_w ? dw.data_ptr<float>() : nullptr,

@@ -61,9 +61,33 @@ LR_DEVICE uint4 ld_row(const uint4* p) {
   return v;
 }
 
+// Read-only loads that stay where they are issued (ahead of their use).
+LR_DEVICE uint4 ld_ahead16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+LR_DEVICE uint2 ld_ahead8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
 LR_DEVICE void cp_async_16(void* smem, const void* gmem) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(gmem)
                : "memory");
+}
+// Zeros instead of a copy where !ok (gmem is then not read).
+LR_DEVICE void cp_async_16_zfill(void* smem, const void* gmem, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(gmem),
+               "r"(ok ? 16 : 0)
+               : "memory");
+}
+LR_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+LR_DEVICE void cp_async_wait_group() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 LR_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // silu(gate) * up of eight fp16 values
@@ -197,12 +221,12 @@ struct RankTile {
         const __half* q = bp + (unsigned(2 * j) * unsigned(ldb) + b * 32);
         if (RV == 16) {
           uint2 v = make_uint2(0, 0);
-          if (in) v = __ldg(reinterpret_cast<const uint2*>(q));
+          if (in) v = ld_ahead8(q);
           w[0][j][0] = v.x;
           w[0][j][1] = v.y;
         } else {
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (in) v = __ldg(reinterpret_cast<const uint4*>(q));
+          if (in) v = ld_ahead16(q);
           w[2 * b][j][0] = v.x;
           w[2 * b][j][1] = v.y;
           w[(2 * b + 1) % kSteps][j][0] = v.z;
@@ -498,7 +522,7 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
     RankTile<RV> w0[BANKS], w1[BANKS];
     int c = cg0 + warp;
     const int end = cg0 + warp + n_tiles * kTileGroups;
-    if (RV <= 64 && MODE != kExpandSwiglu) {
+    if (RV <= (MODE == kExpandProduct ? 32 : 64) && MODE != kExpandSwiglu) {
       weights(w0, c);
       while (true) {
         weights(w1, c + kTileGroups);

@@ -10,7 +10,7 @@
 //   dl_e   = p_e (dp_e - sum_i p_i dp_i)              (f is a constant, as in the loss)
 //   dW     = dl^T h,  dh = dl W,  db = sum_t dl
 //   dy_row = w dout_t,  dw = <dout_t, y_row>,  dx_t = sum_j dpermuted[row_j]
-#include "lr_common.cuh"
+#include "lr_lowrank.cuh"
 
 namespace lr {
 
@@ -364,9 +364,8 @@ static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 // ---------------------------------------------------------------------------
 // gate projection: gradients
 // ---------------------------------------------------------------------------
-// fp32 gradients meet fp16 rows and weights on mma.sync m16n8k8 tf32: an fp16
-// value is a tf32 value, and the fp32 one goes in as two tf32 terms (rounded,
-// and rounded remainder: 2^-22 relative), so no rounding beyond fp32's is added.
+// fp32 gradients meet fp16 rows and weights: they go in as two terms (rounded, and
+// rounded remainder: 2^-22 left over), so no rounding beyond fp32's is added.
 LR_DEVICE void split_tf32(float v, uint32_t& hi, uint32_t& lo) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
   const float h = __uint_as_float(hi);
@@ -392,127 +391,256 @@ LR_DEVICE void half8_bits(const uint4& v, uint32_t (&f)[8]) {
   }
 }
 
-// dW[E,d] = dl^T h.  A block owns 64 columns of h and a token range that its 8
-// warps split; rows are the k axis.  A lane's 16-byte load holds 8 neighbouring
-// columns of one row; column g*8 + 2m (+1) is row g (g + 8) of m-tile m, so the
-// fragments need no shuffle.  A warp adds at most 256 rows in one accumulator
-// chain; warps are joined in shared memory, token ranges by a second launch,
-// both in a fixed order.
-constexpr int kDwWarps = 8;
-constexpr int kDwChain = 256;
+// dW[E,d] = dl^T h on mma.sync m16n8k16 fp16 with tokens as the k axis.  dl is
+// split once, per chunk of 128 tokens and expert, into two fp16 terms of the
+// column scaled by a power of two to [2^14, 2^15) (2^-22 of the column's largest
+// is left over); rows g and g + 8 of an m-tile are the value and the remainder of
+// expert g, so one instruction multiplies both and their sums stay apart until
+// the chunk is done.  Every chunk is added to fp32 totals: a tensor-core chain is
+// 8 steps long.
+constexpr int kChunk = 128;     // tokens of a scale, and of a tensor-core chain
+constexpr int kStage = 64;      // tokens of a pipeline stage
+constexpr int kDwCols = 256;    // columns of h per block, 32 per warp
+constexpr int kDwStages = 3;
+constexpr int kHPitch = kDwCols * 2 + 16;  // bytes: ldmatrix rows in different banks
 
-template <int ET>
-__global__ void __launch_bounds__(kDwWarps * 32)
-    gate_dw_kernel(const __half* __restrict__ h, const float* __restrict__ dl, int T, int d, int E,
-                   int tokens_per_warp, float* __restrict__ part, float* __restrict__ part_b) {
-  __shared__ float red[kDwWarps][8][65];
-  __shared__ float red_b[kDwWarps][8 * ET];
+// The scaled terms in fragment order [16-token step][8-expert tile][lane], the
+// powers of two that undo the scaling [chunk][E8], column sums [chunk][E8], and
+// the transposed weight [d][E8] (zero past E) for the row gradient.  Blocks
+// [0, chunks * groups) split dl, a chunk and 64 experts each; the rest transpose
+// 64 columns each.
+struct SplitArgs {
+  const float* dl;
+  const __half* wg;
+  int T, d, E, E8;
+  int split_blocks, groups;
+  uint4* frag;
+  float* down;
+  float* colsum;  // nullable
+  __half* wt;
+};
+
+__global__ void __launch_bounds__(256) gate_split_kernel(SplitArgs p) {
+  __shared__ float s_dl[kChunk][65];
+  __shared__ float s_red[4][64];
+  __shared__ float s_up[64];
+  pdl_wait();
+  pdl_trigger();
+  if (int(blockIdx.x) >= p.split_blocks) {
+    const int c0 = (blockIdx.x - p.split_blocks) * 64;
+    __half(*s_w)[66] = reinterpret_cast<__half(*)[66]>(&s_dl[0][0]);  // [expert][column]
+    for (int e0 = 0; e0 < p.E8; e0 += 64) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int e = e0 + (i >> 6), c = c0 + (i & 63);
+        s_w[i >> 6][i & 63] = e < p.E && c < p.d ? p.wg[size_t(e) * p.d + c] : __half(0.f);
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+        const int c = c0 + (i >> 6), e = e0 + (i & 63);
+        if (c < p.d && e < p.E8) p.wt[size_t(c) * p.E8 + e] = s_w[i & 63][i >> 6];
+      }
+    }
+    return;
+  }
+  const int chunk = blockIdx.x / p.groups, e0 = (blockIdx.x % p.groups) * 64;
+  const int ne = min(64, p.E - e0), ne8 = min(64, p.E8 - e0);
+  const long t0 = long(chunk) * kChunk;
+  for (int i = threadIdx.x; i < kChunk * 64; i += 256) {
+    const int t = i >> 6, e = i & 63;
+    s_dl[t][e] = t0 + t < p.T && e < ne ? __ldg(p.dl + size_t(t0 + t) * p.E + e0 + e) : 0.f;
+  }
+  __syncthreads();
+  {
+    const int e = threadIdx.x & 63, q = threadIdx.x >> 6;
+    float m = 0.f, sum = 0.f;
+    for (int t = q; t < kChunk; t += 4) {
+      m = fmaxf(m, fabsf(s_dl[t][e]));
+      sum += s_dl[t][e];
+    }
+    s_red[q][e] = m;
+    __syncthreads();
+    if (q == 0) {
+      m = fmaxf(fmaxf(s_red[0][e], s_red[1][e]), fmaxf(s_red[2][e], s_red[3][e]));
+      int ex = 0;
+      if (m > 0.f && m < INFINITY) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
+      s_up[e] = __uint_as_float(unsigned(127 + ex) << 23);
+      if (e < ne8) p.down[size_t(chunk) * p.E8 + e0 + e] = __uint_as_float(unsigned(127 - ex) << 23);
+    }
+    __syncthreads();
+    s_red[q][e] = sum;
+    __syncthreads();
+    if (q == 0 && p.colsum && e < ne8)
+      p.colsum[size_t(chunk) * p.E8 + e0 + e] =
+          (s_red[0][e] + s_red[1][e]) + (s_red[2][e] + s_red[3][e]);
+  }
+  // a thread writes a lane's A operand: 4 tokens of an expert, value and remainder
+  const int tiles = p.E8 / 8, my_tiles = ne8 / 8;
+  for (int i = threadIdx.x; i < (kChunk / 16) * my_tiles * 32; i += 256) {
+    const int lane = i & 31, tile = (i >> 5) % my_tiles, step = (i >> 5) / my_tiles;
+    const int e = tile * 8 + (lane >> 2), tq = lane & 3;
+    uint32_t w[4];
+#pragma unroll
+    for (int half_k = 0; half_k < 2; ++half_k) {
+      unsigned short h[2], l[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float x = s_dl[step * 16 + half_k * 8 + 2 * tq + u][e] * s_up[e];
+        const __half hi = __float2half_rn(x);
+        const float hf = __half2float(hi);
+        h[u] = __half_as_ushort(hi);
+        l[u] = __half_as_ushort(__float2half_rn(fabsf(hf) < INFINITY ? x - hf : 0.f));
+      }
+      w[2 * half_k] = h[0] | (uint32_t(h[1]) << 16);
+      w[2 * half_k + 1] = l[0] | (uint32_t(l[1]) << 16);
+    }
+    p.frag[((size_t(chunk) * (kChunk / 16) + step) * tiles + e0 / 8 + tile) * 32 + lane] =
+        make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+LR_DEVICE void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t saddr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(saddr));
+}
+
+// A block: 256 columns of h, up to 64 experts (blockIdx.z), a range of chunks.
+// Stages of 64 tokens (rows of h and dl fragments) come in by cp.async, three
+// deep.
+template <int MTL>
+__global__ void __launch_bounds__(256)
+    gate_dw_kernel(const __half* __restrict__ h, const uint4* __restrict__ frag,
+                   const float* __restrict__ down, int T, int d, int E, int E8, int chunks,
+                   int chunks_per_block, float* __restrict__ part) {
+  constexpr int kFragBytes = (kStage / 16) * MTL * 512;
+  constexpr int kHBytes = kStage * kHPitch;
+  extern __shared__ __align__(128) unsigned char s_dyn[];  // [stage][h rows, fragments]
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-  const int d0 = blockIdx.x * 64, e0 = blockIdx.z * 64;
-  const long tb = (long(blockIdx.y) * kDwWarps + warp) * tokens_per_warp;
-  const long te = min(long(T), tb + tokens_per_warp);
-  const bool dok = d0 + g * 8 < d;
-  float acc[4][ET][4];
-  float bsum[ET];
+  const int d0 = blockIdx.x * kDwCols, e0 = blockIdx.z * 64;
+  const int tiles = E8 / 8;
+  const int c0 = blockIdx.y * chunks_per_block, c1 = min(chunks, c0 + chunks_per_block);
+  const int stages = (c1 - c0) * (kChunk / kStage);
+  const auto fetch = [&](int i) {
+    if (i < stages) {
+      unsigned char* sh = s_dyn + (i % kDwStages) * (kHBytes + kFragBytes);
+      const long t0 = long(c0) * kChunk + long(i) * kStage;
 #pragma unroll
-  for (int n = 0; n < ET; ++n) {
-    bsum[n] = 0.f;
-#pragma unroll
-    for (int m = 0; m < 4; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
-  }
-#pragma unroll 2
-  for (long t0 = tb; t0 < te; t0 += 8) {
-    uint32_t x[2][8];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const long t = t0 + tq + 4 * u;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (t < te && dok) v = ld_stream(reinterpret_cast<const uint4*>(h + size_t(t) * d + d0 + g * 8));
-      half8_bits(v, x[u]);
-    }
-#pragma unroll
-    for (int n = 0; n < ET; ++n) {
-      if (e0 + n * 8 < E) {
-        const int e = e0 + n * 8 + g;
-        uint32_t hi[2], lo[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const long t = t0 + tq + 4 * u;
-          const float v = (t < te && e < E) ? __ldg(dl + size_t(t) * E + e) : 0.f;
-          bsum[n] += v;
-          split_tf32(v, hi[u], lo[u]);
-        }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const uint32_t a[4] = {x[0][2 * m], x[0][2 * m + 1], x[1][2 * m], x[1][2 * m + 1]};
-          mma_tf32(acc[m][n], a, hi[0], hi[1]);
-          mma_tf32(acc[m][n], a, lo[0], lo[1]);
-        }
+      for (int u = 0; u < kStage / 8; ++u) {  // a warp per row
+        const int t = u * 8 + warp, c = d0 + lane * 8;
+        const bool ok = t0 + t < T && c < d;
+        cp_async_16_zfill(sh + t * kHPitch + lane * 16, h + size_t(ok ? t0 + t : 0) * d + (ok ? c : 0),
+                          ok);
+      }
+      const uint4* fp = frag + (t0 / 16) * tiles * 32 + (e0 / 8) * 32;
+      for (int x = threadIdx.x; x < (kStage / 16) * MTL * 32; x += 256) {
+        const int step = x / (MTL * 32), in = x % (MTL * 32);
+        const bool ok = e0 / 8 + in / 32 < tiles;
+        cp_async_16_zfill(sh + kHBytes + x * 16, fp + (ok ? step * tiles * 32 + in : 0), ok);
       }
     }
-  }
+    cp_async_commit();
+  };
+  float total[MTL][4][2];
 #pragma unroll
-  for (int n = 0; n < ET; ++n) {
-    if (e0 + n * 8 < E) {  // the same for the whole block
-      __syncthreads();
+  for (int m = 0; m < MTL; ++m)
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+    for (int n = 0; n < 4; ++n) total[m][n][0] = total[m][n][1] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          red[warp][2 * tq + (i & 1)][g * 8 + 2 * m + (i >> 1)] = acc[m][n][i];
-      __syncthreads();
-      for (int o = threadIdx.x; o < 8 * 64; o += kDwWarps * 32) {
-        const int r = o >> 6, c = o & 63;
-        const int e = e0 + n * 8 + r;
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < kDwWarps; ++w) s += red[w][r][c];
-        if (e < E && d0 + c < d) part[(size_t(blockIdx.y) * E + e) * d + d0 + c] = s;
-      }
-    }
-  }
-  if (part_b && blockIdx.x == 0) {
-#pragma unroll
-    for (int n = 0; n < ET; ++n) {
-      float s = bsum[n];
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      if (tq == 0) red_b[warp][n * 8 + g] = s;
-    }
+  for (int i = 0; i < kDwStages - 1; ++i) fetch(i);
+  float acc[MTL][4][4];
+  for (int i = 0; i < stages; ++i) {
+    cp_async_wait_group<kDwStages - 2>();
     __syncthreads();
-    for (int o = threadIdx.x; o < 8 * ET; o += kDwWarps * 32) {
-      float s = 0.f;
+    fetch(i + kDwStages - 1);
+    if (i % (kChunk / kStage) == 0) {
 #pragma unroll
-      for (int w = 0; w < kDwWarps; ++w) s += red_b[w][o];
-      if (e0 + o < E) part_b[size_t(blockIdx.y) * E + e0 + o] = s;
+      for (int m = 0; m < MTL; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[m][n][c] = 0.f;
+    }
+    const unsigned char* sh = s_dyn + (i % kDwStages) * (kHBytes + kFragBytes);
+    const uint32_t hrow = smem_u32(sh) + (lane & 15) * kHPitch + warp * 64 + (lane >> 4) * 16;
+    const uint4* fr = reinterpret_cast<const uint4*>(sh + kHBytes) + lane;
+#pragma unroll
+    for (int step = 0; step < kStage / 16; ++step) {
+      uint32_t b[2][4];
+      ldmatrix_x4_trans(b[0], hrow + step * 16 * kHPitch);
+      ldmatrix_x4_trans(b[1], hrow + step * 16 * kHPitch + 32);
+#pragma unroll
+      for (int m = 0; m < MTL; ++m) {
+        const uint4 a = fr[(step * MTL + m) * 32];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          mma_f16(acc[m][n], a.x, a.y, a.z, a.w, b[n >> 1][(n & 1) * 2], b[n >> 1][(n & 1) * 2 + 1]);
+      }
+    }
+    if (i % (kChunk / kStage) == kChunk / kStage - 1) {
+      const int chunk = c0 + i / (kChunk / kStage);
+#pragma unroll
+      for (int m = 0; m < MTL; ++m) {
+        const int e = e0 + m * 8 + g;
+        const float f = e < E8 ? __ldg(down + size_t(chunk) * E8 + e) : 0.f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          total[m][n][0] = fmaf(acc[m][n][0] + acc[m][n][2], f, total[m][n][0]);
+          total[m][n][1] = fmaf(acc[m][n][1] + acc[m][n][3], f, total[m][n][1]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MTL; ++m) {
+    const int e = e0 + m * 8 + g;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const int c = d0 + warp * 32 + n * 8 + 2 * tq;
+      if (e < E && c < d)
+        *reinterpret_cast<float2*>(part + (size_t(blockIdx.y) * E + e) * d + c) =
+            make_float2(total[m][n][0], total[m][n][1]);
     }
   }
 }
 
-// out[i] = sum over the token ranges of part[s][i], in range order.
+// out[i] = sum over the token ranges of part[s][i], in range order; the bias
+// gradient from the chunks' column sums, a warp per expert.
 __global__ void __launch_bounds__(256)
-    sum_parts_kernel(const float* __restrict__ part, long n, const float* __restrict__ part_b,
-                     int nb, int splits, float* __restrict__ out, float* __restrict__ out_b) {
+    sum_parts_kernel(const float* __restrict__ part, long n4, int splits, long blocks,
+                     float* __restrict__ out, const float* __restrict__ colsum, int chunks, int E,
+                     int E8, float* __restrict__ out_b) {
   pdl_wait();
   pdl_trigger();
+  if (blockIdx.x >= blocks) {
+    const int e = int(blockIdx.x - blocks) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    float s = 0.f;
+    if (e < E)
+      for (int c = lane; c < chunks; c += 32) s += colsum[size_t(c) * E8 + e];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (e < E && lane == 0) out_b[e] = s;
+    return;
+  }
   const long i = long(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n) {
-    float s = 0.f;
-    for (int p = 0; p < splits; ++p) s += part[size_t(p) * n + i];
-    out[i] = s;
+  if (i >= n4) return;
+  const float4* q = reinterpret_cast<const float4*>(part) + i;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) {
+    const float4 v = q[size_t(k) * n4];
+    s.x += v.x;
+    s.y += v.y;
+    s.z += v.z;
+    s.w += v.w;
   }
-  if (out_b && i < nb) {
-    float s = 0.f;
-    for (int p = 0; p < splits; ++p) s += part_b[size_t(p) * nb + i];
-    out_b[i] = s;
-  }
+  reinterpret_cast<float4*>(out)[i] = s;
 }
 
-// dh[T,d] = dl W, fp16 out.  A warp owns MT*16 tokens x 64 columns; experts are
+// dh[T,d] = dl W, fp16 out, for more experts than the low-rank kernel takes (128).
+// fp32 gradients go in as two tf32 terms.  A warp owns MT*16 tokens x 64 columns; experts are
 // the k axis.  n-tile j takes column g*8 + j of the lane's 16-byte weight load,
 // so a lane ends with 16 neighbouring columns of its rows.
 template <int MT>
@@ -575,18 +703,41 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-struct DwPlan {
-  int tokens_per_warp, splits;
+struct GatePlan {
+  int E8, chunks, groups, per_block, splits;
+  size_t frag, down, colsum, wt, part, bytes;  // workspace offsets
 };
 
-// Token ranges of the weight gradient: chains of at most kDwChain rows per warp,
-// shorter ones while the grid has fewer than two blocks per SM.
-static DwPlan dw_plan(int T, int d, int E) {
-  const long cols = long((d + 63) / 64) * ((E + 63) / 64);
-  int tpw = kDwChain;
-  while (tpw > 16 && cols * ((T + long(tpw) * kDwWarps - 1) / (long(tpw) * kDwWarps)) < 296)
-    tpw /= 2;
-  return {tpw, int((T + long(tpw) * kDwWarps - 1) / (long(tpw) * kDwWarps))};
+// Token ranges of the weight gradient: as many chunks per block as keep two
+// blocks per SM.
+static GatePlan gate_plan(int T, int d, int E) {
+  GatePlan p;
+  p.E8 = (E + 7) & ~7;
+  p.groups = (E + 63) / 64;
+  p.chunks = (T + kChunk - 1) / kChunk;
+  const long cols = long((d + kDwCols - 1) / kDwCols) * p.groups;
+  p.per_block = int(p.chunks * cols / (2 * kTargetBlocks));
+  if (p.per_block < 1) p.per_block = 1;
+  p.splits = (p.chunks + p.per_block - 1) / p.per_block;
+  p.frag = 0;
+  p.down = p.frag + size_t(p.chunks) * (kChunk / 16) * (p.E8 / 8) * 512;
+  p.colsum = p.down + align256(size_t(p.chunks) * p.E8 * sizeof(float));
+  p.wt = p.colsum + align256(size_t(p.chunks) * p.E8 * sizeof(float));
+  p.part = p.wt + align256(size_t(d) * p.E8 * sizeof(__half));
+  p.bytes = p.part + (p.splits > 1 ? size_t(p.splits) * E * d * sizeof(float) : 0);
+  return p;
+}
+
+template <int MTL>
+static int launch_dw(const __half* h, const uint4* frag, const float* down, int T, int d, int E,
+                     const GatePlan& gp, float* part, cudaStream_t stream) {
+  constexpr int smem = kDwStages * (kStage * kHPitch + (kStage / 16) * MTL * 512);
+  auto kern = gate_dw_kernel<MTL>;
+  static unsigned long long configured = 0;
+  if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
+  const dim3 grid((d + kDwCols - 1) / kDwCols, gp.splits, gp.groups);
+  return launch_pdl(kern, grid, dim3(256), smem, stream, h, frag, down, T, d, E, gp.E8, gp.chunks,
+                    gp.per_block, part);
 }
 
 // ---------------------------------------------------------------------------
@@ -772,9 +923,7 @@ extern "C" int lr_balanced_gating_backward(const float* logits, const uint8_t* t
 
 extern "C" size_t lr_gate_backward_workspace_bytes(int num_tokens, int d_model, int num_experts) {
   if (num_tokens < 1 || d_model < 1 || num_experts < 1) return 0;
-  const DwPlan p = dw_plan(num_tokens, d_model, num_experts);
-  if (p.splits == 1) return 0;
-  return size_t(p.splits) * num_experts * (size_t(d_model) + 1) * sizeof(float);
+  return gate_plan(num_tokens, d_model, num_experts).bytes;
 }
 
 extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d,
@@ -788,43 +937,66 @@ extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_lo
     return LR_OK;
   }
   if (!d_logits || (d_h && !wg) || (d_wg && !h)) return LR_ERR_INVALID_ARGUMENT;
-  if (!aligned16(h) || !aligned16(wg) || !aligned16(d_h)) return LR_ERR_INVALID_ARGUMENT;
-  if (d_wg) {
-    const DwPlan p = dw_plan(T, d, E);
-    float* part = d_wg;
-    float* part_b = d_bias;
-    if (p.splits > 1) {
-      if (!workspace || workspace_bytes < lr_gate_backward_workspace_bytes(T, d, E))
-        return LR_ERR_WORKSPACE;
-      part = static_cast<float*>(workspace);
-      part_b = d_bias ? part + size_t(p.splits) * E * d : nullptr;
-    }
-    if (p.splits > 65535) return LR_ERR_INVALID_ARGUMENT;
-    const dim3 grid((d + 63) / 64, p.splits, (E + 63) / 64);
-    auto run = [&](auto kern) {
-      return launch_pdl(kern, grid, dim3(kDwWarps * 32), 0, stream,
-                        static_cast<const __half*>(h), d_logits, T, d, E, p.tokens_per_warp, part,
-                        part_b);
-    };
-    const int rc = E <= 8    ? run(gate_dw_kernel<1>)
-                   : E <= 16 ? run(gate_dw_kernel<2>)
-                   : E <= 32 ? run(gate_dw_kernel<4>)
-                             : run(gate_dw_kernel<8>);
-    if (rc != LR_OK) return rc;
-    if (p.splits > 1) {
-      const long n = long(E) * d;
-      const int rc2 =
-          launch_pdl(sum_parts_kernel, dim3(unsigned((n + 255) / 256)), dim3(256), 0, stream,
-                     static_cast<const float*>(part), n, static_cast<const float*>(part_b), E,
-                     p.splits, d_wg, d_bias);
-      if (rc2 != LR_OK) return rc2;
+  if (!aligned16(h) || !aligned16(wg) || !aligned16(d_h) || !aligned16(d_wg))
+    return LR_ERR_INVALID_ARGUMENT;
+  if (!d_wg && !d_h) return LR_OK;
+  const GatePlan gp = gate_plan(T, d, E);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < gp.bytes) return LR_ERR_WORKSPACE;
+  if (gp.splits > 65535) return LR_ERR_INVALID_ARGUMENT;
+  char* ws = static_cast<char*>(workspace);
+  const bool low_rank = d_h && E <= kMaxRank;
+  SplitArgs sp;
+  sp.dl = d_logits;
+  sp.wg = static_cast<const __half*>(wg);
+  sp.T = T;
+  sp.d = d;
+  sp.E = E;
+  sp.E8 = gp.E8;
+  sp.groups = gp.groups;
+  sp.split_blocks = d_wg ? gp.chunks * gp.groups : 0;
+  sp.frag = reinterpret_cast<uint4*>(ws + gp.frag);
+  sp.down = reinterpret_cast<float*>(ws + gp.down);
+  sp.colsum = d_bias ? reinterpret_cast<float*>(ws + gp.colsum) : nullptr;
+  sp.wt = reinterpret_cast<__half*>(ws + gp.wt);
+  const int blocks = sp.split_blocks + (low_rank ? (d + 63) / 64 : 0);
+  if (blocks > 0)
+    if (const int rc = launch_pdl(gate_split_kernel, dim3(blocks), dim3(256), 0, stream, sp))
+      return rc;
+  if (d_h) {
+    if (low_rank) {
+      ExpandArgs ep{};
+      ep.v = d_logits;
+      ep.b[0] = sp.wt;
+      ep.out = static_cast<__half*>(d_h);
+      ep.R = T;
+      ep.N = d;
+      ep.n = 1;
+      ep.r = E;
+      ep.ldb = gp.E8;
+      if (const int rc = run_expand<kExpandProduct>(ep, 1024, stream)) return rc;
+    } else {
+      constexpr int MT = 2;
+      const dim3 grid((T + 16 * MT - 1) / (16 * MT), (d + 511) / 512);
+      if (const int rc = launch_pdl(gate_dh_kernel<MT>, grid, dim3(256), 0, stream, d_logits,
+                                    static_cast<const __half*>(wg), T, d, E,
+                                    static_cast<__half*>(d_h)))
+        return rc;
     }
   }
-  if (d_h) {
-    constexpr int MT = 2;
-    const dim3 grid((T + 16 * MT - 1) / (16 * MT), (d + 511) / 512);
-    return launch_pdl(gate_dh_kernel<MT>, grid, dim3(256), 0, stream, d_logits,
-                      static_cast<const __half*>(wg), T, d, E, static_cast<__half*>(d_h));
+  if (d_wg) {
+    float* part = gp.splits > 1 ? reinterpret_cast<float*>(ws + gp.part) : d_wg;
+    const __half* hp = static_cast<const __half*>(h);
+    const int rc = E <= 8    ? launch_dw<1>(hp, sp.frag, sp.down, T, d, E, gp, part, stream)
+                   : E <= 16 ? launch_dw<2>(hp, sp.frag, sp.down, T, d, E, gp, part, stream)
+                   : E <= 32 ? launch_dw<4>(hp, sp.frag, sp.down, T, d, E, gp, part, stream)
+                             : launch_dw<8>(hp, sp.frag, sp.down, T, d, E, gp, part, stream);
+    if (rc != LR_OK) return rc;
+    const long n4 = gp.splits > 1 ? long(E) * d / 4 : 0;
+    const long sum_blocks = (n4 + 255) / 256, bias_blocks = d_bias ? (E + 7) / 8 : 0;
+    if (sum_blocks + bias_blocks > 0)
+      return launch_pdl(sum_parts_kernel, dim3(unsigned(sum_blocks + bias_blocks)), dim3(256), 0,
+                        stream, static_cast<const float*>(part), n4, gp.splits, sum_blocks, d_wg,
+                        static_cast<const float*>(sp.colsum), gp.chunks, E, gp.E8, d_bias);
   }
   return LR_OK;
 }
