@@ -446,17 +446,21 @@ __global__ void __launch_bounds__(256) gate_split_kernel(SplitArgs p) {
   const int chunk = blockIdx.x / p.groups, e0 = (blockIdx.x % p.groups) * 64;
   const int ne = min(64, p.E - e0), ne8 = min(64, p.E8 - e0);
   const long t0 = long(chunk) * kChunk;
-  for (int i = threadIdx.x; i < kChunk * 64; i += 256) {
-    const int t = i >> 6, e = i & 63;
+  const int lg = ne8 <= 8 ? 3 : ne8 <= 16 ? 4 : ne8 <= 32 ? 5 : 6;  // columns read: 2^lg >= ne8
+#pragma unroll 8
+  for (int i = threadIdx.x; i < (kChunk << lg); i += 256) {
+    const int t = i >> lg, e = i & ((1 << lg) - 1);
     s_dl[t][e] = t0 + t < p.T && e < ne ? __ldg(p.dl + size_t(t0 + t) * p.E + e0 + e) : 0.f;
   }
   __syncthreads();
   {
     const int e = threadIdx.x & 63, q = threadIdx.x >> 6;
     float m = 0.f, sum = 0.f;
-    for (int t = q; t < kChunk; t += 4) {
-      m = fmaxf(m, fabsf(s_dl[t][e]));
-      sum += s_dl[t][e];
+    if (e < ne8) {
+      for (int t = q; t < kChunk; t += 4) {
+        m = fmaxf(m, fabsf(s_dl[t][e]));
+        sum += s_dl[t][e];
+      }
     }
     s_red[q][e] = m;
     __syncthreads();
@@ -624,19 +628,35 @@ __global__ void __launch_bounds__(256)
     if (e < E && lane == 0) out_b[e] = s;
     return;
   }
-  const long i = long(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= n4) return;
-  const float4* q = reinterpret_cast<const float4*>(part) + i;
+  // 32 columns of four; warp w adds ranges w, w + 8, ..., then the warps in order
+  __shared__ float4 s_sum[8][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long i = long(blockIdx.x) * 32 + lane;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (i < n4) {
+    const float4* q = reinterpret_cast<const float4*>(part) + i;
 #pragma unroll 4
-  for (int k = 0; k < splits; ++k) {
-    const float4 v = q[size_t(k) * n4];
-    s.x += v.x;
-    s.y += v.y;
-    s.z += v.z;
-    s.w += v.w;
+    for (int k = warp; k < splits; k += 8) {
+      const float4 v = __ldcg(q + size_t(k) * n4);
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
   }
-  reinterpret_cast<float4*>(out)[i] = s;
+  s_sum[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && i < n4) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      const float4 v = s_sum[w][lane];
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    reinterpret_cast<float4*>(out)[i] = s;
+  }
 }
 
 // dh[T,d] = dl W, fp16 out, for more experts than the low-rank kernel takes (128).
@@ -708,15 +728,15 @@ struct GatePlan {
   size_t frag, down, colsum, wt, part, bytes;  // workspace offsets
 };
 
-// Token ranges of the weight gradient: as many chunks per block as keep two
-// blocks per SM.
+// Token ranges of the weight gradient: as many chunks per block as keep the SMs
+// full (two blocks on each up to 32 experts, whose stages leave room for two).
 static GatePlan gate_plan(int T, int d, int E) {
   GatePlan p;
   p.E8 = (E + 7) & ~7;
   p.groups = (E + 63) / 64;
   p.chunks = (T + kChunk - 1) / kChunk;
   const long cols = long((d + kDwCols - 1) / kDwCols) * p.groups;
-  p.per_block = int(p.chunks * cols / (2 * kTargetBlocks));
+  p.per_block = int(p.chunks * cols / (E > 32 ? kTargetBlocks : 2 * kTargetBlocks));
   if (p.per_block < 1) p.per_block = 1;
   p.splits = (p.chunks + p.per_block - 1) / p.per_block;
   p.frag = 0;
@@ -992,7 +1012,7 @@ extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_lo
                              : launch_dw<8>(hp, sp.frag, sp.down, T, d, E, gp, part, stream);
     if (rc != LR_OK) return rc;
     const long n4 = gp.splits > 1 ? long(E) * d / 4 : 0;
-    const long sum_blocks = (n4 + 255) / 256, bias_blocks = d_bias ? (E + 7) / 8 : 0;
+    const long sum_blocks = (n4 + 31) / 32, bias_blocks = d_bias ? (E + 7) / 8 : 0;
     if (sum_blocks + bias_blocks > 0)
       return launch_pdl(sum_parts_kernel, dim3(unsigned(sum_blocks + bias_blocks)), dim3(256), 0,
                         stream, static_cast<const float*>(part), n4, gp.splits, sum_blocks, d_wg,

@@ -145,6 +145,149 @@ __global__ void __launch_bounds__(kGateWarps * 32)
   }
 }
 
+// The same logits for large batches, bit for bit: warp w of a block owns the d-chunk
+// of warp w above and runs the same mma sequence over it, for MTL 16-token tiles
+// and NT 8-expert groups at once, and the chunks are added in the same order.
+// Only the operands' way differs: rows come in by 16-byte asynchronous copies, 32
+// k at a time into the warp's own ring, and reach the registers by ldmatrix (in
+// place of 4-byte loads from global memory).  16384 x 4096 rows, 8 experts: see
+// lr_gate_logits.
+constexpr int kGateTiledTokens = 2048;
+constexpr int kGlPitch = 80;  // bytes of a 32-k row in the ring: ldmatrix rows in different banks
+
+template <int MTL, int NT>
+constexpr int gate_tile_stages() {
+  return (MTL * 16 + NT * 8) * kGlPitch * kGateWarps * 4 <= 220 * 1024 ? 4 : 3;
+}
+
+LR_DEVICE void ldmatrix_x4(uint32_t (&r)[4], uint32_t saddr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(saddr));
+}
+LR_DEVICE void ldmatrix_x2(uint32_t (&r)[2], uint32_t saddr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(saddr));
+}
+
+template <int MTL, int NT>
+__global__ void __launch_bounds__(kGateWarps * 32)
+    gate_logits_tiled_kernel(const __half* __restrict__ h, const __half* __restrict__ wg,
+                             const float* __restrict__ bias, int T, int d, int E,
+                             float* __restrict__ logits) {
+  constexpr int TM = MTL * 16, EM = NT * 8, S = gate_tile_stages<MTL, NT>();
+  constexpr int kStageBytes = (TM + EM) * kGlPitch;
+  extern __shared__ __align__(16) unsigned char s_gl[];  // [warp][stage][rows of h, of wg]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const long t0 = long(blockIdx.x) * TM;
+  const int e0 = blockIdx.y * EM;
+  const int kc = ((d / 16 + kGateWarps - 1) / kGateWarps) * 16;
+  const int kbeg = min(d, warp * kc), kend = min(d, kbeg + kc);
+  const int stages = (kend - kbeg + 31) / 32;
+  unsigned char* ring = s_gl + warp * S * kStageBytes;
+  const auto fetch = [&](int i) {
+    if (i < stages) {
+      const uint32_t dst = smem_u32(ring + (i % S) * kStageBytes) + (lane >> 2) * kGlPitch +
+                           (lane & 3) * 16;
+      const int k = kbeg + i * 32 + (lane & 3) * 8;
+      const bool kok = k < kend;
+#pragma unroll
+      for (int r = 0; r < TM + EM; r += 8) {
+        const int row = r + (lane >> 2);
+        const bool ok = kok && (r < TM ? t0 + row < T : e0 + row - TM < E);
+        const __half* src = r < TM ? h + size_t(ok ? t0 + row : 0) * d
+                                   : wg + size_t(ok ? e0 + row - TM : 0) * d;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * kGlPitch),
+                     "l"(src + (ok ? k : 0)), "r"(ok ? 16 : 0)
+                     : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  float acc[MTL][NT][4];
+#pragma unroll
+  for (int m = 0; m < MTL; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch(i);
+  for (int i = 0; i < stages; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+    __syncwarp();
+    fetch(i + S - 1);  // into the stage read one iteration ago
+    const uint32_t sh = smem_u32(ring + (i % S) * kStageBytes);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (kbeg + i * 32 + u * 16 < kend) {
+        uint32_t b[NT][2];
+        if (NT == 1) {
+          ldmatrix_x2(b[0], sh + (TM + (lane & 7)) * kGlPitch + u * 32 + ((lane >> 3) & 1) * 16);
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; n += 2) {
+            uint32_t q[4];
+            ldmatrix_x4(q, sh + (TM + n * 8 + (lane & 7) + (lane >> 4) * 8) * kGlPitch + u * 32 +
+                               ((lane >> 3) & 1) * 16);
+            b[n][0] = q[0];
+            b[n][1] = q[1];
+            b[(n + 1) % NT][0] = q[2];
+            b[(n + 1) % NT][1] = q[3];
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < MTL; ++m) {
+          uint32_t a[4];
+          ldmatrix_x4(a, sh + (m * 16 + (lane & 15)) * kGlPitch + u * 32 + (lane >> 4) * 16);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816(acc[m][n], a, b[n][0], b[n][1]);
+        }
+      }
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(s_gl);  // [warp][TM][EM + 2]
+  constexpr int RP = EM + 2;
+#pragma unroll
+  for (int m = 0; m < MTL; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<float2*>(red + (warp * TM + m * 16 + g + 8 * i) * RP + n * 8 + 2 * tq) =
+            make_float2(acc[m][n][2 * i], acc[m][n][2 * i + 1]);
+  __syncthreads();
+  for (int o = threadIdx.x; o < TM * EM; o += kGateWarps * 32) {
+    const int rr = o / EM, cc = o % EM;
+    if (t0 + rr < T && e0 + cc < E) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kGateWarps; ++w) v += red[(w * TM + rr) * RP + cc];
+      if (bias) v += bias[e0 + cc];
+      logits[size_t(t0 + rr) * E + e0 + cc] = v;
+    }
+  }
+}
+
+template <int MTL, int NT>
+static int launch_gate_tiled(const __half* h, const __half* wg, const float* bias, int T, int d,
+                             int E, float* logits, cudaStream_t stream) {
+  constexpr int TM = MTL * 16, EM = NT * 8;
+  constexpr int ring = kGateWarps * gate_tile_stages<MTL, NT>() * (TM + EM) * kGlPitch;
+  constexpr int red = kGateWarps * TM * (EM + 2) * 4;
+  constexpr int smem = ring > red ? ring : red;
+  auto kern = gate_logits_tiled_kernel<MTL, NT>;
+  static unsigned long long configured = 0;
+  if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
+  kern<<<dim3(unsigned((T + TM - 1) / TM), (E + EM - 1) / EM), kGateWarps * 32, smem, stream>>>(
+      h, wg, bias, T, d, E, logits);
+  LR_LAUNCH_CHECK();
+  return LR_OK;
+}
+
 // ---------------------------------------------------------------------------
 // block-level slot ranking (shared by both route kernels)
 // ---------------------------------------------------------------------------
@@ -989,6 +1132,14 @@ extern "C" int lr_gate_logits(const void* h, const void* wg, const float* bias, 
   if (T < 0 || d <= 0 || d % 16 != 0 || E < 1 || E > 256) return LR_ERR_INVALID_ARGUMENT;
   if (T == 0) return LR_OK;
   if (!h || !wg || !logits) return LR_ERR_INVALID_ARGUMENT;
+  if (T >= kGateTiledTokens && aligned16(h) && aligned16(wg)) {
+    const __half* hp = static_cast<const __half*>(h);
+    const __half* wp = static_cast<const __half*>(wg);
+    return E <= 8    ? launch_gate_tiled<4, 1>(hp, wp, bias, T, d, E, logits, stream)
+           : E <= 16 ? launch_gate_tiled<4, 2>(hp, wp, bias, T, d, E, logits, stream)
+           : E <= 32 ? launch_gate_tiled<4, 4>(hp, wp, bias, T, d, E, logits, stream)
+                     : launch_gate_tiled<2, 8>(hp, wp, bias, T, d, E, logits, stream);
+  }
   const int n_eg = (E + 31) / 32;
   const long blocks = long((T + 15) / 16) * n_eg;
   gate_logits_kernel<<<unsigned(blocks), kGateWarps * 32, 0, stream>>>(static_cast<const __half*>(h),
