@@ -23,6 +23,9 @@ bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 
 // Contiguous, 16-byte aligned, of type `type` (a copy only where it is not already).
 at::Tensor rows16(const at::Tensor& t, at::ScalarType type) {
+  if (t.scalar_type() == type && t.is_contiguous() &&
+      (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0)
+    return t;
   at::Tensor r = t.detach().to(type).contiguous();
   if (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15u) r = r.clone(at::MemoryFormat::Contiguous);
   return r;
@@ -54,7 +57,7 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
     TORCH_CHECK(logits_in.dim() == 2 && logits_in.scalar_type() == at::kFloat,
                 "logits: (T,E) fp32");
     c10::cuda::CUDAGuard g(logits_in.device());
-    const at::Tensor logits = logits_in.detach().contiguous();
+    const at::Tensor logits = logits_in.is_contiguous() ? logits_in : logits_in.detach().contiguous();
     const int64_t T = logits.size(0), E = logits.size(1);
     TORCH_CHECK(E >= 1 && E <= 64 && k >= 1 && k <= 8 && k <= E,
                 "balanced_gating: 1 <= E <= 64 and 1 <= k <= min(E, 8) expected, got E=", E,
@@ -70,13 +73,15 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
     auto gw = at::empty({T * k}, logits.options());
     auto stats = at::empty({E + 1}, logits.options().dtype(at::kInt));
     auto aux = at::empty({}, logits.options());
-    auto ws = workspace(lr_balanced_gating_workspace_bytes(int(T), int(E)), logits);
+    const size_t wsb = lr_balanced_gating_workspace_bytes(int(T), int(E));
+    at::Tensor ws;
+    if (wsb) ws = workspace(wsb, logits);
     check_status(lr_balanced_gating(logits.data_ptr<float>(),
                                     mask.defined() ? static_cast<const uint8_t*>(mask.data_ptr())
                                                    : nullptr,
                                     int(T), int(E), int(k), float(lbw), ids.data_ptr<int32_t>(),
                                     gw.data_ptr<float>(), stats.data_ptr<int32_t>(),
-                                    aux.data_ptr<float>(), ws.data_ptr(), size_t(ws.numel()),
+                                    aux.data_ptr<float>(), wsb ? ws.data_ptr() : nullptr, wsb,
                                     cur_stream()),
                  "balanced_gating");
     ctx->mark_non_differentiable({ids, stats});
@@ -145,7 +150,7 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     ctx->set_materialize_grads(false);
     // an input that is used as it is goes in as the input, so that writing to it
     // before the backward pass is noticed
-    ctx->save_for_backward({hh.is_same(h) || hh.data_ptr() == h.data_ptr() ? h : hh,
+    ctx->save_for_backward({hh.data_ptr() == h.data_ptr() ? h : hh,
                             wh.data_ptr() == w.data_ptr() ? w : wh});
     ctx->saved_data["need_h"] = h.requires_grad();
     ctx->saved_data["need_w"] = w.requires_grad();

@@ -90,17 +90,19 @@ LR_DEVICE void row_softmax(const float* __restrict__ logits, int t, bool valid, 
   for (int i = 0; i < 8; ++i) p[i] = p[i] / z;
 }
 
-// counts[0..E), counts[E] = live tokens, and the loss, from totals in double.
-LR_DEVICE void write_gating_stats(int E, int k, float lbw, const double* s_p, const int32_t* s_c,
+// counts[0..E), counts[E] = live tokens, and the loss, from totals in double: a
+// thread per expert for the divisions, one for the sum in expert order.
+LR_DEVICE void write_gating_stats(int E, int k, float lbw, double* s_p, const int32_t* s_c,
                                   int32_t* __restrict__ counts, float* __restrict__ aux) {
+  const int n = s_c[E];
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
+    counts[e] = s_c[e];
+    if (e < E) s_p[e] = n > 0 ? (double(s_c[e]) / (double(n) * k)) * (s_p[e] / n) : 0.0;
+  }
+  __syncthreads();
   if (threadIdx.x == 0) {
-    const int n = s_c[E];
     double a = 0.0;
-    for (int e = 0; e < E; ++e) {
-      counts[e] = s_c[e];
-      if (n > 0) a += (double(s_c[e]) / (double(n) * k)) * (s_p[e] / n);
-    }
-    counts[E] = n;
+    for (int e = 0; e < E; ++e) a += s_p[e];
     aux[0] = static_cast<float>(double(lbw) * E * a);
   }
 }

@@ -324,7 +324,7 @@ LR_DEVICE int rank_chunk(int e, bool valid, int E, int32_t* s_wcnt, int32_t* s_r
 // writes offsets / kept_counts and the aux loss, resets the ticket.
 LR_DEVICE void route_tail(const RouteWs& ws, int B, int E, int C, int num_slots, int T, int k,
                           float lbw, int32_t* offsets, int32_t* kept_counts, float* aux_loss,
-                          double* prob_sums, int32_t* s_tot, double* s_P) {
+                          double* prob_sums, int32_t* s_tot, double* s_P, double* s_f) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int e = warp; e < E; e += kWarps) {
     int carry = 0;
@@ -350,18 +350,28 @@ LR_DEVICE void route_tail(const RouteWs& ws, int B, int E, int C, int num_slots,
     }
   }
   __syncthreads();
+  // a thread per expert divides; one thread then scans and sums in expert order
+  for (int e = tid; e < E; e += kRouteThreads) {
+    if (kept_counts) kept_counts[e] = min(s_tot[e], C);
+    if (prob_sums) prob_sums[e] = s_P[e];
+    if (aux_loss) {
+      s_f[e] = double(s_tot[e]) / double(num_slots);
+      s_P[e] = s_P[e] / double(T);
+    }
+  }
+  __syncthreads();
   if (tid == 0) {
     int run = 0;
-    double aux = 0.0;
     offsets[0] = 0;
     for (int e = 0; e < E; ++e) {
       run += s_tot[e];
       offsets[e + 1] = run;
-      if (kept_counts) kept_counts[e] = min(s_tot[e], C);
-      if (prob_sums) prob_sums[e] = s_P[e];
-      aux += (double(s_tot[e]) / double(num_slots)) * (s_P[e] / double(T));
     }
-    if (aux_loss) aux_loss[0] = static_cast<float>(double(lbw) * double(E) * aux);
+    if (aux_loss) {
+      double aux = 0.0;
+      for (int e = 0; e < E; ++e) aux = fma(s_f[e], s_P[e], aux);
+      aux_loss[0] = static_cast<float>(double(lbw) * double(E) * aux);
+    }
     *ws.ticket = 0;
     (void)k;
   }
@@ -459,7 +469,7 @@ __global__ void __launch_bounds__(kRouteThreads)
   __shared__ int32_t s_wcnt[kWarps * MAXE];
   __shared__ int32_t s_run[MAXE];
   __shared__ float s_pw[kWarps * MAXE];
-  __shared__ double s_P[MAXE];
+  __shared__ double s_P[MAXE], s_f[MAXE];
   __shared__ int32_t s_tot[MAXE];
   __shared__ int s_last;
 
@@ -474,8 +484,20 @@ __global__ void __launch_bounds__(kRouteThreads)
   {
     float l[MAXE];
     const float* row = logits + size_t(valid ? t : 0) * E;
+    if (E == MAXE && (reinterpret_cast<uintptr_t>(logits) & 15u) == 0) {
 #pragma unroll
-    for (int i = 0; i < MAXE; ++i) l[i] = (i < E && valid) ? __ldg(row + i) : 0.f;
+      for (int i = 0; i < MAXE; i += 4) {
+        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (valid) q = __ldg(reinterpret_cast<const float4*>(row + i));
+        l[i] = q.x;
+        l[i + 1] = q.y;
+        l[i + 2] = q.z;
+        l[i + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MAXE; ++i) l[i] = (i < E && valid) ? __ldg(row + i) : 0.f;
+    }
     int ids[kMaxTopK];
     float wsel[kMaxTopK];
     topk_softmax<MAXE>(l, E, k, p, ids, wsel);
@@ -521,7 +543,7 @@ __global__ void __launch_bounds__(kRouteThreads)
   }
   if (!arrive_last(ws.ticket, num_blocks, &s_last)) return;
   route_tail(ws, num_blocks, E, C, T * k, T, k, lbw, offsets, kept_counts, aux_loss, prob_sums,
-             s_tot, s_P);
+             s_tot, s_P, s_f);
 }
 
 // ---------------------------------------------------------------------------
@@ -560,7 +582,7 @@ __global__ void __launch_bounds__(kRouteThreads)
   for (int i = tid; i < E; i += kRouteThreads) ws.blk_counts[size_t(blockIdx.x) * E + i] = s_run[i];
   if (!arrive_last(ws.ticket, num_blocks, &s_last)) return;
   route_tail(ws, num_blocks, E, C, S, 1, 1, 0.f, offsets, kept_counts, nullptr, nullptr, s_tot,
-             s_P);
+             s_P, nullptr);
 }
 
 // ---------------------------------------------------------------------------
@@ -767,6 +789,7 @@ __global__ void __launch_bounds__(kRouteThreads)
   __shared__ int32_t s_run[MAXE];
   __shared__ int32_t s_off[MAXE];
   __shared__ float s_pw[kWarps * MAXE];
+  __shared__ double s_f[MAXE], s_Pm[MAXE];
   __shared__ int s_last;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
@@ -875,22 +898,30 @@ __global__ void __launch_bounds__(kRouteThreads)
     if (sv) s_rank[ls] = r;
   }
   // s_run[e] now counts expert e's slots (uncapped)
+  // (a thread per expert divides; one thread then scans and sums in expert order)
+  if (tid < E) {
+    if (kept_counts) kept_counts[tid] = min(s_run[tid], C);
+    if (aux_loss) {
+      double P = 0.0;
+      for (int w = 0; w < kWarps; ++w) P += double(s_pw[w * E + tid]);
+      s_f[tid] = double(s_run[tid]) / double(nslots);
+      s_Pm[tid] = P / double(T);
+    }
+  }
+  __syncthreads();
   if (tid == 0) {
     int run = 0;
-    double aux = 0.0;
     offsets[0] = 0;
     for (int e = 0; e < E; ++e) {
       s_off[e] = run;
       run += s_run[e];
       offsets[e + 1] = run;
-      if (kept_counts) kept_counts[e] = min(s_run[e], C);
-      if (aux_loss) {
-        double P = 0.0;
-        for (int w = 0; w < kWarps; ++w) P += double(s_pw[w * E + e]);
-        aux += (double(s_run[e]) / double(nslots)) * (P / double(T));
-      }
     }
-    if (aux_loss) aux_loss[0] = static_cast<float>(double(lbw) * double(E) * aux);
+    if (aux_loss) {
+      double aux = 0.0;
+      for (int e = 0; e < E; ++e) aux = fma(s_f[e], s_Pm[e], aux);
+      aux_loss[0] = static_cast<float>(double(lbw) * double(E) * aux);
+    }
     *ws.ticket = 0;
   }
   __syncthreads();
