@@ -326,7 +326,7 @@ LR_DEVICE void route_tail(const RouteWs& ws, int B, int E, int C, int num_slots,
                           float lbw, int32_t* offsets, int32_t* kept_counts, float* aux_loss,
                           double* prob_sums, int32_t* s_tot, double* s_P, double* s_f) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int e = warp; e < E; e += kWarps) {
+  for (int e = warp; e < E; e += blockDim.x / 32) {
     int carry = 0;
     double psum = 0.0;
     for (int b0 = 0; b0 < B; b0 += 32) {
@@ -351,7 +351,7 @@ LR_DEVICE void route_tail(const RouteWs& ws, int B, int E, int C, int num_slots,
   }
   __syncthreads();
   // a thread per expert divides; one thread then scans and sums in expert order
-  for (int e = tid; e < E; e += kRouteThreads) {
+  for (int e = tid; e < E; e += blockDim.x) {
     if (kept_counts) kept_counts[e] = min(s_tot[e], C);
     if (prob_sums) prob_sums[e] = s_P[e];
     if (aux_loss) {
@@ -533,6 +533,204 @@ __global__ void __launch_bounds__(kRouteThreads)
     if (sv) slot_rank[slot0 + ls] = r;
   }
   for (int i = tid; i < E; i += kRouteThreads) {
+    ws.blk_counts[size_t(blockIdx.x) * E + i] = s_run[i];
+    if (want_p) {
+      double sum = 0.0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum += double(s_pw[w * E + i]);
+      ws.blk_psum[size_t(blockIdx.x) * E + i] = sum;
+    }
+  }
+  if (!arrive_last(ws.ticket, num_blocks, &s_last)) return;
+  route_tail(ws, num_blocks, E, C, T * k, T, k, lbw, offsets, kept_counts, aux_loss, prob_sums,
+             s_tot, s_P, s_f);
+}
+
+// The same for more than 8 experts, bit for bit, with a token's logits spread over
+// LPT lanes (8 neighbouring experts each): the one-thread form above unrolls 64
+// experts times k selections into more instructions than the caches hold (777
+// tokens, 64 experts, top-6: 60 us).  The softmax denominator runs through the
+// lanes in expert order and the probability sums follow the shuffle tree of
+// warp_prob_sums, so sums keep their order; a NaN is selected where the scan of
+// topk_softmax would (as the first expert not yet taken).
+template <int LPT>
+constexpr int route_lanes_threads() {
+  return 256 * LPT < 1024 ? 256 * LPT : 1024;
+}
+
+template <int LPT>
+__global__ void __launch_bounds__(route_lanes_threads<LPT>())
+    topk_route_lanes_kernel(const float* __restrict__ logits, int T, int E, int k, int C, float lbw,
+                            int32_t* __restrict__ expert_ids, float* __restrict__ gate_w,
+                            int32_t* __restrict__ token_idx, int32_t* __restrict__ slot_rank,
+                            int32_t* __restrict__ offsets, int32_t* __restrict__ kept_counts,
+                            float* __restrict__ aux_loss, double* __restrict__ prob_sums,
+                            RouteWs ws, int num_blocks) {
+  constexpr int MAXE = 8 * LPT;
+  constexpr int kThreads = route_lanes_threads<LPT>();
+  constexpr int kTok = kThreads / LPT;  // tokens at a time
+  __shared__ int32_t s_ids[kRouteThreads * kMaxTopK];
+  __shared__ int32_t s_wcnt[kWarps * MAXE];
+  __shared__ int32_t s_run[MAXE];
+  __shared__ float s_pw[kWarps * MAXE];
+  __shared__ float s_p[kTok][MAXE + 1];
+  __shared__ double s_P[MAXE], s_f[MAXE];
+  __shared__ int32_t s_tot[MAXE];
+  __shared__ int s_last;
+
+  const int tid = threadIdx.x, lane = tid & 31, l = tid % LPT;
+  const int group0 = lane & ~(LPT - 1);
+  const int ntok = min(kRouteThreads, T - int(blockIdx.x) * kRouteThreads);
+  const int nslots = ntok * k;
+  const bool want_p = aux_loss != nullptr || prob_sums != nullptr;
+  const bool vec = E % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & 15u) == 0;
+  for (int i = tid; i < E; i += kThreads) s_run[i] = 0;
+
+  for (int it = 0; it * kTok < ntok; ++it) {
+    const int lt = it * kTok + tid / LPT;
+    const bool valid = lt < ntok;
+    const long t = long(blockIdx.x) * kRouteThreads + lt;
+    const float* row = logits + size_t(valid ? t : 0) * E + 8 * l;
+    float v[8], p[8];
+#pragma unroll
+    for (int c = 0; c < 8; c += 4) {
+      if (vec) {
+        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (valid && 8 * l + c < E) q = __ldg(reinterpret_cast<const float4*>(row + c));
+        v[c] = q.x;
+        v[c + 1] = q.y;
+        v[c + 2] = q.z;
+        v[c + 3] = q.w;
+      } else {
+#pragma unroll
+        for (int i = c; i < c + 4; ++i) v[i] = valid && 8 * l + i < E ? __ldg(row + i) : 0.f;
+      }
+    }
+    float m = __int_as_float(0x7fffffff);  // NaN: fmaxf passes it over
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (8 * l + i < E) {
+        m = fmaxf(m, v[i]);
+        nan = nan || v[i] != v[i];
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < LPT; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = 8 * l + i < E ? expf(v[i] - m) : 0.f;
+    float z = 0.f;
+#pragma unroll
+    for (int s = 0; s < LPT; ++s) {
+      if (l == s) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z += p[i];
+      }
+      z = __shfl_sync(0xffffffffu, z, group0 + s);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = 8 * l + i < E ? p[i] / z : 0.f;
+    const bool row_nan = (__ballot_sync(0xffffffffu, nan) >> group0 & ((1u << LPT) - 1u)) != 0;
+
+    unsigned taken = 0;
+    int ids[kMaxTopK];
+    float psel[kMaxTopK];
+    float ssum = 0.f;
+#pragma unroll
+    for (int j = 0; j < kMaxTopK; ++j) {
+      if (j < k) {
+        // largest (ordered logit, lowest expert first) key; NaN below every number
+        unsigned long long best = 0;
+        int first = MAXE;  // the first expert not yet taken, in this lane
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+          const int e = 8 * l + i;
+          if (e < E && !((taken >> i) & 1u)) {
+            uint32_t u = __float_as_uint(v[i] + 0.f);
+            u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+            if (v[i] != v[i]) u = 0u;
+            const unsigned long long key =
+                (static_cast<unsigned long long>(u) << 32) | (0xffffffffu - unsigned(e));
+            if (key > best) best = key;
+            first = e;
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < LPT; o <<= 1) {
+          const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+          if (other > best) best = other;
+        }
+        int e = int(0xffffffffu - unsigned(best));
+        if (__any_sync(0xffffffffu, row_nan)) {
+#pragma unroll
+          for (int o = 1; o < LPT; o <<= 1)
+            first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+          float fv = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (8 * l + i == first) fv = v[i];
+          fv = __shfl_sync(0xffffffffu, fv, group0 + first / 8);
+          if (fv != fv) e = first;
+        }
+        float pe = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (8 * l + i == e) {
+            taken |= 1u << i;
+            pe = p[i];
+          }
+        }
+        pe = __shfl_sync(0xffffffffu, pe, group0 + e / 8);
+        ids[j] = e;
+        psel[j] = pe;
+        ssum += pe;
+      }
+    }
+    const float denom = ssum + 1e-9f;
+    if (valid) {
+#pragma unroll
+      for (int j = 0; j < kMaxTopK; ++j) {
+        if (j < k && j % LPT == l) {
+          const size_t s = size_t(t) * k + j;
+          s_ids[lt * k + j] = ids[j];
+          expert_ids[s] = ids[j];
+          gate_w[s] = psel[j] / denom;
+          if (token_idx) token_idx[s] = int(t);
+        }
+      }
+    }
+    if (want_p) {
+      if (it > 0) __syncthreads();  // the last tokens' sums are taken
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s_p[tid / LPT][8 * l + i] = valid ? p[i] : 0.f;
+      __syncthreads();
+      for (int i = tid; i < kTok / 32 * E; i += kThreads) {
+        const int w = i / E, e = i % E;
+        float a[16];
+#pragma unroll
+        for (int x = 0; x < 16; ++x) a[x] = s_p[w * 32 + x][e] + s_p[w * 32 + x + 16][e];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+          for (int x = 0; x < o; ++x) a[x] += a[x + o];
+        s_pw[(it * (kTok / 32) + w) * E + e] = a[0];
+      }
+    }
+  }
+  if (want_p)  // warps of tokens past the end
+    for (int i = tid; i < kWarps * E; i += kThreads)
+      if (i / E * 32 >= (ntok + kTok - 1) / kTok * kTok) s_pw[i] = 0.f;
+  __syncthreads();
+
+  const size_t slot0 = size_t(blockIdx.x) * kRouteThreads * k;
+  for (int c = 0; c < k; ++c) {
+    const int ls = c * kRouteThreads + tid;  // the block's first 256 threads rank
+    const bool sv = tid < kRouteThreads && ls < nslots;
+    const int e = sv ? s_ids[ls] : -1;
+    const int r = rank_chunk(e, sv, E, s_wcnt, s_run);
+    if (sv) slot_rank[slot0 + ls] = r;
+  }
+  for (int i = tid; i < E; i += kThreads) {
     ws.blk_counts[size_t(blockIdx.x) * E + i] = s_run[i];
     if (want_p) {
       double sum = 0.0;
@@ -1201,18 +1399,18 @@ extern "C" int lr_topk_route(const float* logits, int T, int E, int k, int capac
   if (!workspace || workspace_bytes < route_ws_bytes_for(B, E, true)) return LR_ERR_WORKSPACE;
   RouteWs ws = carve_route_ws(workspace, B, E, true);
   LR_CUDA_TRY(cudaMemsetAsync(ws.ticket, 0, sizeof(int32_t), stream));
-#define LR_ROUTE_CASE(ME)                                                                      \
-  topk_route_kernel<ME><<<B, kRouteThreads, 0, stream>>>(                                      \
+#define LR_ROUTE_CASE(KERNEL, THREADS)                                                         \
+  KERNEL<<<B, THREADS, 0, stream>>>(                                      \
       logits, T, E, k, capacity, load_balance_weight, expert_ids, gate_weights, token_indices, \
       slot_pos, offsets, kept_counts, aux_loss, prob_sums, ws, B)
   if (E <= 8)
-    LR_ROUTE_CASE(8);
+    LR_ROUTE_CASE(topk_route_kernel<8>, kRouteThreads);
   else if (E <= 16)
-    LR_ROUTE_CASE(16);
+    LR_ROUTE_CASE(topk_route_lanes_kernel<2>, route_lanes_threads<2>());
   else if (E <= 32)
-    LR_ROUTE_CASE(32);
+    LR_ROUTE_CASE(topk_route_lanes_kernel<4>, route_lanes_threads<4>());
   else
-    LR_ROUTE_CASE(64);
+    LR_ROUTE_CASE(topk_route_lanes_kernel<8>, route_lanes_threads<8>());
 #undef LR_ROUTE_CASE
   LR_LAUNCH_CHECK();
   return LR_OK;
