@@ -35,26 +35,20 @@ struct ShrinkArgs {
   int32_t* err;
 };
 
+// The window's groups [base0, s.n) in rounds: a round's groups share the block's
+// warps, 2^n warps splitting K for a group.
 template <int RB, int NT>
-__global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p, int rank_groups) {
+LR_DEVICE void shrink_groups(const ShrinkArgs& p, const Groups& s, float* s_part, long row0,
+                             int bank, int rank0, int base0, int per_round) {
   constexpr int W = 8 * NT;
   constexpr int RK = 16 * RB;
   constexpr int PITCH = W + 2;
   // k-blocks whose loads are in flight together: 12 to 16 16-byte loads per lane
-  constexpr int U = NT == 1 ? (RB == 1 ? 4 : RB == 2 ? 3 : 2) : (RB == 4 ? 1 : 2);
-  extern __shared__ float s_part[];  // [kAdWarps][RK][PITCH]
-  __shared__ Groups s;
-  pdl_wait();
-  pdl_trigger();
+  constexpr int U = NT == 1 ? (RB == 1 ? 4 : RB == 2 ? 3 : 2) : 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const int cs = int(cluster_nctarank()), cr = int(cluster_ctarank());
-  const long row0 = long(blockIdx.x / cs) * W;
-  const int bank = blockIdx.y / rank_groups, rank0 = (blockIdx.y % rank_groups) * RK;
-  const int per_round = kAdWarps / gridDim.z;  // groups a block takes at a time
-  if (warp == 0) group_rows<W>(s, p.index, row0, p.R, p.n, false, bank == 0 ? p.err : nullptr);
-  __syncthreads();
   const int nb = (p.K + 31) / 32;
-  for (int base = blockIdx.z * per_round; base < s.n; base += kAdWarps) {
+  for (int base = base0; base < s.n; base += kAdWarps) {
     const int ng = min(per_round, s.n - base);
     const int wpg = warps_per_group(ng);
     const int grp = warp / wpg, sub = warp % wpg;
@@ -170,6 +164,163 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
   }
 }
 
+// Small batches: windows of 8 rows; the grid's z deals a window's groups out to blocks.
+template <int RB>
+__global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p, int rank_groups) {
+  constexpr int RK = 16 * RB;
+  extern __shared__ __align__(128) unsigned char s_dyn[];  // [kAdWarps][RK][10] floats
+  __shared__ Groups s;
+  const int cs = int(cluster_nctarank());
+  const long row0 = long(blockIdx.x / cs) * 8;
+  const int bank = blockIdx.y / rank_groups, rank0 = (blockIdx.y % rank_groups) * RK;
+  const int per_round = kAdWarps / gridDim.z;  // groups a block takes at a time
+  pdl_wait();
+  pdl_trigger();
+  if (threadIdx.x < 32)
+    group_rows<8>(s, p.index, row0, p.R, p.n, false, bank == 0 ? p.err : nullptr);
+  __syncthreads();
+  shrink_groups<RB, 1>(p, s, reinterpret_cast<float*>(s_dyn), row0, bank, rank0,
+                       blockIdx.z * per_round, per_round);
+}
+
+// Larger batches: windows of 64 rows.  A window with one adapter (a prompt's rows)
+// streams tiles of 128 k, its rows of x and the adapter's rows of A, through a ring
+// of cp.async stages; warp w multiplies 32 of the 128 k (w & 3) for half of the
+// rows (w >> 2).  (Bulk copies of these 256-byte rows measured 127 us at 16384 x
+// 4096, rank 32: the copy engine takes about 25 ns per row.)  A mixed window
+// takes its halves through shrink_groups.
+constexpr int kTileK = 128;
+constexpr int kTileKPitch = kTileK * 2 + 64;  // bytes; neighbouring rows in different banks
+
+template <int RB>
+constexpr int shrink_stages() {
+  return 3;
+}
+template <int RB>
+constexpr int shrink_smem_bytes() {
+  constexpr int ring = shrink_stages<RB>() * (64 + 16 * RB) * kTileKPitch;
+  constexpr int part = kAdWarps * 16 * RB * 34 * int(sizeof(float));
+  return ring > part ? ring : part;
+}
+
+template <int RB>
+__global__ void __launch_bounds__(kAdThreads, RB == 4 ? 1 : 2)
+    adapter_shrink_stream_kernel(ShrinkArgs p, int rank_groups) {
+  constexpr int RK = 16 * RB, S = shrink_stages<RB>(), PITCH = 34;
+  constexpr int kStageBytes = (64 + RK) * kTileKPitch;
+  extern __shared__ __align__(128) unsigned char s_dyn[];  // ring, then the warps' sums
+  __shared__ Groups s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const int cs = int(cluster_nctarank()), cr = int(cluster_ctarank());
+  const long row0 = long(blockIdx.x / cs) * 64;
+  const int nrows = int(min(64l, p.R - row0));
+  const int bank = blockIdx.y / rank_groups, rank0 = (blockIdx.y % rank_groups) * RK;
+  float* s_part = reinterpret_cast<float*>(s_dyn);
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) group_rows<64>(s, p.index, row0, p.R, p.n, false, bank == 0 ? p.err : nullptr);
+  __syncthreads();
+  if (!s.uniform) {
+    for (int half = 0; half < 2; ++half) {
+      __syncthreads();
+      if (warp == 0)
+        group_rows<32>(s, p.index, row0 + 32 * half, p.R, p.n, false, nullptr);
+      __syncthreads();
+      shrink_groups<RB, 4>(p, s, s_part, row0 + 32 * half, bank, rank0, 0, kAdWarps);
+    }
+    return;
+  }
+  const int all = (p.K + kTileK - 1) / kTileK;
+  const int tile0 = int(long(all) * cr / cs), tiles = int(long(all) * (cr + 1) / cs) - tile0;
+  const __half* ap = (bank ? p.a[1] : p.a[0]) + (size_t(s.adapter[0]) * p.r + rank0) * p.K;
+  const int ranks = min(RK, p.r - rank0);
+  const auto fetch = [&](int i) {  // tile i into its stage: 16 lanes per row, zeros past the ends
+    if (i < tiles) {
+      const int k = (tile0 + i) * kTileK + (threadIdx.x & 15) * 8;
+      unsigned char* to = s_dyn + (i % S) * kStageBytes + (threadIdx.x & 15) * 16;
+#pragma unroll
+      for (int u = 0; u < 64 + RK; u += 16) {
+        const int row = u + (threadIdx.x >> 4);
+        const bool ok = k < p.K && (u < 64 ? row < nrows : row - 64 < ranks);
+        const __half* from = u < 64 ? p.x + size_t(row0 + row) * p.K : ap + size_t(row - 64) * p.K;
+        cp_async_16_zfill(to + row * kTileKPitch, ok ? from + k : p.x, ok);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) fetch(i);
+  const int kq = warp & 3, half = warp >> 2;
+  float acc[RB][4][4];
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+  for (int i = 0; i < tiles; ++i) {
+    cp_async_wait_group<S - 2>();
+    __syncthreads();
+    fetch(i + S - 1);  // into the stage read one tile ago
+    const int st = i % S;
+    const unsigned char* from = s_dyn + st * kStageBytes + kq * 64 + tq * 16;
+    uint4 av[2 * RB], xv[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      xv[j] = *reinterpret_cast<const uint4*>(from + (half * 32 + j * 8 + g) * kTileKPitch);
+#pragma unroll
+    for (int j = 0; j < 2 * RB; ++j)
+      av[j] = *reinterpret_cast<const uint4*>(from + (64 + j * 8 + g) * kTileKPitch);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const uint4 lo = av[2 * r], hi = av[2 * r + 1], x = xv[j];
+        mma_f16(acc[r][j], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+        mma_f16(acc[r][j], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+      }
+  }
+  cp_async_wait_all();
+  __syncthreads();  // every tile is read: the ring becomes the warps' sums [warp][RK][PITCH]
+  float* mine = s_part + warp * RK * PITCH;
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<float2*>(mine + (i * 16 + g + 8 * c) * PITCH + j * 8 + 2 * tq) =
+            make_float2(acc[i][j][2 * c], acc[i][j][2 * c + 1]);
+  __syncthreads();
+  // the four k-quarters, then the blocks of the cluster, in order
+  for (int o = threadIdx.x; o < 64 * RK; o += kAdThreads) {
+    const int t = o / RK, i = o % RK;
+    if (t >= nrows || i >= ranks) continue;
+    float* at = s_part + ((t >> 5) * 4 * RK + i) * PITCH + (t & 31);
+    const float sum = ((at[0] + at[RK * PITCH]) + at[2 * RK * PITCH]) + at[3 * RK * PITCH];
+    if (cs == 1)
+      p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
+    else
+      *at = sum;
+  }
+  if (cs > 1) {
+    cluster_sync();
+    for (int o = cr * kAdThreads + threadIdx.x; o < 64 * RK; o += cs * kAdThreads) {
+      const int t = o / RK, i = o % RK;
+      if (t >= nrows || i >= ranks) continue;
+      const uint32_t at = smem_u32(s_part + ((t >> 5) * 4 * RK + i) * PITCH + (t & 31));
+      float q[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) q[c] = c < cs ? ld_cluster_f32(at, c) : 0.f;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) sum += q[c];
+      p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
+    }
+    cluster_sync();  // the sums stay until every block of the cluster has read them
+  }
+}
+
 // ---------------------------------------------------------------------------
 // adapter numbers of the expert rows
 // ---------------------------------------------------------------------------
@@ -237,31 +388,34 @@ static int launch_cluster(void (*kern)(KArgs...), dim3 grid, unsigned cluster, s
 
 constexpr long kSmallRows = 256;  // up to here windows of 8 (shrink) and 16 rows (expand)
 
-template <int RB, int NT>
+template <int RB>
 static int launch_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
-  constexpr int W = 8 * NT, RK = 16 * RB;
-  constexpr int smem = kAdWarps * RK * (W + 2) * int(sizeof(float));
-  auto kern = adapter_shrink_kernel<RB, NT>;
-  static unsigned long long configured = 0;
-  if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
+  const bool small = p.R <= kSmallRows;
+  const int W = small ? 8 : 64, RK = 16 * RB;
+  const int smem = small ? kAdWarps * RK * 10 * int(sizeof(float)) : shrink_smem_bytes<RB>();
   const long windows = (p.R + W - 1) / W;
   const int rank_groups = (p.r + RK - 1) / RK;
-  // fill the SMs by splitting K over a cluster, then a window's groups over blocks
+  // fill one wave of blocks by splitting K over a cluster, then (small batches) a
+  // window's groups over blocks
+  const long fill = kTargetBlocks * (!small && RB == 4 ? 1 : 2);
+  const long blocks = windows * rank_groups * banks;
   unsigned cs = 1, gs = 1;
-  while (cs < 8 && windows * rank_groups * banks * cs < kTargetBlocks) cs *= 2;
-  while (gs < 4 && gs < p.R && windows * rank_groups * banks * cs * gs < kTargetBlocks) gs *= 2;
+  while (cs < 8 && blocks * cs * 2 <= fill) cs *= 2;
+  while (small && gs < 4 && gs < p.R && blocks * cs * gs * 2 <= fill) gs *= 2;
   if (windows * cs > 0x7fffffffL) return LR_ERR_INVALID_ARGUMENT;
-  return launch_cluster(kern, dim3(unsigned(windows * cs), rank_groups * banks, gs), cs, smem,
-                        stream, p, rank_groups);
+  const dim3 grid(unsigned(windows * cs), rank_groups * banks, gs);
+  if (small)
+    return launch_cluster(adapter_shrink_kernel<RB>, grid, cs, smem, stream, p, rank_groups);
+  static unsigned long long configured = 0;
+  if (const int rc = set_dyn_smem_once(adapter_shrink_stream_kernel<RB>, smem, configured))
+    return rc;
+  return launch_cluster(adapter_shrink_stream_kernel<RB>, grid, cs, smem, stream, p, rank_groups);
 }
 
 static int run_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
-  const bool small = p.R <= kSmallRows;
-  if (p.r <= 16)
-    return small ? launch_shrink<1, 1>(p, banks, stream) : launch_shrink<1, 4>(p, banks, stream);
-  if (p.r <= 32)
-    return small ? launch_shrink<2, 1>(p, banks, stream) : launch_shrink<2, 4>(p, banks, stream);
-  return small ? launch_shrink<4, 1>(p, banks, stream) : launch_shrink<4, 4>(p, banks, stream);
+  return p.r <= 16   ? launch_shrink<1>(p, banks, stream)
+         : p.r <= 32 ? launch_shrink<2>(p, banks, stream)
+                     : launch_shrink<4>(p, banks, stream);
 }
 
 static int check_adapter_args(const void* x, long R, int K, const int32_t* index, int n, int r,
@@ -303,7 +457,7 @@ extern "C" int lr_adapter_add(const void* x, int R, int K, const int32_t* index,
   ExpandArgs ep{sp.v, {static_cast<const __half*>(b), nullptr}, {scale, nullptr}, index,
                 {static_cast<const __half*>(base), nullptr}, static_cast<__half*>(out), R, N,
                 num_adapters, rank, rank, 0, base == out, err};
-  return run_expand<kExpandAdd>(ep, kSmallRows, stream);
+  return run_expand<kExpandAdd>(ep, stream);
 }
 
 extern "C" int lr_adapter_swiglu(const void* x, int R, int K, const int32_t* index,
@@ -327,7 +481,7 @@ extern "C" int lr_adapter_swiglu(const void* x, int R, int K, const int32_t* ind
                 {scale_gate, scale_up}, index,
                 {static_cast<const __half*>(gate), static_cast<const __half*>(up)},
                 static_cast<__half*>(out), R, N, num_adapters, rank, rank, 0, false, err};
-  return run_expand<kExpandSwiglu>(ep, kSmallRows, stream);
+  return run_expand<kExpandSwiglu>(ep, stream);
 }
 
 extern "C" int lr_adapter_rows(const int32_t* adapter_ids, int T, int num_adapters,

@@ -89,6 +89,10 @@ template <int N>
 LR_DEVICE void cp_async_wait_group() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// Arrives on an mbarrier when this thread's earlier cp.async have landed.
+LR_DEVICE void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 LR_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // silu(gate) * up of eight fp16 values
 LR_DEVICE uint4 swiglu8(const uint4& gate, const uint4& up) {
@@ -285,7 +289,8 @@ constexpr int expand_ahead() {
 }
 
 // Larger windows stream the base rows: stages of the window's rows x 256 columns
-// by bulk copies of a producer warp, a consumer warp per 32 columns.
+// by cp.async of a producer warp, a row per instruction, a consumer warp per 32
+// columns.
 constexpr int kTileCols = 256;
 constexpr int kTileGroups = kTileCols / 32;
 constexpr int kTilePitch = kTileCols * 2 + 64;  // bytes; neighbouring rows in different banks
@@ -311,7 +316,8 @@ constexpr int expand_threads() {
 // Nine warps leave 96 registers a thread to two blocks on an SM: enough up to rank 32.
 template <int RV, int MT, int MODE>
 constexpr int expand_min_blocks() {
-  return MODE == kExpandSwiglu || RV > 64 ? 1 : RV > 32 && MT > 1 && MODE == kExpandAdd ? 1 : 2;
+  if (MT == 1) return RV <= (MODE == kExpandSwiglu ? 32 : 64) ? 2 : 1;
+  return MODE == kExpandSwiglu || RV > 64 ? 1 : RV > 32 && MODE == kExpandAdd ? 1 : 2;
 }
 
 // Eight results of a row: base (and base2) with the scaled sums of both banks.
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
     group_rows<W>(s, p.index, row0, p.R, p.n, !p.in_place, nullptr);
   if (MT > 1 && MODE != kExpandProduct && threadIdx.x == 32) {
     for (int i = 0; i < kTileStages; ++i) {
-      mbar_init(s_full + i, 1);
+      mbar_init(s_full + i, 32);  // the producer's lanes
       mbar_init(s_empty + i, kAdWarps);
     }
     s_abort = 0;
@@ -369,26 +375,28 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
   __syncthreads();
   const bool stream = MT > 1 && MODE != kExpandProduct && s.uniform;
 
-  // Producer: tiles [first, last) of the base rows as bulk copies, each as soon as
-  // its stage has been read.  The first stages start ahead of everything else.
+  // Producer: tiles [first, last) of the base rows, each as soon as its stage has
+  // been read.  The first stages start ahead of everything else.
   const int n_tiles = (cg1 - cg0 + kTileGroups - 1) / kTileGroups;
   const auto produce = [&](int first, int last) {
     for (int i = first; i < last; ++i) {
       const int st = i % kTileStages, round = i / kTileStages, cg = cg0 + i * kTileGroups;
       if (round > 0 &&
           !mbar_wait_bounded(s_empty + st, (round - 1) & 1, &s_abort, p.err, kCopyWaitNs))
-        return i;
+        return;
       __syncwarp();
-      const unsigned bytes = unsigned(min(kTileCols, p.N - cg * 32)) * 2u;
-      if (lane == 0) mbar_arrive_expect_tx(s_full + st, bytes * nrows * BANKS);
-      __syncwarp();
+      if (cg * 32 + lane * 8 < p.N) {
 #pragma unroll
-      for (int bk = 0; bk < BANKS; ++bk)
-        for (int t = lane; t < nrows; t += 32)
-          bulk_load(s_dyn + ((st * BANKS + bk) * W + t) * kTilePitch,
-                    p.base[bk] + size_t(row0 + t) * p.N + cg * 32, bytes, s_full + st);
+        for (int bk = 0; bk < BANKS; ++bk) {
+          const __half* from = p.base[bk] + size_t(row0) * p.N + cg * 32 + lane * 8;
+          unsigned char* to = s_dyn + (st * BANKS + bk) * W * kTilePitch + lane * 16;
+#pragma unroll 8
+          for (int t = 0; t < nrows; ++t)
+            cp_async_16(to + t * kTilePitch, from + size_t(unsigned(t) * unsigned(p.N)));
+        }
+      }
+      cp_async_arrive(s_full + st);
     }
-    return last;
   };
   if (stream && warp == kAdWarps) produce(0, min(n_tiles, kTileStages));
   if (threadIdx.x < kAdThreads) {  // v: fp32 -> scaled (value, remainder) pairs in fragment order
@@ -446,12 +454,8 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
     // One entry of b for the whole window (a prompt's rows): a warp takes every
     // eighth column group for all rows.
     if (warp == kAdWarps) {
-      const int issued = produce(min(n_tiles, kTileStages), n_tiles);
-      // the last copies arrive before the block's shared memory goes
-      int none = 0;
-      for (int i = max(0, issued - kTileStages); i < issued; ++i)
-        mbar_wait_bounded(s_full + i % kTileStages, (i / kTileStages) & 1, &none, p.err,
-                          kCopyWaitNs);
+      produce(min(n_tiles, kTileStages), n_tiles);
+      cp_async_wait_all();  // leave no copy behind
       return;
     }
     const int ad = MODE == kExpandProduct ? 0 : s.adapter[0];
@@ -653,20 +657,28 @@ static int launch_expand(ExpandArgs p, cudaStream_t stream) {
   if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
   const long windows = (p.R + W - 1) / W;
   const int cgs = (p.N + 31) / 32;
-  // 256 columns per block, more while the grid stays above eight blocks per SM
   int gpc = kTileGroups;
-  while (gpc < 64 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
+  if (MT == 1) {
+    // one wave of two blocks per SM where that leaves a block 8 to 64 groups
+    const long per = (windows * cgs + 2 * kTargetBlocks - 1) / (2 * kTargetBlocks);
+    gpc = int(per < 8 ? 8 : per > 64 ? 64 : per);
+  } else {
+    // 256 columns per block, more while the grid stays above eight blocks per SM
+    while (gpc < 64 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
+  }
   p.groups_per_chunk = gpc;
   if (windows > 0x7fffffffL || (cgs + gpc - 1) / gpc > 65535) return LR_ERR_INVALID_ARGUMENT;
   return launch_pdl(kern, dim3(unsigned(windows), (cgs + gpc - 1) / gpc),
                     dim3(expand_threads<MT, MODE>()), smem, stream, p);
 }
 
-// Row windows of 16 up to `small_rows` rows, else of 64 (32 for SwiGLU).
+// Row windows of 64 (32 for SwiGLU), or of 16 while the larger ones would leave
+// fewer than two blocks of 256 columns for an SM.
 template <int MODE>
-static int run_expand(const ExpandArgs& p, long small_rows, cudaStream_t stream) {
+static int run_expand(const ExpandArgs& p, cudaStream_t stream) {
   constexpr int MT = MODE == kExpandSwiglu ? 2 : 4;
-  const bool small = p.R <= small_rows;
+  const long blocks = (p.R + 16 * MT - 1) / (16 * MT) * ((p.N + kTileCols - 1) / kTileCols);
+  const bool small = blocks < 2 * kTargetBlocks;
   if (p.r <= 16)
     return small ? launch_expand<16, 1, MODE>(p, stream) : launch_expand<16, MT, MODE>(p, stream);
   if (p.r <= 32)

@@ -995,7 +995,7 @@ extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_lo
       ep.n = 1;
       ep.r = E;
       ep.ldb = gp.E8;
-      if (const int rc = run_expand<kExpandProduct>(ep, 1024, stream)) return rc;
+      if (const int rc = run_expand<kExpandProduct>(ep, stream)) return rc;
     } else {
       constexpr int MT = 2;
       const dim3 grid((T + 16 * MT - 1) / (16 * MT), (d + 511) / 512);
