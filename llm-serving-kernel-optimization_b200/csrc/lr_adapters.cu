@@ -183,12 +183,12 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
                        blockIdx.z * per_round, per_round);
 }
 
-// Larger batches: windows of 64 rows.  A window with one adapter (a prompt's rows)
-// streams tiles of 128 k, its rows of x and the adapter's rows of A, through a ring
-// of cp.async stages; warp w multiplies 32 of the 128 k (w & 3) for half of the
-// rows (w >> 2).  (Bulk copies of these 256-byte rows measured 127 us at 16384 x
-// 4096, rank 32: the copy engine takes about 25 ns per row.)  A mixed window
-// takes its halves through shrink_groups.
+// Larger batches: windows of 64 rows.  A group (a prompt's rows) streams tiles of
+// 128 k, its rows of x and its adapter's rows of A, through a ring of cp.async
+// stages; warp w multiplies 32 of the 128 k (w & 3) for half of the rows (w >> 2).
+// A window of up to three groups (requests that meet in it) takes them one after
+// the other, one of more takes its halves through shrink_groups.  (Bulk copies of these 256-byte rows measured 127 us at 16384 x
+// 4096, rank 32: the copy engine takes about 25 ns per row.)
 constexpr int kTileK = 128;
 constexpr int kTileKPitch = kTileK * 2 + 64;  // bytes; neighbouring rows in different banks
 
@@ -213,14 +213,13 @@ __global__ void __launch_bounds__(kAdThreads, RB == 4 ? 1 : 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const int cs = int(cluster_nctarank()), cr = int(cluster_ctarank());
   const long row0 = long(blockIdx.x / cs) * 64;
-  const int nrows = int(min(64l, p.R - row0));
   const int bank = blockIdx.y / rank_groups, rank0 = (blockIdx.y % rank_groups) * RK;
   float* s_part = reinterpret_cast<float*>(s_dyn);
   pdl_wait();
   pdl_trigger();
   if (warp == 0) group_rows<64>(s, p.index, row0, p.R, p.n, false, bank == 0 ? p.err : nullptr);
   __syncthreads();
-  if (!s.uniform) {
+  if (s.n > 3) {
     for (int half = 0; half < 2; ++half) {
       __syncthreads();
       if (warp == 0)
@@ -232,92 +231,96 @@ __global__ void __launch_bounds__(kAdThreads, RB == 4 ? 1 : 2)
   }
   const int all = (p.K + kTileK - 1) / kTileK;
   const int tile0 = int(long(all) * cr / cs), tiles = int(long(all) * (cr + 1) / cs) - tile0;
-  const __half* ap = (bank ? p.a[1] : p.a[0]) + (size_t(s.adapter[0]) * p.r + rank0) * p.K;
   const int ranks = min(RK, p.r - rank0);
-  const auto fetch = [&](int i) {  // tile i into its stage: 16 lanes per row, zeros past the ends
-    if (i < tiles) {
-      const int k = (tile0 + i) * kTileK + (threadIdx.x & 15) * 8;
-      unsigned char* to = s_dyn + (i % S) * kStageBytes + (threadIdx.x & 15) * 16;
-#pragma unroll
-      for (int u = 0; u < 64 + RK; u += 16) {
-        const int row = u + (threadIdx.x >> 4);
-        const bool ok = k < p.K && (u < 64 ? row < nrows : row - 64 < ranks);
-        const __half* from = u < 64 ? p.x + size_t(row0 + row) * p.K : ap + size_t(row - 64) * p.K;
-        cp_async_16_zfill(to + row * kTileKPitch, ok ? from + k : p.x, ok);
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < S - 1; ++i) fetch(i);
   const int kq = warp & 3, half = warp >> 2;
-  float acc[RB][4][4];
+  for (int grp = 0; grp < s.n; ++grp) {
+    const __half* ap = (bank ? p.a[1] : p.a[0]) + (size_t(s.adapter[s.first[grp]]) * p.r + rank0) * p.K;
+    const auto fetch = [&](int i) {  // tile i into its stage: 16 lanes per row, zeros past the ends
+      if (i < tiles) {
+        const int k = (tile0 + i) * kTileK + (threadIdx.x & 15) * 8;
+        unsigned char* to = s_dyn + (i % S) * kStageBytes + (threadIdx.x & 15) * 16;
 #pragma unroll
-  for (int i = 0; i < RB; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
-  for (int i = 0; i < tiles; ++i) {
-    cp_async_wait_group<S - 2>();
-    __syncthreads();
-    fetch(i + S - 1);  // into the stage read one tile ago
-    const int st = i % S;
-    const unsigned char* from = s_dyn + st * kStageBytes + kq * 64 + tq * 16;
-    uint4 av[2 * RB], xv[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      xv[j] = *reinterpret_cast<const uint4*>(from + (half * 32 + j * 8 + g) * kTileKPitch);
-#pragma unroll
-    for (int j = 0; j < 2 * RB; ++j)
-      av[j] = *reinterpret_cast<const uint4*>(from + (64 + j * 8 + g) * kTileKPitch);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const uint4 lo = av[2 * r], hi = av[2 * r + 1], x = xv[j];
-        mma_f16(acc[r][j], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
-        mma_f16(acc[r][j], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+        for (int u = 0; u < 64 + RK; u += 16) {
+          const int row = u + (threadIdx.x >> 4);
+          const bool ok = k < p.K && (u < 64 ? s.group[row] == grp : row - 64 < ranks);
+          const __half* from = u < 64 ? p.x + size_t(row0 + row) * p.K : ap + size_t(row - 64) * p.K;
+          cp_async_16_zfill(to + row * kTileKPitch, ok ? from + k : p.x, ok);
+        }
       }
-  }
-  cp_async_wait_all();
-  __syncthreads();  // every tile is read: the ring becomes the warps' sums [warp][RK][PITCH]
-  float* mine = s_part + warp * RK * PITCH;
+      cp_async_commit();
+    };
 #pragma unroll
-  for (int i = 0; i < RB; ++i)
+    for (int i = 0; i < S - 1; ++i) fetch(i);
+    float acc[RB][4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int i = 0; i < RB; ++i)
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<float2*>(mine + (i * 16 + g + 8 * c) * PITCH + j * 8 + 2 * tq) =
-            make_float2(acc[i][j][2 * c], acc[i][j][2 * c + 1]);
-  __syncthreads();
-  // the four k-quarters, then the blocks of the cluster, in order
-  for (int o = threadIdx.x; o < 64 * RK; o += kAdThreads) {
-    const int t = o / RK, i = o % RK;
-    if (t >= nrows || i >= ranks) continue;
-    float* at = s_part + ((t >> 5) * 4 * RK + i) * PITCH + (t & 31);
-    const float sum = ((at[0] + at[RK * PITCH]) + at[2 * RK * PITCH]) + at[3 * RK * PITCH];
-    if (cs == 1)
-      p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
-    else
-      *at = sum;
-  }
-  if (cs > 1) {
-    cluster_sync();
-    for (int o = cr * kAdThreads + threadIdx.x; o < 64 * RK; o += cs * kAdThreads) {
-      const int t = o / RK, i = o % RK;
-      if (t >= nrows || i >= ranks) continue;
-      const uint32_t at = smem_u32(s_part + ((t >> 5) * 4 * RK + i) * PITCH + (t & 31));
-      float q[8];
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) q[c] = c < cs ? ld_cluster_f32(at, c) : 0.f;
-      float sum = 0.f;
+        for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+    for (int i = 0; i < tiles; ++i) {
+      cp_async_wait_group<S - 2>();
+      __syncthreads();
+      fetch(i + S - 1);  // into the stage read one tile ago
+      const int st = i % S;
+      const unsigned char* from = s_dyn + st * kStageBytes + kq * 64 + tq * 16;
+      uint4 av[2 * RB], xv[4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) sum += q[c];
-      p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
+      for (int j = 0; j < 4; ++j)
+        xv[j] = *reinterpret_cast<const uint4*>(from + (half * 32 + j * 8 + g) * kTileKPitch);
+#pragma unroll
+      for (int j = 0; j < 2 * RB; ++j)
+        av[j] = *reinterpret_cast<const uint4*>(from + (64 + j * 8 + g) * kTileKPitch);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          const uint4 lo = av[2 * r], hi = av[2 * r + 1], x = xv[j];
+          mma_f16(acc[r][j], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+          mma_f16(acc[r][j], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+        }
     }
-    cluster_sync();  // the sums stay until every block of the cluster has read them
+    cp_async_wait_all();
+    __syncthreads();  // every tile is read: the ring becomes the warps' sums [warp][RK][PITCH]
+    float* mine = s_part + warp * RK * PITCH;
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<float2*>(mine + (i * 16 + g + 8 * c) * PITCH + j * 8 + 2 * tq) =
+              make_float2(acc[i][j][2 * c], acc[i][j][2 * c + 1]);
+    __syncthreads();
+    // the four k-quarters, then the blocks of the cluster, in order
+    for (int o = threadIdx.x; o < 64 * RK; o += kAdThreads) {
+      const int t = o / RK, i = o % RK;
+      if (s.group[t] != grp || i >= ranks) continue;
+      float* at = s_part + ((t >> 5) * 4 * RK + i) * PITCH + (t & 31);
+      const float sum = ((at[0] + at[RK * PITCH]) + at[2 * RK * PITCH]) + at[3 * RK * PITCH];
+      if (cs == 1)
+        p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
+      else
+        *at = sum;
+    }
+    if (cs > 1) {
+      cluster_sync();
+      for (int o = cr * kAdThreads + threadIdx.x; o < 64 * RK; o += cs * kAdThreads) {
+        const int t = o / RK, i = o % RK;
+        if (s.group[t] != grp || i >= ranks) continue;
+        const uint32_t at = smem_u32(s_part + ((t >> 5) * 4 * RK + i) * PITCH + (t & 31));
+        float q[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) q[c] = c < cs ? ld_cluster_f32(at, c) : 0.f;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) sum += q[c];
+        p.v[(size_t(bank) * p.R + row0 + t) * p.r + rank0 + i] = sum;
+      }
+      cluster_sync();  // the sums stay until every block of the cluster has read them
+    } else {
+      __syncthreads();
+    }
   }
 }
 

@@ -288,19 +288,27 @@ constexpr int expand_ahead() {
                              : RV == 64 && MODE != kExpandSwiglu ? 2 : 1;
 }
 
-// Larger windows stream the base rows: stages of the window's rows x 256 columns
-// by cp.async of a producer warp, a row per instruction, a consumer warp per 32
-// columns.
-constexpr int kTileCols = 256;
-constexpr int kTileGroups = kTileCols / 32;
-constexpr int kTilePitch = kTileCols * 2 + 64;  // bytes; neighbouring rows in different banks
-constexpr int kTileStages = 2;
+// Larger windows stream the base rows: stages of the window's rows x 224 columns
+// by cp.async of a producer warp, a row per instruction, to seven consumer warps of
+// 32 columns.  (A ninth warp for the producer would cost the others a quarter of
+// their registers at two blocks on an SM: 18 warps do not spread over its four
+// parts.)  Without base rows all eight warps consume.
+template <int MODE>
+constexpr int consumers() {
+  return MODE == kExpandProduct ? kAdWarps : kAdWarps - 1;
+}
+constexpr int kTilePitch = (kAdWarps - 1) * 64;  // bytes, 64 mod 128: neighbouring rows in
+                                                 // different banks
+template <int MODE>
+constexpr int tile_stages() {
+  return MODE == kExpandSwiglu ? 2 : 3;
+}
 
 template <int RV, int MT, int MODE>
 constexpr int expand_base_bytes() {
   return MODE == kExpandProduct ? 0
          : MT == 1 ? kAdWarps * expand_ahead<RV, MODE>() * (MODE == kExpandSwiglu ? 2 : 1) * 2 * 512
-                   : kTileStages * (MODE == kExpandSwiglu ? 2 : 1) * MT * 16 * kTilePitch;
+                   : tile_stages<MODE>() * (MODE == kExpandSwiglu ? 2 : 1) * MT * 16 * kTilePitch;
 }
 
 template <int RV, int MT, int MODE>
@@ -308,16 +316,10 @@ constexpr int expand_smem_bytes() {
   return expand_base_bytes<RV, MT, MODE>() + (MODE == kExpandSwiglu ? 2 : 1) * 2 * MT * 16 * RV * 2;
 }
 
-template <int MT, int MODE>
-constexpr int expand_threads() {
-  return kAdThreads + (MT > 1 && MODE != kExpandProduct ? 32 : 0);
-}
-
-// Nine warps leave 96 registers a thread to two blocks on an SM: enough up to rank 32.
+// Two blocks on an SM (128 registers a thread) where the weights leave room for it.
 template <int RV, int MT, int MODE>
 constexpr int expand_min_blocks() {
-  if (MT == 1) return RV <= (MODE == kExpandSwiglu ? 32 : 64) ? 2 : 1;
-  return MODE == kExpandSwiglu || RV > 64 ? 1 : RV > 32 && MODE == kExpandAdd ? 1 : 2;
+  return RV <= (MODE == kExpandSwiglu ? (MT == 1 ? 32 : 16) : 64) ? 2 : 1;
 }
 
 // Eight results of a row: base (and base2) with the scaled sums of both banks.
@@ -343,11 +345,13 @@ LR_DEVICE uint4 expand_epilogue(const float (&acc)[BANKS][4][4], int h, const fl
 }
 
 template <int RV, int MT, int MODE>
-__global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<RV, MT, MODE>())
+__global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     expand_kernel(ExpandArgs p) {
   constexpr int W = 16 * MT;
   constexpr int BANKS = MODE == kExpandSwiglu ? 2 : 1;
   constexpr int kTerm = W * RV / 8;  // uint4 of one term of v
+  constexpr int kTileGroups = consumers<MODE>(), kTileStages = tile_stages<MODE>();
+  constexpr int kProducer = kTileGroups;  // the producer warp
   extern __shared__ __align__(128) unsigned char s_dyn[];  // base rows, then v
   uint4* s_v = reinterpret_cast<uint4*>(s_dyn + expand_base_bytes<RV, MT, MODE>());
   // s_v: [bank][hi, lo][row tile][step][lane]
@@ -367,13 +371,13 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
   if (MT > 1 && MODE != kExpandProduct && threadIdx.x == 32) {
     for (int i = 0; i < kTileStages; ++i) {
       mbar_init(s_full + i, 32);  // the producer's lanes
-      mbar_init(s_empty + i, kAdWarps);
+      mbar_init(s_empty + i, kTileGroups);
     }
     s_abort = 0;
     fence_mbarrier_init();
   }
   __syncthreads();
-  const bool stream = MT > 1 && MODE != kExpandProduct && s.uniform;
+  const bool stream = MT > 1 && MODE != kExpandProduct && s.n > 0;
 
   // Producer: tiles [first, last) of the base rows, each as soon as its stage has
   // been read.  The first stages start ahead of everything else.
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
           !mbar_wait_bounded(s_empty + st, (round - 1) & 1, &s_abort, p.err, kCopyWaitNs))
         return;
       __syncwarp();
-      if (cg * 32 + lane * 8 < p.N) {
+      if (lane < kTileGroups * 4 && cg * 32 + lane * 8 < p.N) {
 #pragma unroll
         for (int bk = 0; bk < BANKS; ++bk) {
           const __half* from = p.base[bk] + size_t(row0) * p.N + cg * 32 + lane * 8;
@@ -398,8 +402,8 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
       cp_async_arrive(s_full + st);
     }
   };
-  if (stream && warp == kAdWarps) produce(0, min(n_tiles, kTileStages));
-  if (threadIdx.x < kAdThreads) {  // v: fp32 -> scaled (value, remainder) pairs in fragment order
+  if (stream && warp == kProducer) produce(0, min(n_tiles, kTileStages));
+  {  // v: fp32 -> scaled (value, remainder) pairs in fragment order
     constexpr int LPR = kAdThreads / W;               // lanes of a row
     constexpr int EL = (RV / 2 + LPR - 1) / LPR;      // pairs of a lane
     const int t = threadIdx.x / LPR, q = threadIdx.x % LPR;
@@ -450,46 +454,41 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
   __syncthreads();
 
   const unsigned n8 = 8u * unsigned(p.N);
-  if (MT > 1 && (stream || MODE == kExpandProduct)) {
-    // One entry of b for the whole window (a prompt's rows): a warp takes every
-    // eighth column group for all rows.
-    if (warp == kAdWarps) {
-      produce(min(n_tiles, kTileStages), n_tiles);
+  if (MT > 1) {
+    // Every consumer takes its 32 of a tile's columns for all rows: a window's groups
+    // one after the other (one for a prompt), each on its own row tiles.
+    if (MODE != kExpandProduct && warp == kProducer) {
+      if (stream) produce(min(n_tiles, kTileStages), n_tiles);
       cp_async_wait_all();  // leave no copy behind
       return;
     }
-    const int ad = MODE == kExpandProduct ? 0 : s.adapter[0];
-    const __half* wp[BANKS];
-#pragma unroll
-    for (int bk = 0; bk < BANKS; ++bk)
-      wp[bk] = p.b[bk] +
-               (size_t(ad) * p.N + (cg0 + warp) * 32 + (g >> 1) * 8 + (g & 1)) * p.ldb +
-               tq * RankTile<RV>::kPer;
-    const size_t wstep = size_t(kTileCols) * p.ldb;
+    const int n_groups = MODE == kExpandProduct ? 1 : s.n;
     float fac[2 * MT][BANKS];
 #pragma unroll
-    for (int bk = 0; bk < BANKS; ++bk)
+    for (int i = 0; i < 2 * MT; ++i)
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) fac[i][bk] = s_fac[bk][g + 8 * i];
+      for (int bk = 0; bk < BANKS; ++bk) fac[i][bk] = s_fac[bk][g + 8 * i];
     __half* out = p.out + size_t(row0 + g) * p.N + (cg0 + warp) * 32 + tq * 8;
     const unsigned char* bp = s_dyn + g * kTilePitch + warp * 64 + tq * 16;
     const uint4* vp = s_v + lane;
     unsigned st = 0, parity = 0;
 
-    const auto weights = [&](RankTile<RV>(&wt)[BANKS], int c) {
-#pragma unroll
-      for (int bk = 0; bk < BANKS; ++bk) {
-        wt[bk].load(wp[bk], p.ldb, c < cg1 && c * 32 + (g >> 1) * 8 < p.N, tq);
-        wp[bk] += wstep;
-      }
+    const auto arrived = [&]() {
+      return MODE == kExpandProduct ||
+             mbar_wait_bounded(s_full + st, parity, &s_abort, p.err, kCopyWaitNs);
     };
-    const auto tile = [&](const RankTile<RV>(&wt)[BANKS], int c) {
-      if (MODE != kExpandProduct &&
-          !mbar_wait_bounded(s_full + st, parity, &s_abort, p.err, kCopyWaitNs))
-        return false;
+    // One group's rows of the tile of column group c.  `whole`: the window is one
+    // group and `grp` is not looked at; `last`: the tile is not read again.
+    const auto multiply = [&](const RankTile<RV>(&wt)[BANKS], int c, const bool whole, int grp,
+                              bool last) {
       const bool cok = c < cg1 && c * 32 + tq * 8 < p.N;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
+        bool mine[2] = {g + 16 * m < nrows, g + 16 * m + 8 < nrows};
+        if (!whole) {
+          mine[0] = s.group[g + 16 * m] == grp;
+          mine[1] = s.group[g + 16 * m + 8] == grp;
+        }
         uint4 bs[2][BANKS];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -498,10 +497,11 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
             if (MODE != kExpandProduct)
               bs[h][bk] = *reinterpret_cast<const uint4*>(
                   bp + ((st * BANKS + bk) * W + 16 * m + 8 * h) * kTilePitch);
-        if (m == MT - 1 && MODE != kExpandProduct) {
+        if (m == MT - 1 && MODE != kExpandProduct && last) {
           __syncwarp();
           if (lane == 0) mbar_arrive(s_empty + st);
         }
+        if (!whole && !__any_sync(0xffffffffu, mine[0] || mine[1])) continue;
         float acc[BANKS][4][4];
 #pragma unroll
         for (int bk = 0; bk < BANKS; ++bk) {
@@ -511,41 +511,82 @@ __global__ void __launch_bounds__(expand_threads<MT, MODE>(), expand_min_blocks<
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint4 o = expand_epilogue<MODE, BANKS>(acc, h, fac[2 * m + h], bs[h]);
-          if (cok && g + 16 * m + 8 * h < nrows)
+          if (cok && mine[h])
             *reinterpret_cast<uint4*>(out + size_t(unsigned(2 * m + h) * n8)) = o;
         }
       }
-      out += kTileCols;
+    };
+    const auto advance = [&]() {
+      out += kTileGroups * 32;
       if (++st == kTileStages) {
         st = 0;
         parity ^= 1;
       }
-      return true;
     };
-    // the next column group's weights load while one is multiplied
-    RankTile<RV> w0[BANKS], w1[BANKS];
-    int c = cg0 + warp;
     const int end = cg0 + warp + n_tiles * kTileGroups;
-    if (RV <= (MODE == kExpandProduct ? 32 : 64) && MODE != kExpandSwiglu) {
-      weights(w0, c);
-      while (true) {
-        weights(w1, c + kTileGroups);
-        if (!tile(w0, c) || (c += kTileGroups) >= end) break;
-        weights(w0, c + kTileGroups);
-        if (!tile(w1, c) || (c += kTileGroups) >= end) break;
-      }
-    } else {
-      for (; c < end; c += kTileGroups) {
+    int c = cg0 + warp;
+    if (MODE == kExpandProduct || s.uniform) {
+      const int ad = MODE == kExpandProduct ? 0 : s.adapter[0];
+      const __half* wp[BANKS];
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk)
+        wp[bk] = p.b[bk] + (size_t(ad) * p.N + c * 32 + (g >> 1) * 8 + (g & 1)) * p.ldb +
+                 tq * RankTile<RV>::kPer;
+      const size_t wstep = size_t(kTileGroups) * 32 * p.ldb;
+      const auto weights = [&](RankTile<RV>(&wt)[BANKS], int cw) {
+#pragma unroll
+        for (int bk = 0; bk < BANKS; ++bk) {
+          wt[bk].load(wp[bk], p.ldb, cw < cg1 && cw * 32 + (g >> 1) * 8 < p.N, tq);
+          wp[bk] += wstep;
+        }
+      };
+      // the next column group's weights load while one is multiplied
+      RankTile<RV> w0[BANKS], w1[BANKS];
+      if (RV <= (MODE == kExpandProduct ? 32 : 64) && MODE != kExpandSwiglu) {
         weights(w0, c);
-        if (!tile(w0, c)) break;
+        while (true) {
+          weights(w1, c + kTileGroups);
+          if (!arrived()) break;
+          multiply(w0, c, true, 0, true);
+          advance();
+          if ((c += kTileGroups) >= end) break;
+          weights(w0, c + kTileGroups);
+          if (!arrived()) break;
+          multiply(w1, c, true, 0, true);
+          advance();
+          if ((c += kTileGroups) >= end) break;
+        }
+      } else {
+        for (; c < end; c += kTileGroups) {
+          weights(w0, c);
+          if (!arrived()) break;
+          multiply(w0, c, true, 0, true);
+          advance();
+        }
       }
+      return;
+    }
+    if (n_groups == 0) return;
+    for (; c < end; c += kTileGroups) {
+      if (!arrived()) break;
+      for (int grp = 0; grp < n_groups; ++grp) {
+        const int ad = s.adapter[s.first[grp]];
+        const int nr = c * 32 + (g >> 1) * 8;
+        RankTile<RV> wt[BANKS];  // zeros for the rows without an adapter
+#pragma unroll
+        for (int bk = 0; bk < BANKS; ++bk)
+          wt[bk].load(p.b[bk] + (size_t(max(ad, 0)) * p.N + nr + (g & 1)) * p.ldb +
+                          tq * RankTile<RV>::kPer,
+                      p.ldb, ad >= 0 && c < cg1 && nr < p.N, tq);
+        multiply(wt, c, false, grp, grp == n_groups - 1);
+      }
+      advance();
     }
     return;
   }
 
-  // Mixed windows and small batches: the warps are dealt out to the groups.
-  if (warp >= kAdWarps) return;
-  constexpr int S = MT == 1 ? expand_ahead<RV, MODE>() : 1;
+  // Small batches: the warps are dealt out to the groups.
+  constexpr int S = expand_ahead<RV, MODE>();
   const int n_groups = MODE == kExpandProduct ? 1 : s.n;
   for (int base = 0; base < n_groups; base += kAdWarps) {
     const int ng = min(kAdWarps, n_groups - base);
@@ -657,19 +698,19 @@ static int launch_expand(ExpandArgs p, cudaStream_t stream) {
   if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
   const long windows = (p.R + W - 1) / W;
   const int cgs = (p.N + 31) / 32;
-  int gpc = kTileGroups;
+  int gpc = consumers<MODE>();
   if (MT == 1) {
     // one wave of two blocks per SM where that leaves a block 8 to 64 groups
     const long per = (windows * cgs + 2 * kTargetBlocks - 1) / (2 * kTargetBlocks);
     gpc = int(per < 8 ? 8 : per > 64 ? 64 : per);
   } else {
-    // 256 columns per block, more while the grid stays above eight blocks per SM
-    while (gpc < 64 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
+    // one tile's columns per block, more while the grid stays above eight blocks per SM
+    while (gpc < 50 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
   }
   p.groups_per_chunk = gpc;
   if (windows > 0x7fffffffL || (cgs + gpc - 1) / gpc > 65535) return LR_ERR_INVALID_ARGUMENT;
   return launch_pdl(kern, dim3(unsigned(windows), (cgs + gpc - 1) / gpc),
-                    dim3(expand_threads<MT, MODE>()), smem, stream, p);
+                    dim3(kAdThreads), smem, stream, p);
 }
 
 // Row windows of 64 (32 for SwiGLU), or of 16 while the larger ones would leave
@@ -677,7 +718,7 @@ static int launch_expand(ExpandArgs p, cudaStream_t stream) {
 template <int MODE>
 static int run_expand(const ExpandArgs& p, cudaStream_t stream) {
   constexpr int MT = MODE == kExpandSwiglu ? 2 : 4;
-  const long blocks = (p.R + 16 * MT - 1) / (16 * MT) * ((p.N + kTileCols - 1) / kTileCols);
+  const long blocks = (p.R + 16 * MT - 1) / (16 * MT) * ((p.N + 255) / 256);
   const bool small = blocks < 2 * kTargetBlocks;
   if (p.r <= 16)
     return small ? launch_expand<16, 1, MODE>(p, stream) : launch_expand<16, MT, MODE>(p, stream);
