@@ -186,8 +186,9 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
 // Larger batches: windows of 64 rows.  A group (a prompt's rows) streams tiles of
 // 128 k, its rows of x and its adapter's rows of A, through a ring of cp.async
 // stages; warp w multiplies 32 of the 128 k (w & 3) for half of the rows (w >> 2).
-// A window of up to three groups (requests that meet in it) takes them one after
-// the other, one of more takes its halves through shrink_groups.  (Bulk copies of these 256-byte rows measured 127 us at 16384 x
+// The groups of a window that up to three requests share go to the two blocks of
+// the grid's z (one of them leaves at once otherwise: its slot is free while the
+// others stream); a window of more groups takes its halves through shrink_groups.  (Bulk copies of these 256-byte rows measured 127 us at 16384 x
 // 4096, rank 32: the copy engine takes about 25 ns per row.)
 constexpr int kTileK = 128;
 constexpr int kTileKPitch = kTileK * 2 + 64;  // bytes; neighbouring rows in different banks
@@ -220,6 +221,7 @@ __global__ void __launch_bounds__(kAdThreads, RB == 4 ? 1 : 2)
   if (warp == 0) group_rows<64>(s, p.index, row0, p.R, p.n, false, bank == 0 ? p.err : nullptr);
   __syncthreads();
   if (s.n > 3) {
+    if (blockIdx.z > 0) return;
     for (int half = 0; half < 2; ++half) {
       __syncthreads();
       if (warp == 0)
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(kAdThreads, RB == 4 ? 1 : 2)
   const int tile0 = int(long(all) * cr / cs), tiles = int(long(all) * (cr + 1) / cs) - tile0;
   const int ranks = min(RK, p.r - rank0);
   const int kq = warp & 3, half = warp >> 2;
-  for (int grp = 0; grp < s.n; ++grp) {
+  for (int grp = blockIdx.z; grp < s.n; grp += gridDim.z) {
     const __half* ap = (bank ? p.a[1] : p.a[0]) + (size_t(s.adapter[s.first[grp]]) * p.r + rank0) * p.K;
     const auto fetch = [&](int i) {  // tile i into its stage: 16 lanes per row, zeros past the ends
       if (i < tiles) {
@@ -404,6 +406,7 @@ static int launch_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
   const long blocks = windows * rank_groups * banks;
   unsigned cs = 1, gs = 1;
   while (cs < 8 && blocks * cs * 2 <= fill) cs *= 2;
+  if (!small) gs = 2;
   while (small && gs < 4 && gs < p.R && blocks * cs * gs * 2 <= fill) gs *= 2;
   if (windows * cs > 0x7fffffffL) return LR_ERR_INVALID_ARGUMENT;
   const dim3 grid(unsigned(windows * cs), rank_groups * banks, gs);
