@@ -193,21 +193,19 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
 constexpr int kTileK = 128;
 constexpr int kTileKPitch = kTileK * 2 + 64;  // bytes; neighbouring rows in different banks
 
-template <int RB>
-constexpr int shrink_stages() {
-  return 3;
-}
+constexpr int kShrinkStages = 3;
+
 template <int RB>
 constexpr int shrink_smem_bytes() {
-  constexpr int ring = shrink_stages<RB>() * (64 + 16 * RB) * kTileKPitch;
+  constexpr int ring = kShrinkStages * (64 + 16 * RB) * kTileKPitch;
   constexpr int part = kAdWarps * 16 * RB * 34 * int(sizeof(float));
   return ring > part ? ring : part;
 }
 
 template <int RB>
-__global__ void __launch_bounds__(kAdThreads, RB == 4 ? 1 : 2)
+__global__ void __launch_bounds__(kAdThreads, 2)
     adapter_shrink_stream_kernel(ShrinkArgs p, int rank_groups) {
-  constexpr int RK = 16 * RB, S = shrink_stages<RB>(), PITCH = 34;
+  constexpr int RK = 16 * RB, S = kShrinkStages, PITCH = 34;
   constexpr int kStageBytes = (64 + RK) * kTileKPitch;
   extern __shared__ __align__(128) unsigned char s_dyn[];  // ring, then the warps' sums
   __shared__ Groups s;
@@ -393,35 +391,50 @@ static int launch_cluster(void (*kern)(KArgs...), dim3 grid, unsigned cluster, s
 
 constexpr long kSmallRows = 256;  // up to here windows of 8 (shrink) and 16 rows (expand)
 
+// Blocks are made to fill one wave of two per SM: K is split over a cluster, and a
+// small batch's window over blocks of its groups.
 template <int RB>
-static int launch_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
-  const bool small = p.R <= kSmallRows;
-  const int W = small ? 8 : 64, RK = 16 * RB;
-  const int smem = small ? kAdWarps * RK * 10 * int(sizeof(float)) : shrink_smem_bytes<RB>();
-  const long windows = (p.R + W - 1) / W;
+static int launch_shrink_small(const ShrinkArgs& p, int banks, cudaStream_t stream) {
+  constexpr int RK = 16 * RB;
+  const long windows = (p.R + 7) / 8;
   const int rank_groups = (p.r + RK - 1) / RK;
-  // fill one wave of blocks by splitting K over a cluster, then (small batches) a
-  // window's groups over blocks
-  const long fill = kTargetBlocks * (!small && RB == 4 ? 1 : 2);
   const long blocks = windows * rank_groups * banks;
   unsigned cs = 1, gs = 1;
-  while (cs < 8 && blocks * cs * 2 <= fill) cs *= 2;
-  if (!small) gs = 2;
-  while (small && gs < 4 && gs < p.R && blocks * cs * gs * 2 <= fill) gs *= 2;
-  if (windows * cs > 0x7fffffffL) return LR_ERR_INVALID_ARGUMENT;
-  const dim3 grid(unsigned(windows * cs), rank_groups * banks, gs);
-  if (small)
-    return launch_cluster(adapter_shrink_kernel<RB>, grid, cs, smem, stream, p, rank_groups);
-  static unsigned long long configured = 0;
-  if (const int rc = set_dyn_smem_once(adapter_shrink_stream_kernel<RB>, smem, configured))
-    return rc;
-  return launch_cluster(adapter_shrink_stream_kernel<RB>, grid, cs, smem, stream, p, rank_groups);
+  while (cs < 8 && blocks * cs * 2 <= 2 * kTargetBlocks) cs *= 2;
+  while (gs < 4 && gs < p.R && blocks * cs * gs * 2 <= 2 * kTargetBlocks) gs *= 2;
+  return launch_cluster(adapter_shrink_kernel<RB>,
+                        dim3(unsigned(windows * cs), rank_groups * banks, gs), cs,
+                        kAdWarps * RK * 10 * sizeof(float), stream, p, rank_groups);
 }
 
+// Clusters of 8 wait long for eight free SMs next to one another: only where the
+// grid stays under half a block per SM (1111 rows, K 2048, rank 64: 35 us against
+// 21 with clusters of 4; 400 rows, K 4096, rank 16: 13 against 15).
+template <int RB>
+static int launch_shrink_stream(const ShrinkArgs& p, int banks, cudaStream_t stream) {
+  constexpr int RK = 16 * RB, smem = shrink_smem_bytes<RB>();
+  auto kern = adapter_shrink_stream_kernel<RB>;
+  static unsigned long long configured = 0;
+  if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
+  const long windows = (p.R + 63) / 64;
+  const int rank_groups = (p.r + RK - 1) / RK;
+  const long blocks = windows * rank_groups * banks;
+  unsigned cs = 1;
+  while (cs < 8 && blocks * cs * 2 <= (cs < 4 ? 2 * kTargetBlocks : kTargetBlocks / 2)) cs *= 2;
+  if (windows * cs > 0x7fffffffL) return LR_ERR_INVALID_ARGUMENT;
+  return launch_cluster(kern, dim3(unsigned(windows * cs), rank_groups * banks, 2), cs, smem,
+                        stream, p, rank_groups);
+}
+
+// Ranks above 32 (64 in small batches) are taken in parts, each reading x again:
+// one kernel for rank 64 measured the same time in four times the registers.
 static int run_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
-  return p.r <= 16   ? launch_shrink<1>(p, banks, stream)
-         : p.r <= 32 ? launch_shrink<2>(p, banks, stream)
-                     : launch_shrink<4>(p, banks, stream);
+  if (p.R > kSmallRows)
+    return p.r <= 16 ? launch_shrink_stream<1>(p, banks, stream)
+                     : launch_shrink_stream<2>(p, banks, stream);
+  return p.r <= 16   ? launch_shrink_small<1>(p, banks, stream)
+         : p.r <= 32 ? launch_shrink_small<2>(p, banks, stream)
+                     : launch_shrink_small<4>(p, banks, stream);
 }
 
 static int check_adapter_args(const void* x, long R, int K, const int32_t* index, int n, int r,
