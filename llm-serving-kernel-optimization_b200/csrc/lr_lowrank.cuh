@@ -94,20 +94,6 @@ LR_DEVICE void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 LR_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// silu(gate) * up of eight fp16 values
-LR_DEVICE uint4 swiglu8(const uint4& gate, const uint4& up) {
-  const __half2* a = reinterpret_cast<const __half2*>(&gate);
-  const __half2* b = reinterpret_cast<const __half2*>(&up);
-  float o[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 x = __half22float2(a[i]), y = __half22float2(b[i]);
-    o[2 * i] = silu_f32(x.x) * y.x;
-    o[2 * i + 1] = silu_f32(x.y) * y.y;
-  }
-  return pack_half8(o);
-}
-
 // ---------------------------------------------------------------------------
 // a window's groups
 // ---------------------------------------------------------------------------
@@ -280,7 +266,7 @@ LR_DEVICE int fragment_word(int t, int c) {
   return ((m * (RV / 16) + step) * 32 + g * 4 + tq) * 4 + kh * 2 + h;
 }
 
-// One row tile: column groups of a warp whose loads are in flight together.
+// Small batches: groups of a window whose weights are in flight together.
 template <int RV, int MODE>
 constexpr int expand_ahead() {
   return RV == 16 ? (MODE == kExpandSwiglu ? 4 : 8)
@@ -306,9 +292,9 @@ constexpr int tile_stages() {
 
 template <int RV, int MT, int MODE>
 constexpr int expand_base_bytes() {
-  return MODE == kExpandProduct ? 0
-         : MT == 1 ? kAdWarps * expand_ahead<RV, MODE>() * (MODE == kExpandSwiglu ? 2 : 1) * 2 * 512
-                   : tile_stages<MODE>() * (MODE == kExpandSwiglu ? 2 : 1) * MT * 16 * kTilePitch;
+  return MODE == kExpandProduct || MT == 1
+             ? 0
+             : tile_stages<MODE>() * (MODE == kExpandSwiglu ? 2 : 1) * MT * 16 * kTilePitch;
 }
 
 template <int RV, int MT, int MODE>
@@ -585,101 +571,76 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     return;
   }
 
-  // Small batches: the warps are dealt out to the groups.
+  // Small batches: a warp takes its column groups for all 16 rows.  The window's
+  // groups come S at a time, all their weights in flight; each is multiplied with
+  // every row and kept for its own, so the base rows are finished once, by all lanes.
   constexpr int S = expand_ahead<RV, MODE>();
   const int n_groups = MODE == kExpandProduct ? 1 : s.n;
-  for (int base = 0; base < n_groups; base += kAdWarps) {
-    const int ng = min(kAdWarps, n_groups - base);
-    const int wpg = warps_per_group(ng);
-    const int grp = warp / wpg, sub = warp % wpg;
-    if (grp >= ng) continue;
-    const int slot = base + grp;
-    const int ad = MODE == kExpandProduct ? 0 : s.adapter[s.first[slot]];
-    unsigned rows_ok = 0, tiles = 0;  // this lane's member rows, the warp's used row tiles
+  int gid[2];
+  bool none[2];
+  float fac[2][BANKS];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+  for (int h = 0; h < 2; ++h) {
+    const int t = g + 8 * h;
+    gid[h] = MODE == kExpandProduct ? (t < nrows ? 0 : -1) : s.group[t];
+    none[h] = MODE != kExpandProduct && s.adapter[t] < 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int t = m * 16 + g + 8 * h;
-        if (MODE == kExpandProduct ? t < nrows : s.group[t] == slot) rows_ok |= 1u << (2 * m + h);
-      }
-      if (__any_sync(0xffffffffu, (rows_ok >> (2 * m)) & 3u)) tiles |= 1u << m;
-    }
-    // This lane's element offsets from the window's first row: row g + 8 i, column nc.
-    const unsigned row_n = unsigned(g) * unsigned(p.N) + tq * 8;
-    const size_t window = size_t(row0) * p.N;
-    const __half* base0 = MODE == kExpandProduct ? nullptr : p.base[0] + window;
-    const __half* base1 = MODE == kExpandProduct ? nullptr : p.base[BANKS - 1] + window;
-    __half* out = p.out + window;
-    if (ad < 0) {  // no adapter: the base rows as they are
-      for (int c = cg0 + sub; c < cg1; c += wpg) {
+    for (int bk = 0; bk < BANKS; ++bk) fac[h][bk] = s_fac[bk][t];
+  }
+  const size_t row_off = size_t(row0 + g) * p.N + tq * 8;
+  for (int c = cg0 + warp; c < cg1; c += kAdWarps) {
+    const bool cok = c * 32 + tq * 8 < p.N;
+    const size_t off = row_off + c * 32;
+    uint4 bs[2][BANKS];
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-          if (!((rows_ok >> i) & 1u) || c * 32 + tq * 8 >= p.N) continue;
-          const unsigned o = row_n + c * 32 + i * n8;
-          uint4 v = ld_row(reinterpret_cast<const uint4*>(base0 + o));
-          if (MODE == kExpandSwiglu)
-            v = swiglu8(v, ld_row(reinterpret_cast<const uint4*>(base1 + o)));
-          *reinterpret_cast<uint4*>(out + o) = v;
-        }
-      }
-      continue;
-    }
-    // The base rows go through this lane's own slots of shared memory.
-    uint4* slots = reinterpret_cast<uint4*>(s_dyn) + warp * (S * BANKS * MT * 2 * 32) + lane;
-    for (int c0 = cg0 + sub; c0 < cg1; c0 += wpg * S) {  // all loads of S groups in flight
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk)
+        if (MODE != kExpandProduct && cok && gid[h] >= 0)
+          bs[h][bk] = ld_row(reinterpret_cast<const uint4*>(p.base[bk] + off + h * n8));
+    float acc[BANKS][4][4];
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[bk][j][i] = 0.f;
+    const int nr = c * 32 + (g >> 1) * 8;
+    for (int g0 = 0; g0 < n_groups; g0 += S) {
       RankTile<RV> wt[S][BANKS];
 #pragma unroll
       for (int u = 0; u < S; ++u) {
-        const int c = c0 + u * wpg;
-        const bool cin = c < cg1;
-        const int nr = c * 32 + (g >> 1) * 8;
-        const unsigned o = row_n + c * 32;
+        const int ad = MODE == kExpandProduct ? 0
+                       : g0 + u < n_groups    ? s.adapter[s.first[g0 + u]]
+                                              : -1;
 #pragma unroll
-        for (int bk = 0; bk < BANKS; ++bk) {
-          if (MODE != kExpandProduct && cin && c * 32 + tq * 8 < p.N) {
-#pragma unroll
-            for (int i = 0; i < 2 * MT; ++i)
-              if ((rows_ok >> i) & 1u)
-                cp_async_16(slots + ((u * BANKS + bk) * MT * 2 + i) * 32,
-                            (bk ? base1 : base0) + (o + i * n8));
-          }
-          wt[u][bk].load(p.b[bk] + (size_t(ad) * p.N + nr + (g & 1)) * p.ldb +
+        for (int bk = 0; bk < BANKS; ++bk)
+          wt[u][bk].load(p.b[bk] + (size_t(max(ad, 0)) * p.N + nr + (g & 1)) * p.ldb +
                              tq * RankTile<RV>::kPer,
-                         p.ldb, cin && nr < p.N, tq);
-        }
+                         p.ldb, ad >= 0 && nr < p.N, tq);
       }
-      cp_async_wait_all();
 #pragma unroll
       for (int u = 0; u < S; ++u) {
-        const int c = c0 + u * wpg;
-        if (c >= cg1) break;
-        const bool cok = c * 32 + tq * 8 < p.N;
+        if (g0 + u >= n_groups) break;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if (!((tiles >> m) & 1u)) continue;
-          float acc[BANKS][4][4];
+        for (int bk = 0; bk < BANKS; ++bk) {
+          float mine[4][4];
+          const uint4* hi = s_v + lane + 2 * bk * kTerm;
+          wt[u][bk].multiply(mine, hi, hi + kTerm);
 #pragma unroll
-          for (int bk = 0; bk < BANKS; ++bk) {
-            const uint4* hi = s_v + lane + 2 * bk * kTerm + m * (RV / 16) * 32;
-            wt[u][bk].multiply(acc[bk], hi, hi + kTerm);
-          }
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int i = 2 * m + h;
-            if (!((rows_ok >> i) & 1u) || !cok) continue;
-            uint4 bs[BANKS];
-            float fac[BANKS];
-#pragma unroll
-            for (int bk = 0; bk < BANKS; ++bk) {
-              if (MODE != kExpandProduct) bs[bk] = slots[((u * BANKS + bk) * MT * 2 + i) * 32];
-              fac[bk] = s_fac[bk][g + 8 * i];
-            }
-            *reinterpret_cast<uint4*>(out + (row_n + c * 32 + i * n8)) =
-                expand_epilogue<MODE, BANKS>(acc, h, fac, bs);
-          }
+            for (int i = 0; i < 4; ++i)
+              acc[bk][j][i] = gid[i >> 1] == g0 + u ? mine[j][i] : acc[bk][j][i];
         }
       }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (!cok || gid[h] < 0) continue;
+      uint4 o = expand_epilogue<MODE, BANKS>(acc, h, fac[h], bs[h]);
+      if (MODE == kExpandAdd && none[h]) o = bs[h][0];
+      *reinterpret_cast<uint4*>(p.out + off + h * n8) = o;
     }
   }
 }
@@ -700,9 +661,9 @@ static int launch_expand(ExpandArgs p, cudaStream_t stream) {
   const int cgs = (p.N + 31) / 32;
   int gpc = consumers<MODE>();
   if (MT == 1) {
-    // one wave of two blocks per SM where that leaves a block 8 to 64 groups
-    const long per = (windows * cgs + 2 * kTargetBlocks - 1) / (2 * kTargetBlocks);
-    gpc = int(per < 8 ? 8 : per > 64 ? 64 : per);
+    // one wave of two blocks per SM where that leaves a warp one to eight groups
+    const long per = (windows * cgs + 2 * kTargetBlocks * 8 - 1) / (2 * kTargetBlocks * 8);
+    gpc = int(per < 1 ? 1 : per > 8 ? 8 : per) * 8;
   } else {
     // one tile's columns per block, more while the grid stays above eight blocks per SM
     while (gpc < 50 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
