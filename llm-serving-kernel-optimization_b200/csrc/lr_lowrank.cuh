@@ -269,9 +269,9 @@ LR_DEVICE int fragment_word(int t, int c) {
 // Small batches: groups of a window whose weights are in flight together.
 template <int RV, int MODE>
 constexpr int expand_ahead() {
-  return RV == 16 ? (MODE == kExpandSwiglu ? 4 : 8)
-                  : RV == 32 ? (MODE == kExpandSwiglu ? 2 : 4)
-                             : RV == 64 && MODE != kExpandSwiglu ? 2 : 1;
+  // as many as 64 registers hold; SwiGLU's two banks leave room for half of that
+  // (128 rows, rank 16, N 14336: 31 us a pass with 2 groups, 37 with 4)
+  return MODE == kExpandSwiglu ? (RV == 16 ? 2 : 1) : RV <= 64 ? 128 / RV : 1;
 }
 
 // Larger windows stream the base rows: stages of the window's rows x 224 columns
