@@ -6,7 +6,9 @@ calls keep working.  Additions (ignored by the reference loader):
 
 * ``MoEConfig.expert_activation`` -- ``"swiglu"`` (reference ``ExpertFFN``) or
   ``"silu"`` (non-gated ``down(silu(up x))`` experts);
-* ``MoEConfig.gate_bias`` -- adds a per-expert fp32 logit bias to the gate.
+* ``MoEConfig.gate_bias`` -- adds a per-expert fp32 logit bias to the gate;
+* ``MoEConfig.trainable`` -- with gradients enabled the gate and the layer build an
+  autograd graph (off: outputs carry none, as before).
 
 ``KernelConfig`` tile knobs are accepted and ignored (the reference never read
 them either): tiles are chosen per launch by the CUDA library.
@@ -44,6 +46,7 @@ class MoEConfig:
     routing_implementation: Literal["triton", "torch", "cuda"] = "triton"
     expert_activation: Literal["swiglu", "silu"] = "swiglu"
     gate_bias: bool = False
+    trainable: bool = False
 
 
 @dataclass

@@ -68,7 +68,8 @@ def _no_grad(name: str, *tensors: torch.Tensor | None) -> None:
                            "its inputs")
 
 
-def _index(index: torch.Tensor) -> torch.Tensor:
+def adapter_index(index: torch.Tensor) -> torch.Tensor:
+    """Adapter numbers of any integer type as contiguous int32."""
     if index.dtype.is_floating_point or index.dtype == torch.bool:
         raise ValueError(f"adapter numbers must be integers, got {index.dtype}")
     if index.dtype in (torch.int64, torch.uint32, torch.uint64):
@@ -85,7 +86,7 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, index: t
     flagged (:func:`lightning_router._ext.check_device_errors`)."""
     _ext.require_cuda(base, x, index, *bank)
     _no_grad("adapter_add", base, x, *bank)
-    return _ext.ops().adapter_add(x, _index(index), bank.a, bank.b, bank.scale, base, out,
+    return _ext.ops().adapter_add(x, adapter_index(index), bank.a, bank.b, bank.scale, base, out,
                                   _ext.error_word(x.device.index))
 
 
@@ -96,7 +97,7 @@ def adapter_swiglu(gate: torch.Tensor, up: torch.Tensor, x: torch.Tensor, gate_b
     :func:`adapter_add`.  The banks have the same n, rank and sizes."""
     _ext.require_cuda(gate, up, x, index, *gate_bank, *up_bank)
     _no_grad("adapter_swiglu", gate, up, x, *gate_bank, *up_bank)
-    return _ext.ops().adapter_swiglu(x, _index(index), gate_bank.a, gate_bank.b, gate_bank.scale,
+    return _ext.ops().adapter_swiglu(x, adapter_index(index), gate_bank.a, gate_bank.b, gate_bank.scale,
                                      up_bank.a, up_bank.b, up_bank.scale, gate, up, out,
                                      _ext.error_word(x.device.index))
 
@@ -106,7 +107,7 @@ def adapter_rows(adapter_ids: torch.Tensor, plan, num_adapters: int) -> torch.Te
     adapter per expert, from the tokens' ``adapter_ids`` (T,) in [-1, num_adapters).  Dropped
     rows and tokens without an adapter get -1."""
     _ext.require_cuda(adapter_ids, plan.source_indices)
-    return _ext.ops().adapter_rows(_index(adapter_ids), plan.source_indices, plan.offsets,
+    return _ext.ops().adapter_rows(adapter_index(adapter_ids), plan.source_indices, plan.offsets,
                                    plan.kept_counts, int(num_adapters),
                                    _ext.error_word(adapter_ids.device.index))
 

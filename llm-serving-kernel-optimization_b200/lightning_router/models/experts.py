@@ -18,6 +18,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from lightning_router.kernels.adapters import adapter_add, adapter_swiglu
 from lightning_router.kernels.quantized_matmul import (
     FFN_MODE_PLAIN, FFN_MODE_SILU, FFN_MODE_SWIGLU, WeightTable, grouped_w4a16, table_key,
     weight_table)
@@ -183,6 +184,38 @@ class ExpertGroup(nn.Module):
             if out is None else out
         grouped_w4a16(table, n, FFN_MODE_PLAIN, 2, h, self.hidden_size, seg_start, seg_len,
                       max_rows, out=y)
+        if mark is not None:
+            mark("ffn_out")
+        return y
+
+    def forward_segments_adapted(self, x: torch.Tensor, seg_start: torch.Tensor,
+                                 seg_len: torch.Tensor, max_rows: int, adapters,
+                                 index: torch.Tensor, mark=None) -> torch.Tensor:
+        """:meth:`forward_segments` with low-rank adapters (:class:`ExpertAdapters`) beside
+        every projection; ``index`` holds each row's bank entry (:func:`adapter_rows`).  The
+        projections are rounded to fp16 before their adapters are added (SwiGLU is taken in
+        fp32 from there)."""
+        if not self.quantized:
+            raise RuntimeError("forward_segments_adapted requires quantized experts")
+        n, f = self.num_experts, self.intermediate_size
+        table = self.table(0, n)
+        x = x.half().contiguous()
+
+        def plain(rows, mat, N):
+            return grouped_w4a16(table, n, FFN_MODE_PLAIN, mat, rows, N, seg_start, seg_len,
+                                 max_rows)
+
+        if self.activation == "swiglu":
+            gate = plain(x, 0, f)
+            h = adapter_swiglu(gate, plain(x, 1, f), x, adapters.bank("gate"),
+                               adapters.bank("up"), index, out=gate)
+        else:
+            h = plain(x, 1, f)
+            h = F.silu(adapter_add(h, x, adapters.bank("up"), index, out=h))
+        if mark is not None:
+            mark("ffn_in")
+        y = plain(h, 2, self.hidden_size)
+        adapter_add(y, h, adapters.bank("down"), index, out=y)
         if mark is not None:
             mark("ffn_out")
         return y

@@ -28,8 +28,8 @@ logger = logging.getLogger(__name__)
 
 class _Graph:
     def __init__(self, graph: torch.cuda.CUDAGraph, x: torch.Tensor, out: torch.Tensor,
-                 aux: torch.Tensor):
-        self.graph, self.x, self.out, self.aux = graph, x, out, aux
+                 aux: torch.Tensor, ids: torch.Tensor | None = None):
+        self.graph, self.x, self.out, self.aux, self.ids = graph, x, out, aux, ids
 
 
 class LightningModelRunner:
@@ -67,41 +67,60 @@ class LightningModelRunner:
         self.moe_layer = layer.eval()
         self._graphs.clear()
 
+    def set_adapters(self, adapters) -> None:
+        """Serve these low-rank adapters (:class:`ExpertAdapters`; ``None``: no more).
+        Graphs captured with the former ones are dropped."""
+        layer = self._layer()
+        layer.adapters = None if adapters is None else adapters.to(self.device)
+        self._graphs = {k: g for k, g in self._graphs.items() if g.ids is None}
+
     # -- execution --------------------------------------------------------
     @torch.inference_mode()
-    def capture(self, num_tokens: int, warmup: int = 2) -> None:
+    def capture(self, num_tokens: int, warmup: int = 2, adapters: bool = False) -> None:
         """Record one forward of ``num_tokens`` tokens as a CUDA graph (after
-        ``warmup`` eager runs, which build the weight tables and size the caches)."""
+        ``warmup`` eager runs, which build the weight tables and size the caches).
+        With ``adapters`` the graph takes adapter numbers too."""
         layer = self._layer()
         d = layer.hidden_size
-        key = (num_tokens, d)
+        key = (num_tokens, d, True) if adapters else (num_tokens, d)
+        ids = torch.full((num_tokens,), -1, dtype=torch.int32, device=self.device) \
+            if adapters else None
         x = torch.zeros(num_tokens, d, dtype=torch.float16, device=self.device)
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
             for _ in range(max(1, warmup)):
-                layer(x)
+                layer(x, adapter_ids=ids)
         torch.cuda.current_stream(self.device).wait_stream(side)
         torch.cuda.synchronize(self.device)
         if self._pool is None:
             self._pool = torch.cuda.graph_pool_handle()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, pool=self._pool):
-            out, aux = layer(x)
-        self._graphs[key] = _Graph(g, x, out, aux)
+            out, aux = layer(x, adapter_ids=ids)
+        self._graphs[key] = _Graph(g, x, out, aux, ids)
 
     @torch.inference_mode()
     def execute_model(self, input_ids: torch.Tensor | None,
-                      hidden_states: torch.Tensor) -> torch.Tensor:
+                      hidden_states: torch.Tensor,
+                      adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         """One step through the MoE layer: (..., hidden) -> (..., hidden).
-        ``input_ids`` is accepted for interface compatibility and not used."""
+        ``input_ids`` is accepted for interface compatibility and not used;
+        ``adapter_ids`` gives each token its adapter (:meth:`set_adapters`), -1 for none."""
         layer = self._layer()
         shape = hidden_states.shape
         h = hidden_states.reshape(-1, shape[-1])
-        gr = self._graphs.get((h.shape[0], h.shape[1]))
+        key = (h.shape[0], h.shape[1])
+        gr = self._graphs.get(key if adapter_ids is None else (*key, True))
         if gr is None:
-            out, _ = layer(h)
+            out, _ = layer(h, adapter_ids=adapter_ids)
             return out.view(shape).to(hidden_states.dtype)
+        if adapter_ids is not None:
+            from lightning_router.kernels.adapters import adapter_index
+            if adapter_ids.numel() != h.shape[0]:
+                raise ValueError(f"adapter_ids has {adapter_ids.numel()} entries for "
+                                 f"{h.shape[0]} tokens")
+            gr.ids.copy_(adapter_index(adapter_ids))
         gr.x.copy_(h)
         gr.graph.replay()
         return gr.out.clone().view(shape).to(hidden_states.dtype)

@@ -51,9 +51,9 @@ class LightningRouterWorker:
             self.runner.capture(int(n))
 
     @torch.inference_mode()
-    def execute_model(self, input_ids: torch.Tensor | None,
-                      hidden_states: torch.Tensor) -> torch.Tensor:
-        return self.runner.execute_model(input_ids, hidden_states)
+    def execute_model(self, input_ids: torch.Tensor | None, hidden_states: torch.Tensor,
+                      adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        return self.runner.execute_model(input_ids, hidden_states, adapter_ids)
 
 
 class ExpertParallelWorker(LightningRouterWorker):
@@ -78,10 +78,12 @@ class ExpertParallelWorker(LightningRouterWorker):
             exchange=self.serving_config.get("ep_exchange", "peer"))
 
     @torch.inference_mode()
-    def execute_model(self, input_ids: torch.Tensor | None,
-                      hidden_states: torch.Tensor) -> torch.Tensor:
+    def execute_model(self, input_ids: torch.Tensor | None, hidden_states: torch.Tensor,
+                      adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         if self.ep is None:
             raise RuntimeError("load_model() has not been called")
+        if adapter_ids is not None:
+            raise NotImplementedError("adapters are served by single-GPU workers")
         shape = hidden_states.shape
         out, _ = self.ep.forward(hidden_states.reshape(-1, shape[-1]))
         return out.view(shape).to(hidden_states.dtype)
