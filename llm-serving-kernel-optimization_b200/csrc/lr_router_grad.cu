@@ -738,9 +738,13 @@ static GatePlan gate_plan(int T, int d, int E) {
   p.groups = (E + 63) / 64;
   p.chunks = (T + kChunk - 1) / kChunk;
   const long cols = long((d + kDwCols - 1) / kDwCols) * p.groups;
-  p.per_block = int(p.chunks * cols / (E > 32 ? kTargetBlocks : 2 * kTargetBlocks));
-  if (p.per_block < 1) p.per_block = 1;
+  const long fill = E > 32 ? kTargetBlocks : 2 * kTargetBlocks;
+  p.per_block = int((p.chunks * cols + fill - 1) / fill);
   p.splits = (p.chunks + p.per_block - 1) / p.per_block;
+  if (cols * p.splits > fill && p.splits > 1) {  // no few blocks in a wave of their own
+    p.per_block = int((p.chunks + p.splits - 2) / (p.splits - 1));
+    p.splits = (p.chunks + p.per_block - 1) / p.per_block;
+  }
   p.frag = 0;
   p.down = p.frag + size_t(p.chunks) * (kChunk / 16) * (p.E8 / 8) * 512;
   p.colsum = p.down + align256(size_t(p.chunks) * p.E8 * sizeof(float));

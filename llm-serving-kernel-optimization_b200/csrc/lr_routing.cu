@@ -150,14 +150,16 @@ __global__ void __launch_bounds__(kGateWarps * 32)
 // and NT 8-expert groups at once, and the chunks are added in the same order.
 // Only the operands' way differs: rows come in by 16-byte asynchronous copies, 32
 // k at a time into the warp's own ring, and reach the registers by ldmatrix (in
-// place of 4-byte loads from global memory).  16384 x 4096 rows, 8 experts: see
-// lr_gate_logits.
+// place of 4-byte loads from global memory).  16384 x 4096 rows, 8 experts: 28 us
+// (HBM floor 21) against 61; 8111 x 2048, 64 experts: 18 against 63.
 constexpr int kGateTiledTokens = 2048;
 constexpr int kGlPitch = 80;  // bytes of a 32-k row in the ring: ldmatrix rows in different banks
 
+// Stages of the ring, as measured: two where that lets two blocks share an SM or
+// one hold 64 experts, more for the half-sized tiles of smaller batches.
 template <int MTL, int NT>
 constexpr int gate_tile_stages() {
-  return (MTL * 16 + NT * 8) * kGlPitch * kGateWarps * 4 <= 220 * 1024 ? 4 : 3;
+  return MTL == 2 ? 4 : NT == 4 ? 3 : 2;
 }
 
 LR_DEVICE void ldmatrix_x4(uint32_t (&r)[4], uint32_t saddr) {
@@ -1364,10 +1366,15 @@ extern "C" int lr_gate_logits(const void* h, const void* wg, const float* bias, 
   if (T >= kGateTiledTokens && aligned16(h) && aligned16(wg)) {
     const __half* hp = static_cast<const __half*>(h);
     const __half* wp = static_cast<const __half*>(wg);
+    // tiles of 32 tokens while tiles of 64 would leave SMs idle (3000 x 4096, 8
+    // experts: 9 against 13 us)
+    if (E <= 16 && T < 64 * 148)
+      return E <= 8 ? launch_gate_tiled<2, 1>(hp, wp, bias, T, d, E, logits, stream)
+                    : launch_gate_tiled<2, 2>(hp, wp, bias, T, d, E, logits, stream);
     return E <= 8    ? launch_gate_tiled<4, 1>(hp, wp, bias, T, d, E, logits, stream)
            : E <= 16 ? launch_gate_tiled<4, 2>(hp, wp, bias, T, d, E, logits, stream)
            : E <= 32 ? launch_gate_tiled<4, 4>(hp, wp, bias, T, d, E, logits, stream)
-                     : launch_gate_tiled<2, 8>(hp, wp, bias, T, d, E, logits, stream);
+                     : launch_gate_tiled<4, 8>(hp, wp, bias, T, d, E, logits, stream);
   }
   const int n_eg = (E + 31) / 32;
   const long blocks = long((T + 15) / 16) * n_eg;
