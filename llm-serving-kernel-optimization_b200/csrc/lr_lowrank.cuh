@@ -660,10 +660,10 @@ static int launch_expand(ExpandArgs p, cudaStream_t stream) {
   const long windows = (p.R + W - 1) / W;
   const int cgs = (p.N + 31) / 32;
   int gpc = consumers<MODE>();
-  if (MT == 1) {
-    // one wave of two blocks per SM where that leaves a warp one to eight groups
+  if (MT == 1 || MODE == kExpandProduct) {
+    // one wave of two blocks per SM where that leaves a warp 1 to 16 groups
     const long per = (windows * cgs + 2 * kTargetBlocks * 8 - 1) / (2 * kTargetBlocks * 8);
-    gpc = int(per < 1 ? 1 : per > 8 ? 8 : per) * 8;
+    gpc = int(per < 1 ? 1 : per > 16 ? 16 : per) * 8;
   } else {
     // one tile's columns per block, more while the grid stays above eight blocks per SM
     while (gpc < 50 && windows * ((cgs + 2 * gpc - 1) / (2 * gpc)) >= 8 * kTargetBlocks) gpc *= 2;
