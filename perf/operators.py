@@ -18,7 +18,6 @@ The operators (``op``):
               (form ``swiglu``).
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -31,14 +30,15 @@ LBW = 0.01
 EPS = 1e-9
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
     """The framework's modules, imported once (its package directory goes on sys.path, as for any user)."""
-    where = str(Path(__file__).resolve().parents[1] / "llm-serving-kernel-optimization_b200")
-    if where not in sys.path:
-        sys.path.insert(0, where)
-    from lightning_router.kernels import adapters, routing_grad
-    return adapters, routing_grad
+    if not hasattr(_package, "modules"):
+        where = str(Path(__file__).resolve().parents[1] / "llm-serving-kernel-optimization_b200")
+        if where not in sys.path:
+            sys.path.insert(0, where)
+        from lightning_router.kernels import adapters, routing_grad
+        _package.modules = adapters, routing_grad
+    return _package.modules
 
 
 # ---------------------------------------------------------------------------
