@@ -118,7 +118,10 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
 
 std::vector<at::Tensor> balanced_gating(const at::Tensor& logits, const OptTensor& token_mask,
                                         int64_t k, double lbw) {
-  return BalancedGating::apply(logits, token_mask, k, lbw);
+  auto out = BalancedGating::apply(logits, token_mask, k, lbw);
+  at::AutoDispatchBelowADInplaceOrView below;
+  out[2] = out[2].narrow(0, 0, out[2].size(0) - 1);  // without the live count
+  return out;
 }
 
 // ---------------------------------------------------------------------------
@@ -152,13 +155,11 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     // before the backward pass is noticed
     ctx->save_for_backward({hh.data_ptr() == h.data_ptr() ? h : hh,
                             wh.data_ptr() == w.data_ptr() ? w : wh});
-    ctx->saved_data["need_h"] = h.requires_grad();
-    ctx->saved_data["need_w"] = w.requires_grad();
-    ctx->saved_data["need_b"] = given(bias) && bias->requires_grad();
-    ctx->saved_data["h_type"] = int64_t(h.scalar_type());
-    ctx->saved_data["w_type"] = int64_t(w.scalar_type());
-    ctx->saved_data["b_type"] = int64_t(given(bias) ? bias->scalar_type() : at::kFloat);
-    ctx->saved_data["b_shape"] = given(bias) ? bias->sizes().vec() : std::vector<int64_t>{E};
+    ctx->saved_data["p"] = std::vector<int64_t>{
+        h.requires_grad(), w.requires_grad(), given(bias) && bias->requires_grad(),
+        int64_t(h.scalar_type()), int64_t(w.scalar_type()),
+        int64_t(given(bias) ? bias->scalar_type() : at::kFloat)};
+    if (given(bias)) ctx->saved_data["b_shape"] = bias->sizes().vec();
     return out;
   }
 
@@ -170,9 +171,8 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     c10::cuda::CUDAGuard g(h.device());
     const at::Tensor dl = grads[0].contiguous();
     const int64_t T = h.size(0), d = h.size(1), E = w.size(0);
-    const bool need_h = ctx->saved_data["need_h"].toBool();
-    const bool need_b = ctx->saved_data["need_b"].toBool();
-    const bool need_w = ctx->saved_data["need_w"].toBool() || need_b;
+    const auto saved_p = ctx->saved_data["p"].toIntVector();
+    const bool need_h = saved_p[0], need_b = saved_p[2], need_w = saved_p[1] || need_b;
     const auto fopt = dl.options();
     at::Tensor dh, dw, db;
     if (need_h) dh = at::empty({T, d}, h.options());
@@ -185,10 +185,10 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
                                   need_b ? db.data_ptr<float>() : nullptr, ws.data_ptr(),
                                   size_t(ws.numel()), cur_stream()),
                  "gate_projection (backward)");
-    if (need_h) dh = dh.to(at::ScalarType(ctx->saved_data["h_type"].toInt()));
-    if (need_w) dw = dw.to(at::ScalarType(ctx->saved_data["w_type"].toInt()));
+    if (need_h) dh = dh.to(at::ScalarType(saved_p[3]));
+    if (need_w) dw = dw.to(at::ScalarType(saved_p[4]));
     if (need_b)
-      db = db.to(at::ScalarType(ctx->saved_data["b_type"].toInt()))
+      db = db.to(at::ScalarType(saved_p[5]))
                .view(ctx->saved_data["b_shape"].toIntVector());
     return {dh, dw, db};
   }

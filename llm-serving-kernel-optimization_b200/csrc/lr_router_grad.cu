@@ -264,6 +264,12 @@ __global__ void __launch_bounds__(1024)
 // read, nothing kept from the forward but the ids), one launch, no reductions
 // across tokens.  With `csr` the counts are the differences of CSR offsets and
 // every token is live.
+// dl is a difference of nearly equal terms where a router is balanced or one
+// expert takes all of a token's weight, so the terms are taken relative to the
+// first selected expert's (0): adding a constant to dp changes nothing, and with
+// d'_j = dw_j - dw_0, c' = sum_j d'_j w_j, sum_j w_j = 1 - 1e-9 / q,
+//   dp_i - dp_0 = bal_i - bal_0 + (i selected ? d'_i : c' - dw_0 1e-9 / q) / q,
+// bal_i = dloss lbw E (f_i - 1/E) / n with the difference in double.
 template <int LPT>
 __global__ void __launch_bounds__(kGateThreads)
     balanced_gating_backward_kernel(const float* __restrict__ logits,
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(kGateThreads)
     bal[i] = 0.f;
     if (d_aux && e < E && n > 0) {
       const int c = csr ? counts[e + 1] - counts[e] : counts[e];
-      bal[i] = d_aux[0] * float(double(lbw) * E * (double(c) / (double(n) * k)) / n);
+      bal[i] = d_aux[0] * float(double(lbw) * (double(E) * c / (double(n) * k) - 1.0) / n);
     }
   }
   const long stride = long(gridDim.x) * kW * per_warp;
@@ -298,24 +304,34 @@ __global__ void __launch_bounds__(kGateThreads)
     float v[8], p[8], dw[8];
     row_softmax<LPT>(logits, t, valid, E, vec, l, v, p);
     unsigned taken = 0;
+    float dw0 = 0.f, bal0 = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) dw[i] = 0.f;
-    if (d_w && valid) {
+    if (d_w) {
+      int first = 0;
 #pragma unroll
       for (int j = 0; j < kMaxTopK; ++j) {
         if (j < k) {
-          const size_t s = size_t(t) * k + j;
+          const size_t s = size_t(valid ? t : 0) * k + j;
           const int e = __ldg(expert_ids + s);
           const float g = __ldg(d_w + s);
+          if (j == 0) {
+            first = e;
+            dw0 = g;
+          }
           if ((e >> 2) % LPT == l) {
             const int i = (e >> 2) / LPT * 4 + (e & 3);
             taken |= 1u << i;
 #pragma unroll
             for (int x = 0; x < 8; ++x)
-              if (x == i) dw[x] = g;
+              if (x == i) dw[x] = g - dw0;
           }
         }
       }
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (x == (first >> 2) / LPT * 4 + (first & 3)) bal0 = bal[x];
+      bal0 = __shfl_sync(0xffffffffu, bal0, (lane & ~(LPT - 1)) + ((first >> 2) & (LPT - 1)));
     }
     float q = 0.f, c = 0.f;
 #pragma unroll
@@ -327,10 +343,11 @@ __global__ void __launch_bounds__(kGateThreads)
     }
     q = group_sum<LPT>(q) + 1e-9f;
     c = group_sum<LPT>(c) / q;
+    const float rest = d_w ? (c - dw0 * (1e-9f / q)) / q : 0.f;
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      dw[i] = bal[i] + (((taken >> i) & 1u) ? (dw[i] - c) / q : 0.f);
+      dw[i] = (bal[i] - bal0) + (((taken >> i) & 1u) ? dw[i] / q : rest);
       dot = fmaf(p[i], dw[i], dot);
     }
     dot = group_sum<LPT>(dot);

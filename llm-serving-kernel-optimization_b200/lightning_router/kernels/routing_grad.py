@@ -61,9 +61,8 @@ def balanced_gating(logits: torch.Tensor, top_k: int, load_balance_weight: float
     zero gradient, whatever its logits hold.  ``E <= 64``, ``top_k <= min(E, 8)``; T may be 0.
     """
     _ext.require_cuda(logits, token_mask)
-    ids, weights, stats, aux = _ext.ops().balanced_gating(logits.float(), token_mask, int(top_k),
-                                                          float(load_balance_weight))
-    return BalancedGating(ids, weights, stats[:-1], aux)
+    return BalancedGating(*_ext.ops().balanced_gating(logits.float(), token_mask, int(top_k),
+                                                      float(load_balance_weight)))
 
 
 def gate_projection(hidden: torch.Tensor, gate_weight: torch.Tensor,

@@ -203,6 +203,32 @@ def test_balanced_gating_gradient_against_differences():
     assert abs(got - want) <= 1e-7 + scale * 200 * U
 
 
+@pytest.mark.parametrize("T,E,k", [(20000, 2, 1), (50000, 8, 1), (30000, 64, 1), (4000, 5, 2)])
+def test_balanced_gating_gradient_of_a_balanced_router(T, E, k):
+    """Nearly equal counts, weights of (nearly) 1: the gradient is a difference of nearly equal
+    terms, which is taken before it is rounded."""
+    from lightning_router.kernels.routing_grad import balanced_gating
+    g = _gen(T + E)
+    logits = _randn(g, T, E)
+    dw, da = _randn(g, T * k, std=1.0 / T), torch.ones((), device=DEV)
+    if k == 2:
+        logits[:, 0] += 18.0        # one expert has all of the weight
+    leaf = logits.clone().requires_grad_()
+    out = balanced_gating(leaf, k)
+    (dl,) = torch.autograd.grad((out.gate_weights, out.aux_loss), leaf, (dw, da))
+    # differences of dw and counts are exact or rounded once: the error is that of p alone,
+    # in relation to the gradient itself: the exact form from 64-bit differences
+    ids, p, w, q, counts, _, f, _, n = gating64(logits, k, None)
+    d = dw.double().view(T, k)
+    d0 = d[:, :1]
+    bal = LBW * E * (f - 1.0 / E) / n
+    rest = (((d - d0) * (p.gather(1, ids) / q)).sum(1, keepdim=True) - d0 * 1e-9 / q) / q
+    dp = (bal[None, :] - bal[ids[:, :1]]) + rest.expand(T, E).scatter(1, ids, (d - d0) / q)
+    want = p * (dp - (p * dp).sum(1, keepdim=True))
+    eps = float(_spread(logits).max()) + E + 32
+    assert float((dl.double() - want).norm() / want.norm()) <= eps * 4 * U
+
+
 # ---------------------------------------------------------------------------
 # gate projection
 # ---------------------------------------------------------------------------
