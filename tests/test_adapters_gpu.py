@@ -78,7 +78,10 @@ SHAPES = [  # rows, requests, K, N, adapters, rank
     (64, 64, 1024, 2048, 64, 16), (65, 3, 72, 40, 2, 40), (200, 50, 520, 512, 33, 104),
     (256, 16, 2048, 256, 16, 16), (257, 5, 2048, 1000, 4, 16), (300, 300, 256, 256, 64, 32),
     (333, 9, 136, 8, 6, 64), (1111, 9, 2048, 1408, 6, 64), (1500, 2, 64, 2056, 2, 128),
-    (4099, 11, 512, 512, 7, 32), (5000, 5000, 128, 64, 40, 16)]
+    (4099, 11, 512, 512, 7, 32), (5000, 5000, 128, 64, 40, 16),
+    # windows of 64 rows with streamed base rows: one, a few and many groups in a window
+    (9600, 2, 64, 520, 2, 8), (4099, 11, 512, 1544, 7, 32), (3000, 40, 136, 1808, 33, 104),
+    (2500, 9, 1000, 2056, 6, 64), (5000, 5000, 128, 1032, 40, 16), (19137, 700, 72, 232, 64, 24)]
 
 
 @pytest.mark.parametrize("R,requests,K,N,n,r", SHAPES)
@@ -113,7 +116,7 @@ def test_rows_in_any_order():
         _check_add(out, base[order], x[order], bank, index[order])
 
 
-@pytest.mark.parametrize("R", [24, 400])
+@pytest.mark.parametrize("R", [24, 400, 19000])   # the last: streamed windows
 def test_other_requests_infinities_stay_theirs(R):
     from lightning_router.kernels.adapters import AdapterBank, adapter_add
     g = _gen(4)
@@ -166,7 +169,10 @@ def test_bad_adapter_numbers_are_flagged_and_taken_as_none():
 
 @pytest.mark.parametrize("R,requests,K,N,n,r", [
     (1, 1, 64, 64, 1, 8), (5, 5, 72, 40, 3, 16), (128, 64, 1024, 1408, 64, 16),
-    (100, 7, 256, 520, 4, 128), (257, 4, 512, 264, 8, 32), (1000, 20, 136, 96, 16, 48)])
+    (100, 7, 256, 520, 4, 128), (257, 4, 512, 264, 8, 32), (1000, 20, 136, 96, 16, 48),
+    # windows of 32 rows with streamed base rows
+    (2001, 3, 256, 1288, 3, 16), (1500, 90, 136, 1800, 7, 24), (1100, 1100, 64, 2312, 40, 40),
+    (9000, 12, 520, 264, 5, 128)])
 def test_adapter_swiglu(R, requests, K, N, n, r):
     from lightning_router.kernels.adapters import adapter_swiglu
     g = _gen(R + K + N)
