@@ -286,16 +286,20 @@ __global__ void __launch_bounds__(kGateThreads)
   const int l = lane % LPT;
   const int per_warp = 32 / LPT;
   const int n = csr ? T : counts[E];
-  float bal[8];  // the loss' gradient in p_e
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int e = (i >> 2) * 4 * LPT + 4 * l + (i & 3);
-    bal[i] = 0.f;
+  __shared__ float s_bal[8 * LPT];  // the loss' gradient in p_e
+  if (threadIdx.x < 8 * LPT) {
+    const int e = threadIdx.x;
+    float b = 0.f;
     if (d_aux && e < E && n > 0) {
       const int c = csr ? counts[e + 1] - counts[e] : counts[e];
-      bal[i] = d_aux[0] * float(double(lbw) * (double(E) * c / (double(n) * k) - 1.0) / n);
+      b = d_aux[0] * float(double(lbw) * (double(E) * c / (double(n) * k) - 1.0) / n);
     }
+    s_bal[e] = b;
   }
+  __syncthreads();
+  float bal[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) bal[i] = s_bal[(i >> 2) * 4 * LPT + 4 * l + (i & 3)];
   const long stride = long(gridDim.x) * kW * per_warp;
   for (long tb = (long(blockIdx.x) * kW + warp) * per_warp; tb < T; tb += stride) {
     const int t = int(tb) + lane / LPT;
@@ -328,10 +332,7 @@ __global__ void __launch_bounds__(kGateThreads)
           }
         }
       }
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (x == (first >> 2) / LPT * 4 + (first & 3)) bal0 = bal[x];
-      bal0 = __shfl_sync(0xffffffffu, bal0, (lane & ~(LPT - 1)) + ((first >> 2) & (LPT - 1)));
+      bal0 = s_bal[first & (8 * LPT - 1)];
     }
     float q = 0.f, c = 0.f;
 #pragma unroll
