@@ -10,7 +10,8 @@
  * caller reads back when it chooses.
  *
  * Each entry point names the reference (AlexanderLeonida/LLM-Serving-Kernel-
- * Optimization) interface it replaces.
+ * Optimization) interface it replaces; router training and adapters have none
+ * there.
  */
 #ifndef LIGHTNING_ROUTER_H
 #define LIGHTNING_ROUTER_H

@@ -23,6 +23,9 @@ namespace lr {
 // first) keys.  Probability sums and counts stay in registers over a lane's
 // tokens, go through shuffles and shared memory to one partial per block and
 // expert, and are summed over blocks in double in block order: no atomics.
+// Latency bounds it: 262144 tokens x 8 experts take 10 us (12.6 MB, 2 us of HBM)
+// and 8192 x 64 top-6 takes 8, of which the selection's shuffles are most; one
+// thread per token with 64 experts in registers took 60 at 777 tokens.
 constexpr int kGateThreads = 512;
 constexpr int kGateBlocksMax = 296;  // 2 per SM
 
@@ -230,7 +233,8 @@ __global__ void __launch_bounds__(kGateThreads)
   write_gating_stats(E, k, lbw, s_tp, s_tc, counts, aux);
 }
 
-// One block: totals over the B blocks' partials, a warp per expert.
+// One block: totals over the B blocks' partials, a warp per expert (5 us; a ticket
+// and a last block in the kernel above would need a memset before it instead).
 __global__ void __launch_bounds__(1024)
     gating_stats_kernel(GatingParts parts, int B, int E, int k, float lbw,
                         int32_t* __restrict__ counts, float* __restrict__ aux) {
@@ -270,6 +274,7 @@ __global__ void __launch_bounds__(1024)
 // d'_j = dw_j - dw_0, c' = sum_j d'_j w_j, sum_j w_j = 1 - 1e-9 / q,
 //   dp_i - dp_0 = bal_i - bal_0 + (i selected ? d'_i : c' - dw_0 1e-9 / q) / q,
 // bal_i = dloss lbw E (f_i - 1/E) / n with the difference in double.
+// Forward, statistics and this: 27 us at 262144 x 8, 19 at 8192 x 64 top-6.
 template <int LPT>
 __global__ void __launch_bounds__(kGateThreads)
     balanced_gating_backward_kernel(const float* __restrict__ logits,
@@ -428,7 +433,7 @@ constexpr int kHPitch = kDwCols * 2 + 16;  // bytes: ldmatrix rows in different 
 // powers of two that undo the scaling [chunk][E8], column sums [chunk][E8], and
 // the transposed weight [d][E8] (zero past E) for the row gradient.  Blocks
 // [0, chunks * groups) split dl, a chunk and 64 experts each; the rest transpose
-// 64 columns each.
+// 64 columns each.  6 to 8 us beside the products' 20 to 25.
 struct SplitArgs {
   const float* dl;
   const __half* wg;
@@ -478,7 +483,8 @@ __global__ void __launch_bounds__(256) gate_split_kernel(SplitArgs p) {
     float m = 0.f, sum = 0.f;
     if (e < ne8) {
       for (int t = q; t < kChunk; t += 4) {
-        m = fmaxf(m, fabsf(s_dl[t][e]));
+        const float a = fabsf(s_dl[t][e]);
+        if (a < INFINITY) m = fmaxf(m, a);
         sum += s_dl[t][e];
       }
     }
@@ -487,7 +493,7 @@ __global__ void __launch_bounds__(256) gate_split_kernel(SplitArgs p) {
     if (q == 0) {
       m = fmaxf(fmaxf(s_red[0][e], s_red[1][e]), fmaxf(s_red[2][e], s_red[3][e]));
       int ex = 0;
-      if (m > 0.f && m < INFINITY) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
+      if (m > 0.f) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
       s_up[e] = __uint_as_float(unsigned(127 + ex) << 23);
       if (e < ne8) p.down[size_t(chunk) * p.E8 + e0 + e] = __uint_as_float(unsigned(127 - ex) << 23);
     }
@@ -531,7 +537,9 @@ LR_DEVICE void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t saddr) {
 
 // A block: 256 columns of h, up to 64 experts (blockIdx.z), a range of chunks.
 // Stages of 64 tokens (rows of h and dl fragments) come in by cp.async, three
-// deep.
+// deep.  Reading h bounds it with 8 experts (16384 x 4096: 24 us, 5.5 TB/s), the
+// shared-memory reads of 2 x 64 gradient rows with 64 (8111 x 2048: 21 us).  tf32
+// products of the unsplit gradients took 38 and 117 us.
 template <int MTL>
 __global__ void __launch_bounds__(256)
     gate_dw_kernel(const __half* __restrict__ h, const uint4* __restrict__ frag,
@@ -787,6 +795,7 @@ static int launch_dw(const __half* h, const uint4* frag, const float* down, int 
 // ---------------------------------------------------------------------------
 // weighted combine: gradients
 // ---------------------------------------------------------------------------
+// HBM bounds it: 16384 tokens x 2 slots x 4096 in 107 us, 6.3 TB/s.
 // WPT warps share a token's row: the row of dout is read once, each kept slot's
 // y row once, dy written once; the dot products are summed over lanes and warps
 // in a fixed order.  Rows no slot keeps (the tail of an over-full expert's

@@ -135,6 +135,31 @@ def test_other_requests_infinities_stay_theirs(R):
     assert not torch.isfinite(out[index == 1]).any()
 
 
+@pytest.mark.parametrize("R", [40, 600])
+def test_infinite_rows_are_infinite_where_the_products_are(R):
+    """One infinity in a row of x: every product with it is infinite, of the sign of its factor
+    (all of B positive, one element of A per rank not zero there)."""
+    from lightning_router.kernels.adapters import AdapterBank, adapter_add
+    g = _gen(14)
+    K, N, r = 64, 512, 8
+    x, base = _randn(g, R, K), _randn(g, R, N)
+    a, b = _randn(g, 1, r, K), _randn(g, 1, N, r).abs() + 0.01
+    a[0, :, 3] = 0.0
+    a[0, 2, 3] = -1.0             # the infinity reaches one rank value only
+    x[5, 3] = float("inf")
+    index = torch.zeros(R, dtype=torch.int32, device=DEV)
+    x[7] *= 600.0                 # a large finite row beside it
+    out = adapter_add(base, x, AdapterBank(a, b), index)
+    # 0 * inf is NaN in seven of the eight rank values, so the row is NaN as the formula's
+    v = x.double() @ a[0].double().t()
+    assert torch.isnan(v[5]).sum() == 7 and torch.isnan(out[5]).all()
+    keep = torch.arange(R, device=DEV) != 5
+    _check_add(out[keep], base[keep], x[keep], AdapterBank(a, b), index[keep])
+    a[0, :, 3] = -1.0             # now all rank values are -inf
+    out = adapter_add(base, x, AdapterBank(a, b), index)
+    assert torch.equal(out[5], torch.full((N,), float("-inf"), device=DEV).half())
+
+
 @pytest.mark.parametrize("magnitude", [1e-6, 1.0, 6e4])
 def test_small_and_large_middle_values(magnitude):
     """v = x A^T far outside fp16 (up to 1e9, down to 1e-9) is not rounded to it."""
@@ -217,6 +242,12 @@ def test_expert_row_numbers():
     adapter_rows(torch.full((T,), n, device=DEV), plan, n)
     with pytest.raises(RuntimeError, match="adapter"):
         _ext.check_device_errors()
+    short = adapter_rows(ad[:100], plan, n)      # ids of another batch: flagged, not read past
+    with pytest.raises(RuntimeError, match="source token"):
+        _ext.check_device_errors()
+    tokens = plan.source_indices
+    assert torch.equal(short[tokens < 100], index[tokens < 100])
+    assert bool((short[tokens >= 100] == -1).all())
 
 
 def test_quantized_matmul_adapters():
@@ -249,6 +280,8 @@ def test_strides_alignment_and_no_rows():
     rows[::2] = index
     assert torch.equal(adapter_add(base, x, bank, rows[::2]), out)
     assert adapter_add(base[:0], x[:0], bank, index[:0]).shape == (0, N)
+    from lightning_router.kernels.adapters import adapter_swiglu
+    assert adapter_swiglu(base[:0], base[:0], x[:0], bank, bank, index[:0]).shape == (0, N)
 
 
 def test_streams_and_graphs():

@@ -75,7 +75,7 @@ def _spread(logits):
     return (logits.amax(1, keepdim=True) - logits.amin(1, keepdim=True)).double()
 
 
-GATING = [(1, 2, 1), (1, 64, 8), (7, 3, 3), (31, 5, 2), (64, 8, 2), (300, 16, 4), (333, 17, 5),
+GATING = [(5, 1, 1), (1, 2, 1), (1, 64, 8), (7, 3, 3), (31, 5, 2), (64, 8, 2), (300, 16, 4), (333, 17, 5),
           (512, 32, 8), (513, 33, 1), (1000, 64, 6), (4097, 61, 7), (70001, 8, 2), (40000, 64, 6)]
 
 
