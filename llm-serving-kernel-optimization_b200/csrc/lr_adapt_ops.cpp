@@ -50,9 +50,11 @@ void check_once(const char* what) {
 // ---------------------------------------------------------------------------
 // balanced gating
 // ---------------------------------------------------------------------------
+// The functions' outputs are the differentiable ones; the others leave through `rest`.
 struct BalancedGating : public torch::autograd::Function<BalancedGating> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& logits_in,
-                               const OptTensor& mask_in, int64_t k, double lbw) {
+                               const OptTensor& mask_in, int64_t k, double lbw,
+                               std::vector<at::Tensor>* rest) {
     TORCH_CHECK(logits_in.is_cuda(), "logits must be a CUDA tensor");
     TORCH_CHECK(logits_in.dim() == 2 && logits_in.scalar_type() == at::kFloat,
                 "logits: (T,E) fp32");
@@ -84,12 +86,12 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
                                     aux.data_ptr<float>(), wsb ? ws.data_ptr() : nullptr, wsb,
                                     cur_stream()),
                  "balanced_gating");
-    ctx->mark_non_differentiable({ids, stats});
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({logits_in, mask, ids, stats});
     ctx->saved_data["k"] = k;
     ctx->saved_data["lbw"] = lbw;
-    return {ids, gw, stats, aux};
+    *rest = {ids, stats.narrow(0, 0, E)};  // without the live count
+    return {gw, aux};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -97,11 +99,11 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
     const auto saved = ctx->get_saved_variables();
     const int64_t k = ctx->saved_data["k"].toInt();
     const double lbw = ctx->saved_data["lbw"].toDouble();
-    if (!grads[1].defined() && !grads[3].defined()) return {{}, {}, {}, {}};
+    if (!grads[0].defined() && !grads[1].defined()) return {{}, {}, {}, {}, {}};
     c10::cuda::CUDAGuard g(saved[0].device());
     const at::Tensor logits = saved[0].detach().contiguous();
-    const at::Tensor dw = grads[1].defined() ? grads[1].contiguous() : grads[1];
-    const at::Tensor da = grads[3].defined() ? grads[3].contiguous() : grads[3];
+    const at::Tensor dw = grads[0].defined() ? grads[0].contiguous() : grads[0];
+    const at::Tensor da = grads[1].defined() ? grads[1].contiguous() : grads[1];
     auto dl = at::empty_like(logits);
     check_status(
         lr_balanced_gating_backward(
@@ -112,16 +114,15 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
             da.defined() ? da.data_ptr<float>() : nullptr, int(logits.size(0)),
             int(logits.size(1)), int(k), float(lbw), dl.data_ptr<float>(), cur_stream()),
         "balanced_gating (backward)");
-    return {dl, {}, {}, {}};
+    return {dl, {}, {}, {}, {}};
   }
 };
 
 std::vector<at::Tensor> balanced_gating(const at::Tensor& logits, const OptTensor& token_mask,
                                         int64_t k, double lbw) {
-  auto out = BalancedGating::apply(logits, token_mask, k, lbw);
-  at::AutoDispatchBelowADInplaceOrView below;
-  out[2] = out[2].narrow(0, 0, out[2].size(0) - 1);  // without the live count
-  return out;
+  std::vector<at::Tensor> rest;
+  const auto out = BalancedGating::apply(logits, token_mask, k, lbw, &rest);
+  return {rest[0], out[0], rest[1], out[1]};
 }
 
 // ---------------------------------------------------------------------------
@@ -208,7 +209,8 @@ using DispatchSig = std::vector<at::Tensor>(const OptTensor&, const at::Tensor&,
 // aux 5, permuted 6, routing weights 7, sources 8, slot rows 9.
 struct DispatchTokens : public torch::autograd::Function<DispatchTokens> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& logits,
-                               int64_t k, int64_t capacity, double lbw, const OptTensor& err) {
+                               int64_t k, int64_t capacity, double lbw, const OptTensor& err,
+                               std::vector<at::Tensor>* all) {
     TORCH_CHECK(x.is_cuda() && logits.is_cuda(), "x and logits must be CUDA tensors");
     TORCH_CHECK(x.dim() == 2 && x.scalar_type() == at::kHalf, "x: (T,d) fp16");
     TORCH_CHECK(logits.dim() == 2 && logits.scalar_type() == at::kFloat &&
@@ -220,15 +222,15 @@ struct DispatchTokens : public torch::autograd::Function<DispatchTokens> {
     static const auto op = c10::Dispatcher::singleton()
                                .findSchemaOrThrow("lightning_router::topk_gating_dispatch", "")
                                .typed<DispatchSig>();
-    auto out = op.call(rows16(x, at::kHalf), logits.detach().contiguous(), k, capacity, lbw, true,
-                       true, err);
-    ctx->mark_non_differentiable({out[0], out[2], out[3], out[4], out[7], out[8], out[9]});
+    *all = op.call(rows16(x, at::kHalf), logits.detach().contiguous(), k, capacity, lbw, true,
+                   true, err);
+    const auto& out = *all;
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({logits, out[0], out[3], out[9]});
     ctx->saved_data["k"] = k;
     ctx->saved_data["lbw"] = lbw;
     ctx->saved_data["d"] = x.size(1);
-    return out;
+    return {out[1], out[5], out[6]};
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -240,16 +242,16 @@ struct DispatchTokens : public torch::autograd::Function<DispatchTokens> {
     const int64_t k = ctx->saved_data["k"].toInt(), d = ctx->saved_data["d"].toInt();
     const double lbw = ctx->saved_data["lbw"].toDouble();
     at::Tensor dx, dl;
-    if (grads[6].defined()) {
-      const at::Tensor dp = rows16(grads[6], at::kHalf);
+    if (grads[2].defined()) {
+      const at::Tensor dp = rows16(grads[2], at::kHalf);
       dx = at::empty({T, d}, dp.options());
       check_status(lr_dispatch_backward(dp.data_ptr(), saved[3].data_ptr<int32_t>(), int(T), int(k),
                                         int(d), dx.data_ptr(), cur_stream()),
                    "dispatch_tokens (backward)");
     }
-    if (grads[1].defined() || grads[5].defined()) {
-      const at::Tensor dw = grads[1].defined() ? grads[1].contiguous() : grads[1];
-      const at::Tensor da = grads[5].defined() ? grads[5].contiguous() : grads[5];
+    if (grads[0].defined() || grads[1].defined()) {
+      const at::Tensor dw = grads[0].defined() ? grads[0].contiguous() : grads[0];
+      const at::Tensor da = grads[1].defined() ? grads[1].contiguous() : grads[1];
       dl = at::empty_like(logits);
       check_status(lr_balanced_gating_backward(
                        logits.data_ptr<float>(), nullptr, saved[1].data_ptr<int32_t>(),
@@ -259,13 +261,18 @@ struct DispatchTokens : public torch::autograd::Function<DispatchTokens> {
                        float(lbw), dl.data_ptr<float>(), cur_stream()),
                    "dispatch_tokens (backward)");
     }
-    return {dx, dl, {}, {}, {}, {}};
+    return {dx, dl, {}, {}, {}, {}, {}};
   }
 };
 
 std::vector<at::Tensor> dispatch_tokens(const at::Tensor& x, const at::Tensor& logits, int64_t k,
                                         int64_t capacity, double lbw, const OptTensor& err) {
-  return DispatchTokens::apply(x, logits, k, capacity, lbw, err);
+  std::vector<at::Tensor> all;
+  const auto out = DispatchTokens::apply(x, logits, k, capacity, lbw, err, &all);
+  all[1] = out[0];
+  all[5] = out[1];
+  all[6] = out[2];
+  return all;
 }
 
 // ---------------------------------------------------------------------------

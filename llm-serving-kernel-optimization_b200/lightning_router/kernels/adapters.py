@@ -70,6 +70,8 @@ def _no_grad(name: str, *tensors: torch.Tensor | None) -> None:
 
 def adapter_index(index: torch.Tensor) -> torch.Tensor:
     """Adapter numbers of any integer type as contiguous int32."""
+    if index.dtype == torch.int32 and index.dim() == 1 and index.is_contiguous():
+        return index
     if index.dtype.is_floating_point or index.dtype == torch.bool:
         raise ValueError(f"adapter numbers must be integers, got {index.dtype}")
     if index.dtype in (torch.int64, torch.uint32, torch.uint64):
