@@ -281,6 +281,10 @@ int lr_balanced_gating_backward(const float* logits, const uint8_t* token_mask,
                                 const float* d_aux, int T, int E, int k,
                                 float load_balance_weight, float* d_logits, lr_stream_t stream);
 
+/* dst[n] fp16 = src[n] fp32 rounded (an fp32 master weight for lr_gate_logits).
+ * n % 8 == 0, both 16-byte aligned.                                          */
+int lr_round_half(const float* src, void* dst, long long n, lr_stream_t stream);
+
 /* Gradients of lr_gate_logits: d_h[T,d] fp16 = d_logits . wg, d_wg[E,d] fp32 =
  * d_logits^T . h, d_bias[E] fp32 = column sums (each nullable; d_bias needs
  * d_wg).  d_logits[T,E] fp32 is not rounded.  Limits as lr_gate_logits; h, wg,

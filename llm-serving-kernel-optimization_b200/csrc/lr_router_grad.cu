@@ -751,6 +751,18 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// fp32 -> fp16, n values (a multiple of 8).
+__global__ void __launch_bounds__(256)
+    round_half_kernel(const float4* __restrict__ src, uint4* __restrict__ dst, long n8) {
+  pdl_wait();
+  pdl_trigger();
+  const long i = long(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n8) return;
+  const float4 a = src[2 * i], b = src[2 * i + 1];
+  const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  dst[i] = pack_half8(v);
+}
+
 struct GatePlan {
   int E8, chunks, groups, per_block, splits;
   size_t frag, down, colsum, wt, part, bytes;  // workspace offsets
@@ -972,6 +984,14 @@ extern "C" int lr_balanced_gating_backward(const float* logits, const uint8_t* t
          : E <= 16 ? run(balanced_gating_backward_kernel<2>)
          : E <= 32 ? run(balanced_gating_backward_kernel<4>)
                    : run(balanced_gating_backward_kernel<8>);
+}
+
+extern "C" int lr_round_half(const float* src, void* dst, long long n, lr_stream_t stream) {
+  if (n < 0 || n % 8 != 0) return LR_ERR_INVALID_ARGUMENT;
+  if (n == 0) return LR_OK;
+  if (!src || !dst || !aligned16(src) || !aligned16(dst)) return LR_ERR_INVALID_ARGUMENT;
+  return launch_pdl(round_half_kernel, dim3(unsigned((n / 8 + 255) / 256)), dim3(256), 0, stream,
+                    reinterpret_cast<const float4*>(src), static_cast<uint4*>(dst), long(n / 8));
 }
 
 extern "C" size_t lr_gate_backward_workspace_bytes(int num_tokens, int d_model, int num_experts) {

@@ -66,6 +66,14 @@ def test_gradient_arguments():
     assert lib.lr_dispatch_backward(N, N, 0, 2, 64, N, N) == 0
 
 
+def test_round_half_arguments():
+    lib = _ext.clib()
+    n = ctypes.c_longlong
+    assert lib.lr_round_half(P, P, n(12), N) == -1 and lib.lr_round_half(P, P, n(-8), N) == -1
+    assert lib.lr_round_half(ctypes.c_void_p(260), P, n(8), N) == -1
+    assert lib.lr_round_half(N, N, n(0), N) == 0
+
+
 def test_adapter_arguments():
     lib = _ext.clib()
     big = ctypes.c_size_t(1 << 20)

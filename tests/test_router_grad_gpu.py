@@ -283,6 +283,17 @@ def test_gate_projection_parts_and_empty():
     assert not wr.grad.any() and e.grad.shape == (0, 64)
 
 
+def test_gate_projection_rounds_the_master_weight_as_torch_does():
+    from lightning_router.kernels.routing_grad import gate_projection
+    g = _gen(6)
+    h = torch.eye(64, device=DEV).half()            # logits are the weight's columns
+    w = _randn(g, 9, 64) * torch.logspace(-9, 6, 64, device=DEV)   # subnormal to infinite in fp16
+    w[0, :4] = torch.tensor([1 + 2.0**-11, 1 + 3 * 2.0**-11, 65519.0, 65520.0], device=DEV)
+    w2 = torch.where(torch.isfinite(w.half()), w, 0.0)
+    assert torch.equal(gate_projection(h, w2), w2.half().float().t())
+    assert torch.equal(gate_projection(h, w2[:, ::1].half()), gate_projection(h, w2))
+
+
 def test_gate_projection_unaligned_and_strided_rows():
     from lightning_router.kernels.routing_grad import gate_projection
     g = _gen(4)
