@@ -191,12 +191,14 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     if (need_h) dh = at::empty({T, d}, h.options());
     if (need_w) dw = at::empty({E, d}, fopt);
     if (need_b) db = at::empty({E}, fopt);
-    auto ws = workspace(lr_gate_backward_workspace_bytes(int(T), int(d), int(E)), dl);
+    const size_t wsb = lr_gate_backward_workspace_bytes(int(T), int(d), int(E));
+    at::Tensor ws;
+    if (wsb) ws = workspace(wsb, dl);
     check_status(lr_gate_backward(h.data_ptr(), w.data_ptr(), dl.data_ptr<float>(), int(T), int(d),
                                   int(E), need_h ? dh.data_ptr() : nullptr,
                                   need_w ? dw.data_ptr<float>() : nullptr,
-                                  need_b ? db.data_ptr<float>() : nullptr, ws.data_ptr(),
-                                  size_t(ws.numel()), cur_stream()),
+                                  need_b ? db.data_ptr<float>() : nullptr,
+                                  wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
                  "gate_projection (backward)");
     if (need_h) dh = dh.to(at::ScalarType(saved_p[3]));
     if (need_w) dw = dw.to(at::ScalarType(saved_p[4]));

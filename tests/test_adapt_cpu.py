@@ -31,8 +31,8 @@ def test_workspace_sizes():
     assert f(1 << 24, 64) == f(1 << 20, 64)     # a bounded grid
     g = lib.lr_gate_backward_workspace_bytes
     # two fp16 terms per gradient, the transposed weight, partial sums once there are ranges
-    assert g(0, 4096, 8) == 0
-    assert g(128, 4096, 8) >= 128 * 8 * 4 + 4096 * 8 * 2
+    assert g(0, 4096, 8) == 0 and g(256, 4096, 64) == 0      # small batches need none
+    assert g(257, 4096, 8) >= 257 * 8 * 4 + 4096 * 8 * 2 and g(16, 4096, 65) > 0
     assert g(16384, 4096, 8) >= 16384 * 8 * 4 + 4096 * 8 * 2 + 2 * 4096 * 8 * 4
     h = lib.lr_adapter_workspace_bytes
     assert h(64, 16, 1) == 64 * 16 * 4 and h(64, 16, 2) == 2 * h(64, 16, 1) and h(0, 16, 1) == 0

@@ -232,7 +232,7 @@ def test_balanced_gating_gradient_of_a_balanced_router(T, E, k):
 # ---------------------------------------------------------------------------
 # gate projection
 # ---------------------------------------------------------------------------
-GATE = [(1, 16, 1), (3, 48, 5), (17, 64, 8), (64, 80, 9), (100, 1024, 4), (257, 208, 16),
+GATE = [(1, 16, 1), (3, 48, 5), (17, 64, 8), (64, 80, 9), (256, 496, 64), (100, 64, 70), (255, 4096, 7), (100, 1024, 4), (257, 208, 16),
         (1000, 512, 33), (4000, 1264, 24), (3001, 2000, 100), (2049, 256, 64), (5000, 2048, 8), (300, 64, 130), (6000, 1040, 64)]
 
 
