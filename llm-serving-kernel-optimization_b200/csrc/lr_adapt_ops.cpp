@@ -113,10 +113,10 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
     const double lbw = ctx->saved_data["lbw"].toDouble();
     if (!grads[0].defined() && !grads[1].defined()) return {{}, {}, {}, {}, {}};
     c10::cuda::CUDAGuard g(saved[0].device());
-    const at::Tensor logits = saved[0].detach().contiguous();
+    const at::Tensor logits = saved[0].is_contiguous() ? saved[0] : saved[0].detach().contiguous();
     const at::Tensor dw = grads[0].defined() ? grads[0].contiguous() : grads[0];
     const at::Tensor da = grads[1].defined() ? grads[1].contiguous() : grads[1];
-    auto dl = at::empty_like(logits);
+    auto dl = at::empty(logits.sizes(), logits.options());
     check_status(
         lr_balanced_gating_backward(
             logits.data_ptr<float>(),
@@ -156,7 +156,9 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     if (given(bias)) {
       check_same_device(*bias, h, "bias");
       TORCH_CHECK(bias->numel() == E, "bias: (E,)");
-      b = bias->detach().to(at::kFloat).contiguous();
+      b = *bias;
+      if (b.scalar_type() != at::kFloat || !b.is_contiguous())
+        b = b.detach().to(at::kFloat).contiguous();
     }
     auto out = at::empty({T, E}, h.options().dtype(at::kFloat));
     check_status(lr_gate_logits(hh.data_ptr(), wh.data_ptr(),
@@ -168,11 +170,16 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     // before the backward pass is noticed
     ctx->save_for_backward({hh.data_ptr() == h.data_ptr() ? h : hh,
                             wh.data_ptr() == w.data_ptr() ? w : wh});
-    ctx->saved_data["p"] = std::vector<int64_t>{
-        h.requires_grad(), w.requires_grad(), given(bias) && bias->requires_grad(),
-        int64_t(h.scalar_type()), int64_t(w.scalar_type()),
-        int64_t(given(bias) ? bias->scalar_type() : at::kFloat)};
-    if (given(bias)) ctx->saved_data["b_shape"] = bias->sizes().vec();
+    // what needs a gradient, and the types that differ from the kernels'
+    int64_t need = h.requires_grad() | w.requires_grad() << 1;
+    if (given(bias) && bias->requires_grad()) need |= 4;
+    ctx->saved_data["need"] = need;
+    if (h.scalar_type() != at::kHalf) ctx->saved_data["h_type"] = int64_t(h.scalar_type());
+    if (w.scalar_type() != at::kFloat) ctx->saved_data["w_type"] = int64_t(w.scalar_type());
+    if (need & 4 && (bias->scalar_type() != at::kFloat || bias->dim() != 1)) {
+      ctx->saved_data["b_type"] = int64_t(bias->scalar_type());
+      ctx->saved_data["b_shape"] = bias->sizes().vec();
+    }
     return out;
   }
 
@@ -180,15 +187,15 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     check_once("gate_projection");
     if (!grads[0].defined()) return {{}, {}, {}};
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor h = saved[0].detach(), w = saved[1].detach();
+    const at::Tensor &h = saved[0], &w = saved[1];
     c10::cuda::CUDAGuard g(h.device());
     const at::Tensor dl = grads[0].contiguous();
     const int64_t T = h.size(0), d = h.size(1), E = w.size(0);
-    const auto saved_p = ctx->saved_data["p"].toIntVector();
-    const bool need_h = saved_p[0], need_b = saved_p[2], need_w = saved_p[1] || need_b;
+    const int64_t need = ctx->saved_data["need"].toInt();
+    const bool need_h = need & 1, need_b = need & 4, need_w = need & 6;
     const auto fopt = dl.options();
     at::Tensor dh, dw, db;
-    if (need_h) dh = at::empty({T, d}, h.options());
+    if (need_h) dh = at::empty({T, d}, fopt.dtype(at::kHalf));
     if (need_w) dw = at::empty({E, d}, fopt);
     if (need_b) db = at::empty({E}, fopt);
     const size_t wsb = lr_gate_backward_workspace_bytes(int(T), int(d), int(E));
@@ -200,11 +207,16 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
                                   need_b ? db.data_ptr<float>() : nullptr,
                                   wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
                  "gate_projection (backward)");
-    if (need_h) dh = dh.to(at::ScalarType(saved_p[3]));
-    if (need_w) dw = dw.to(at::ScalarType(saved_p[4]));
-    if (need_b)
-      db = db.to(at::ScalarType(saved_p[5]))
-               .view(ctx->saved_data["b_shape"].toIntVector());
+    const auto cast = [&](at::Tensor& t, const char* key) {
+      const auto it = ctx->saved_data.find(key);
+      if (t.defined() && it != ctx->saved_data.end())
+        t = t.to(at::ScalarType(it->second.toInt()));
+    };
+    cast(dh, "h_type");
+    cast(dw, "w_type");
+    cast(db, "b_type");
+    if (const auto it = ctx->saved_data.find("b_shape"); it != ctx->saved_data.end())
+      db = db.view(it->second.toIntVector());
     return {dh, dw, db};
   }
 };
