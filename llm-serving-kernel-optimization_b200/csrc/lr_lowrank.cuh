@@ -394,6 +394,29 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     }
   };
   if (stream && warp == kProducer) produce(0, min(n_tiles, kTileStages));
+
+  // Small batches: the weights of groups [g0, g0 + S) for column group c.
+  constexpr int S = MT == 1 ? expand_ahead<RV, MODE>() : 1;
+  const int n_groups = MODE == kExpandProduct ? 1 : s.n;
+  RankTile<RV> wt[S][BANKS];
+  const auto group_weights = [&](int c, int g0) {
+    const int nr = c * 32 + (g >> 1) * 8;
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      const int ad = MODE == kExpandProduct ? 0
+                     : g0 + u < n_groups    ? s.adapter[s.first[g0 + u]]
+                                            : -1;
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk)
+        wt[u][bk].load(p.b[bk] + (size_t(max(ad, 0)) * p.N + nr + (g & 1)) * p.ldb +
+                           tq * RankTile<RV>::kPer,
+                       p.ldb, ad >= 0 && c < cg1 && nr < p.N, tq);
+    }
+  };
+  // The first ones are in flight while v is prepared where the registers allow it
+  // (64 rows, rank 16: 17.7 -> 16.8 us a pass; SwiGLU and rank 64 lose more to spills).
+  constexpr bool EARLY = MT == 1 && RV == 16 && MODE == kExpandAdd;
+  if (EARLY) group_weights(cg0 + warp, 0);
   {  // v: fp32 -> scaled (value, remainder) pairs in fragment order
     constexpr int LPR = kAdThreads / W;               // lanes of a row
     constexpr int EL = (RV / 2 + LPR - 1) / LPR;      // pairs of a lane
@@ -455,7 +478,6 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
       cp_async_wait_all();  // leave no copy behind
       return;
     }
-    const int n_groups = MODE == kExpandProduct ? 1 : s.n;
     float fac[2 * MT][BANKS];
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i)
@@ -581,8 +603,6 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   // Small batches: a warp takes its column groups for all 16 rows.  The window's
   // groups come S at a time, all their weights in flight; each is multiplied with
   // every row and kept for its own, so the base rows are finished once, by all lanes.
-  constexpr int S = expand_ahead<RV, MODE>();
-  const int n_groups = MODE == kExpandProduct ? 1 : s.n;
   int gid[2];
   bool none[2];
   float fac[2][BANKS];
@@ -612,20 +632,8 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[bk][j][i] = 0.f;
-    const int nr = c * 32 + (g >> 1) * 8;
     for (int g0 = 0; g0 < n_groups; g0 += S) {
-      RankTile<RV> wt[S][BANKS];
-#pragma unroll
-      for (int u = 0; u < S; ++u) {
-        const int ad = MODE == kExpandProduct ? 0
-                       : g0 + u < n_groups    ? s.adapter[s.first[g0 + u]]
-                                              : -1;
-#pragma unroll
-        for (int bk = 0; bk < BANKS; ++bk)
-          wt[u][bk].load(p.b[bk] + (size_t(max(ad, 0)) * p.N + nr + (g & 1)) * p.ldb +
-                             tq * RankTile<RV>::kPer,
-                         p.ldb, ad >= 0 && nr < p.N, tq);
-      }
+      if (!EARLY || g0 > 0 || c > cg0 + warp) group_weights(c, g0);
 #pragma unroll
       for (int u = 0; u < S; ++u) {
         if (g0 + u >= n_groups) break;
