@@ -71,7 +71,8 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
     TORCH_CHECK(logits_in.dim() == 2 && logits_in.scalar_type() == at::kFloat,
                 "logits: (T,E) fp32");
     c10::cuda::CUDAGuard g(logits_in.device());
-    const at::Tensor logits = logits_in.is_contiguous() ? logits_in : logits_in.detach().contiguous();
+    const at::Tensor logits =
+        logits_in.is_contiguous() ? logits_in : logits_in.detach().contiguous();
     const int64_t T = logits.size(0), E = logits.size(1);
     TORCH_CHECK(E >= 1 && E <= 64 && k >= 1 && k <= 8 && k <= E,
                 "balanced_gating: 1 <= E <= 64 and 1 <= k <= min(E, 8) expected, got E=", E,
@@ -87,16 +88,16 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
     auto gw = at::empty({T * k}, logits.options());
     auto stats = at::empty({E + 1}, logits.options().dtype(at::kInt));
     auto aux = at::empty({}, logits.options());
-    const size_t wsb = lr_balanced_gating_workspace_bytes(int(T), int(E));
+    const size_t wsb = lr_balanced_gating_workspace_bytes(as_int(T), as_int(E));
     at::Tensor ws;
     if (wsb) ws = workspace(wsb, logits);
     check_status(lr_balanced_gating(logits.data_ptr<float>(),
                                     mask.defined() ? static_cast<const uint8_t*>(mask.data_ptr())
                                                    : nullptr,
-                                    int(T), int(E), int(k), float(lbw), ids.data_ptr<int32_t>(),
-                                    gw.data_ptr<float>(), stats.data_ptr<int32_t>(),
-                                    aux.data_ptr<float>(), wsb ? ws.data_ptr() : nullptr, wsb,
-                                    cur_stream()),
+                                    as_int(T), as_int(E), as_int(k), float(lbw),
+                                    ids.data_ptr<int32_t>(), gw.data_ptr<float>(),
+                                    stats.data_ptr<int32_t>(), aux.data_ptr<float>(),
+                                    wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
                  "balanced_gating");
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({logits_in, mask, ids, stats});
@@ -123,8 +124,8 @@ struct BalancedGating : public torch::autograd::Function<BalancedGating> {
             saved[1].defined() ? static_cast<const uint8_t*>(saved[1].data_ptr()) : nullptr,
             saved[2].data_ptr<int32_t>(), saved[3].data_ptr<int32_t>(), 0,
             dw.defined() ? dw.data_ptr<float>() : nullptr,
-            da.defined() ? da.data_ptr<float>() : nullptr, int(logits.size(0)),
-            int(logits.size(1)), int(k), float(lbw), dl.data_ptr<float>(), cur_stream()),
+            da.defined() ? da.data_ptr<float>() : nullptr, as_int(logits.size(0)),
+            as_int(logits.size(1)), as_int(k), float(lbw), dl.data_ptr<float>(), cur_stream()),
         "balanced_gating (backward)");
     return {dl, {}, {}, {}, {}};
   }
@@ -162,8 +163,8 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     }
     auto out = at::empty({T, E}, h.options().dtype(at::kFloat));
     check_status(lr_gate_logits(hh.data_ptr(), wh.data_ptr(),
-                                b.defined() ? b.data_ptr<float>() : nullptr, int(T), int(d),
-                                int(E), out.data_ptr<float>(), cur_stream()),
+                                b.defined() ? b.data_ptr<float>() : nullptr, as_int(T), as_int(d),
+                                as_int(E), out.data_ptr<float>(), cur_stream()),
                  "gate_projection");
     ctx->set_materialize_grads(false);
     // an input that is used as it is goes in as the input, so that writing to it
@@ -198,11 +199,11 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     if (need_h) dh = at::empty({T, d}, fopt.dtype(at::kHalf));
     if (need_w) dw = at::empty({E, d}, fopt);
     if (need_b) db = at::empty({E}, fopt);
-    const size_t wsb = lr_gate_backward_workspace_bytes(int(T), int(d), int(E));
+    const size_t wsb = lr_gate_backward_workspace_bytes(as_int(T), as_int(d), as_int(E));
     at::Tensor ws;
     if (wsb) ws = workspace(wsb, dl);
-    check_status(lr_gate_backward(h.data_ptr(), w.data_ptr(), dl.data_ptr<float>(), int(T), int(d),
-                                  int(E), need_h ? dh.data_ptr() : nullptr,
+    check_status(lr_gate_backward(h.data_ptr(), w.data_ptr(), dl.data_ptr<float>(), as_int(T),
+                                  as_int(d), as_int(E), need_h ? dh.data_ptr() : nullptr,
                                   need_w ? dw.data_ptr<float>() : nullptr,
                                   need_b ? db.data_ptr<float>() : nullptr,
                                   wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
@@ -271,8 +272,8 @@ struct DispatchTokens : public torch::autograd::Function<DispatchTokens> {
     if (grads[2].defined()) {
       const at::Tensor dp = rows16(grads[2], at::kHalf);
       dx = at::empty({T, d}, dp.options());
-      check_status(lr_dispatch_backward(dp.data_ptr(), saved[3].data_ptr<int32_t>(), int(T), int(k),
-                                        int(d), dx.data_ptr(), cur_stream()),
+      check_status(lr_dispatch_backward(dp.data_ptr(), saved[3].data_ptr<int32_t>(), as_int(T),
+                                        as_int(k), as_int(d), dx.data_ptr(), cur_stream()),
                    "dispatch_tokens (backward)");
     }
     if (grads[0].defined() || grads[1].defined()) {
@@ -283,8 +284,8 @@ struct DispatchTokens : public torch::autograd::Function<DispatchTokens> {
                        logits.data_ptr<float>(), nullptr, saved[1].data_ptr<int32_t>(),
                        saved[2].data_ptr<int32_t>(), 1,
                        dw.defined() ? dw.data_ptr<float>() : nullptr,
-                       da.defined() ? da.data_ptr<float>() : nullptr, int(T), int(E), int(k),
-                       float(lbw), dl.data_ptr<float>(), cur_stream()),
+                       da.defined() ? da.data_ptr<float>() : nullptr, as_int(T), as_int(E),
+                       as_int(k), float(lbw), dl.data_ptr<float>(), cur_stream()),
                    "dispatch_tokens (backward)");
     }
     return {dx, dl, {}, {}, {}, {}, {}};
@@ -324,7 +325,7 @@ struct CombineTokens : public torch::autograd::Function<CombineTokens> {
     const int64_t T = S / k, d = y.size(1);
     auto out = at::empty({T, d}, yc.options());
     check_status(lr_combine(yc.data_ptr(), wc.data_ptr<float>(), slot_pos.data_ptr<int32_t>(),
-                            int(T), int(k), int(d), out.data_ptr(), cur_stream()),
+                            as_int(T), as_int(k), as_int(d), out.data_ptr(), cur_stream()),
                  "combine_tokens");
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({yc.data_ptr() == y.data_ptr() ? y : yc, w, slot_pos, offsets, kept});
@@ -345,8 +346,9 @@ struct CombineTokens : public torch::autograd::Function<CombineTokens> {
     auto dw = at::empty({S}, w.options());
     check_status(lr_combine_backward(dout.data_ptr(), y.data_ptr(), w.data_ptr<float>(),
                                      saved[2].data_ptr<int32_t>(), saved[3].data_ptr<int32_t>(),
-                                     saved[4].data_ptr<int32_t>(), int(S / k), int(k), int(d),
-                                     int(E), dy.data_ptr(), dw.data_ptr<float>(), cur_stream()),
+                                     saved[4].data_ptr<int32_t>(), as_int(S / k), as_int(k),
+                                     as_int(d), as_int(E), dy.data_ptr(), dw.data_ptr<float>(),
+                                     cur_stream()),
                  "combine_tokens (backward)");
     return {dy, dw.view(w.sizes()), {}, {}, {}, {}};
   }
@@ -435,11 +437,11 @@ at::Tensor adapter_add(const at::Tensor& x_in, const at::Tensor& index, const at
   const at::Tensor x = rows16(x_in, at::kHalf), base = rows16(base_in, at::kHalf);
   at::Tensor out = result_rows(out_in, x, k.N, {base});
   const int64_t R = x.size(0);
-  auto ws = workspace(lr_adapter_workspace_bytes(int(R), int(k.r), 1), x);
-  check_status(lr_adapter_add(x.data_ptr(), int(R), int(k.K), index.data_ptr<int32_t>(), int(k.n),
-                              k.a, k.b, k.scale, int(k.r), int(k.N), base.data_ptr(),
-                              out.data_ptr(), ws.data_ptr(), size_t(ws.numel()), err_ptr(err),
-                              cur_stream()),
+  auto ws = workspace(lr_adapter_workspace_bytes(as_int(R), as_int(k.r), 1), x);
+  check_status(lr_adapter_add(x.data_ptr(), as_int(R), as_int(k.K), index.data_ptr<int32_t>(),
+                              as_int(k.n), k.a, k.b, k.scale, as_int(k.r), as_int(k.N),
+                              base.data_ptr(), out.data_ptr(), ws.data_ptr(), size_t(ws.numel()),
+                              err_ptr(err), cur_stream()),
                "adapter_add");
   return out;
 }
@@ -461,11 +463,12 @@ at::Tensor adapter_swiglu(const at::Tensor& x_in, const at::Tensor& index, const
                    up = rows16(up_in, at::kHalf);
   at::Tensor out = result_rows(out_in, x, kg.N, {gate, up});
   const int64_t R = x.size(0);
-  auto ws = workspace(lr_adapter_workspace_bytes(int(R), int(kg.r), 2), x);
-  check_status(lr_adapter_swiglu(x.data_ptr(), int(R), int(kg.K), index.data_ptr<int32_t>(),
-                                 int(kg.n), kg.a, kg.b, kg.scale, ku.a, ku.b, ku.scale, int(kg.r),
-                                 int(kg.N), gate.data_ptr(), up.data_ptr(), out.data_ptr(),
-                                 ws.data_ptr(), size_t(ws.numel()), err_ptr(err), cur_stream()),
+  auto ws = workspace(lr_adapter_workspace_bytes(as_int(R), as_int(kg.r), 2), x);
+  check_status(lr_adapter_swiglu(x.data_ptr(), as_int(R), as_int(kg.K), index.data_ptr<int32_t>(),
+                                 as_int(kg.n), kg.a, kg.b, kg.scale, ku.a, ku.b, ku.scale,
+                                 as_int(kg.r), as_int(kg.N), gate.data_ptr(), up.data_ptr(),
+                                 out.data_ptr(), ws.data_ptr(), size_t(ws.numel()), err_ptr(err),
+                                 cur_stream()),
                "adapter_swiglu");
   return out;
 }
@@ -481,10 +484,10 @@ at::Tensor adapter_rows(const at::Tensor& adapter_ids, const at::Tensor& source_
   check_int32(offsets, adapter_ids, E + 1, "offsets");
   c10::cuda::CUDAGuard g(adapter_ids.device());
   auto index = at::empty({S}, adapter_ids.options());
-  check_status(lr_adapter_rows(adapter_ids.data_ptr<int32_t>(), int(adapter_ids.numel()),
-                               int(num_adapters), source_idx.data_ptr<int32_t>(),
-                               offsets.data_ptr<int32_t>(), kept.data_ptr<int32_t>(), int(S),
-                               int(E), index.data_ptr<int32_t>(), err_ptr(err), cur_stream()),
+  check_status(lr_adapter_rows(adapter_ids.data_ptr<int32_t>(), as_int(adapter_ids.numel()),
+                               as_int(num_adapters), source_idx.data_ptr<int32_t>(),
+                               offsets.data_ptr<int32_t>(), kept.data_ptr<int32_t>(), as_int(S),
+                               as_int(E), index.data_ptr<int32_t>(), err_ptr(err), cur_stream()),
                "adapter_rows");
   return index;
 }

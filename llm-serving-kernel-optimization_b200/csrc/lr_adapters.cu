@@ -444,8 +444,8 @@ static int run_shrink(const ShrinkArgs& p, int banks, cudaStream_t stream) {
 
 static int check_adapter_args(const void* x, long R, int K, const int32_t* index, int n, int r,
                               int N) {
-  if (R < 0 || R > 0x7fffffffL || K <= 0 || K % 8 != 0 || N <= 0 || N % 8 != 0 || n < 1 || r < 8 ||
-      r > kMaxRank || r % 8 != 0)
+  if (R < 0 || R > kMaxRows || K <= 0 || K % 8 != 0 || K > kMaxColumns || N <= 0 || N % 8 != 0 ||
+      N > kMaxColumns || n < 1 || r < 8 || r > kMaxRank || r % 8 != 0)
     return LR_ERR_INVALID_ARGUMENT;
   if (R > 0 && (!x || !index || !aligned16(x))) return LR_ERR_INVALID_ARGUMENT;
   return LR_OK;
@@ -512,7 +512,8 @@ extern "C" int lr_adapter_rows(const int32_t* adapter_ids, int T, int num_adapte
                                const int32_t* source_idx, const int32_t* offsets,
                                const int32_t* kept_counts, int S, int E, int32_t* index,
                                int32_t* err, lr_stream_t stream) {
-  if (T < 0 || S < 0 || E < 1 || num_adapters < 1 || long(num_adapters) * E > 0x7fffffffL)
+  if (T < 0 || S < 0 || S > kMaxRows || E < 1 || num_adapters < 1 ||
+      long(num_adapters) * E > 0x7fffffffL)
     return LR_ERR_INVALID_ARGUMENT;
   if (S == 0) return LR_OK;
   if (!adapter_ids || !source_idx || !offsets || !kept_counts || !index)

@@ -174,6 +174,9 @@ LR_DEVICE int warps_per_group(int g) { return g <= 1 ? 8 : g <= 2 ? 4 : g <= 4 ?
 // round) and the power cap's clock keep it from the rest.  64 rows x 14336 with 64
 // adapters of rank 16: 11 us (33 MB, floor 5).  128 rows of 64 SwiGLU adapter pairs:
 // 20 us (70 MB, floor 11).
+// Largest sizes taken: row numbers plus a tile, and 64 rows' offsets, stay in 32 bits.
+constexpr int kMaxRows = 0x7fffffff - 1023;
+constexpr int kMaxColumns = 1 << 26;
 constexpr uint64_t kCopyWaitNs = 1000000000ull;  // bound of every wait for a copy
 
 enum ExpandMode : int {
@@ -667,6 +670,7 @@ constexpr long kTargetBlocks = 148;
 
 template <int RV, int MT, int MODE>
 static int launch_expand(ExpandArgs p, cudaStream_t stream) {
+  if (p.R > kMaxRows || p.N > kMaxColumns) return LR_ERR_INVALID_ARGUMENT;
   constexpr int W = 16 * MT;
   constexpr int smem = expand_smem_bytes<RV, MT, MODE>();
   auto kern = expand_kernel<RV, MT, MODE>;

@@ -23,6 +23,12 @@ inline void check_cuda(const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
 }
 
+// A size as the C interface's int.
+inline int as_int(int64_t n) {
+  TORCH_CHECK(n >= 0 && n <= 0x7fffffff, "lightning_router: a size of ", n, " is out of range");
+  return static_cast<int>(n);
+}
+
 inline int32_t* err_ptr(const c10::optional<at::Tensor>& err) {
   if (!err.has_value() || !err->defined()) return nullptr;
   TORCH_CHECK(err->is_cuda() && err->scalar_type() == at::kInt && err->numel() >= 1,

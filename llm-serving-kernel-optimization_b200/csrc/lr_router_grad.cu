@@ -1004,7 +1004,7 @@ __global__ void __launch_bounds__(256)
 using namespace lr;
 
 static bool gating_args_ok(int T, int E, int k) {
-  return T >= 0 && E >= 1 && E <= 64 && k >= 1 && k <= kMaxTopK && k <= E;
+  return T >= 0 && T <= kMaxRows && E >= 1 && E <= 64 && k >= 1 && k <= kMaxTopK && k <= E;
 }
 
 extern "C" size_t lr_balanced_gating_workspace_bytes(int num_tokens, int num_experts) {
@@ -1089,7 +1089,9 @@ extern "C" size_t lr_gate_backward_workspace_bytes(int num_tokens, int d_model, 
 extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d,
                                 int E, void* d_h, float* d_wg, float* d_bias, void* workspace,
                                 size_t workspace_bytes, lr_stream_t stream) {
-  if (T < 0 || d <= 0 || d % 16 != 0 || E < 1 || E > 256) return LR_ERR_INVALID_ARGUMENT;
+  if (T < 0 || T > kMaxRows || d <= 0 || d % 16 != 0 || d > kMaxColumns || E < 1 ||
+      E > 256)
+    return LR_ERR_INVALID_ARGUMENT;
   if (d_bias && !d_wg) return LR_ERR_INVALID_ARGUMENT;
   if (T == 0) {
     if (d_wg) LR_CUDA_TRY(cudaMemsetAsync(d_wg, 0, size_t(E) * d * sizeof(float), stream));
@@ -1177,7 +1179,7 @@ extern "C" int lr_combine_backward(const void* d_out, const void* y, const float
                                    const int32_t* slot_pos, const int32_t* offsets,
                                    const int32_t* kept_counts, int T, int k, int d, int E,
                                    void* d_y, float* d_weights, lr_stream_t stream) {
-  if (T < 0 || k < 1 || k > kMaxTopK || d <= 0 || d % 8 != 0 || E < 1)
+  if (T < 0 || k < 1 || k > kMaxTopK || long(T) * k > kMaxRows || d <= 0 || d % 8 != 0 || E < 1)
     return LR_ERR_INVALID_ARGUMENT;
   if (T == 0) return LR_OK;
   if (!d_out || !y || !gate_weights || !slot_pos || !offsets || !kept_counts || !d_y || !d_weights)

@@ -284,7 +284,8 @@ static int launch_gate_tiled(const __half* h, const __half* wg, const float* bia
   auto kern = gate_logits_tiled_kernel<MTL, NT>;
   static unsigned long long configured = 0;
   if (const int rc = set_dyn_smem_once(kern, smem, configured)) return rc;
-  kern<<<dim3(unsigned((T + TM - 1) / TM), (E + EM - 1) / EM), kGateWarps * 32, smem, stream>>>(
+  const dim3 grid(unsigned((long(T) + TM - 1) / TM), (E + EM - 1) / EM);
+  kern<<<grid, kGateWarps * 32, smem, stream>>>(
       h, wg, bias, T, d, E, logits);
   LR_LAUNCH_CHECK();
   return LR_OK;
@@ -1604,7 +1605,8 @@ extern "C" int lr_combine(const void* y, const float* gate_weights, const int32_
 
 extern "C" int lr_dispatch_backward(const void* d_permuted, const int32_t* slot_pos, int T, int k,
                                     int d, void* d_x, lr_stream_t stream) {
-  if (T < 0 || k < 1 || k > kMaxTopK || d <= 0 || d % 8 != 0) return LR_ERR_INVALID_ARGUMENT;
+  if (T < 0 || k < 1 || k > kMaxTopK || long(T) * k > 0x7fffffffL || d <= 0 || d % 8 != 0)
+    return LR_ERR_INVALID_ARGUMENT;
   if (T == 0) return LR_OK;
   if (!d_permuted || !slot_pos || !d_x || !aligned16(d_permuted) || !aligned16(d_x))
     return LR_ERR_INVALID_ARGUMENT;

@@ -93,6 +93,37 @@ def test_adapter_arguments():
     assert lib.lr_adapter_rows(P, 4, 1 << 30, P, P, P, 8, 4, P, N, N) == -1
 
 
+def test_sizes_past_32_bit_offsets_are_refused():
+    lib = _ext.clib()
+    lbw, ws, big = ctypes.c_float(0.01), ctypes.c_size_t(0), ctypes.c_size_t(1 << 62)
+    top = 2**31 - 1
+    assert lib.lr_balanced_gating(P, N, top, 8, 2, lbw, P, P, P, P, P, big, N) == -1
+    assert lib.lr_balanced_gating_backward(P, N, P, P, 0, P, P, top, 8, 2, lbw, P, N) == -1
+    assert lib.lr_gate_backward(P, P, P, top, 64, 8, P, P, N, P, big, N) == -1
+    assert lib.lr_gate_backward(P, P, P, 4, (1 << 26) + 16, 8, P, P, N, N, ws, N) == -1
+    assert lib.lr_dispatch_backward(P, P, 1 << 29, 4, 64, P, N) == -1
+    assert lib.lr_combine_backward(P, P, P, P, P, P, 1 << 29, 4, 64, 8, P, P, N) == -1
+    for R, K, F in [(top, 64, 64), (64, (1 << 26) + 8, 64), (64, 64, (1 << 26) + 8)]:
+        assert lib.lr_adapter_add(P, R, K, P, 2, P, P, N, 8, F, P, P, P, big, N, N) == -1
+    assert lib.lr_adapter_rows(P, 4, 2, P, P, P, top, 4, P, N, N) == -1
+
+
+def test_adapters_of_another_layer_are_refused():
+    from lightning_router.models.adapters import ExpertAdapters
+    from lightning_router.models.experts import ExpertGroup
+    swiglu = ExpertGroup(4, 64, 128, quantized=True, group_size=64)
+    silu = ExpertGroup(4, 64, 128, quantized=True, group_size=64, activation="silu")
+    ExpertAdapters(2, 4, 64, 128, 8).check(swiglu)
+    ExpertAdapters(2, 4, 64, 128, 8, gated=False).check(silu)
+    for other, experts in [(ExpertAdapters(2, 8, 64, 128, 8), swiglu),
+                           (ExpertAdapters(2, 4, 128, 128, 8), swiglu),
+                           (ExpertAdapters(2, 4, 64, 64, 8), swiglu),
+                           (ExpertAdapters(2, 4, 64, 128, 8, gated=False), swiglu),
+                           (ExpertAdapters(2, 4, 64, 128, 8), silu)]:
+        with pytest.raises(RuntimeError, match="adapters for"):
+            other.check(experts)
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros(4, 16)
     with pytest.raises(RuntimeError, match="CUDA"):
