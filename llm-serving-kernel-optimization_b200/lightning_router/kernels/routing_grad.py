@@ -77,7 +77,7 @@ def gate_projection(hidden: torch.Tensor, gate_weight: torch.Tensor,
 def dispatch_tokens(x: torch.Tensor, logits: torch.Tensor, top_k: int,
                     capacity_factor: float = 1.25, load_balance_weight: float = 0.01,
                     capacity: int | None = None) -> DispatchPlan:
-    """:func:`topk_gating_dispatch` with gradients; rows of dropped slots are zero."""
+    """:func:`topk_gating_dispatch` with gradients (T >= 1); rows of dropped slots are zero."""
     _ext.require_cuda(x, logits)
     T, E = logits.shape
     C = expert_capacity(T * top_k, E, capacity_factor) if capacity is None else int(capacity)

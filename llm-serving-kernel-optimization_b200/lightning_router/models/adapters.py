@@ -28,7 +28,7 @@ class ExpertAdapters(nn.Module):
         if num_adapters < 1 or num_experts < 1:
             raise ValueError("at least one adapter and one expert")
         self.num_adapters, self.num_experts, self.rank = num_adapters, num_experts, rank
-        self.gated = gated
+        self.hidden_size, self.intermediate_size, self.gated = hidden_size, intermediate_size, gated
         for m in self.mats:
             K, N = (intermediate_size, hidden_size) if m == "down" else (hidden_size,
                                                                          intermediate_size)
@@ -41,6 +41,15 @@ class ExpertAdapters(nn.Module):
     @property
     def mats(self) -> tuple[str, ...]:
         return _MATS if self.gated else _MATS[1:]
+
+    def check(self, experts) -> None:
+        """Refuses the experts (:class:`ExpertGroup`) that these adapters were not made for."""
+        mine = (self.num_experts, self.hidden_size, self.intermediate_size, self.gated)
+        gated = experts.activation == "swiglu"
+        theirs = (experts.num_experts, experts.hidden_size, experts.intermediate_size, gated)
+        if mine != theirs:
+            raise RuntimeError("adapters for (experts, hidden size, intermediate size, gated) "
+                               f"{mine}, the layer has {theirs}")
 
     @torch.no_grad()
     def load(self, adapter: int, expert: int, mat: str, A: torch.Tensor, B: torch.Tensor,

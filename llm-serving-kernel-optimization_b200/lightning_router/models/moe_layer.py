@@ -113,10 +113,12 @@ class MoELayer(nn.Module):
                 raise RuntimeError("adapter_ids given, but layer.adapters is not set")
             if not self.experts.quantized:
                 raise RuntimeError("adapters are served beside INT4 experts only")
-            index = adapter_rows(adapter_ids, plan, self.adapters.num_adapters)
-            return self.experts.forward_segments_adapted(
-                plan.permuted, plan.offsets[:-1], plan.kept_counts, plan.capacity, self.adapters,
-                index, mark=self._mark)
+            self.adapters.check(self.experts)
+            with torch.no_grad():   # as without adapters, the experts build no graph
+                index = adapter_rows(adapter_ids, plan, self.adapters.num_adapters)
+                return self.experts.forward_segments_adapted(
+                    plan.permuted, plan.offsets[:-1], plan.kept_counts, plan.capacity,
+                    self.adapters, index, mark=self._mark)
         if self.experts.quantized:
             seg_start = plan.offsets[:-1]
             return self.experts.forward_segments(plan.permuted, seg_start, plan.kept_counts,

@@ -28,8 +28,9 @@ logger = logging.getLogger(__name__)
 
 class _Graph:
     def __init__(self, graph: torch.cuda.CUDAGraph, x: torch.Tensor, out: torch.Tensor,
-                 aux: torch.Tensor, ids: torch.Tensor | None = None):
-        self.graph, self.x, self.out, self.aux, self.ids = graph, x, out, aux, ids
+                 aux: torch.Tensor, ids: torch.Tensor | None = None, adapters=None):
+        self.graph, self.x, self.out, self.aux = graph, x, out, aux
+        self.ids, self.adapters = ids, adapters   # the adapters that the graph reads
 
 
 class LightningModelRunner:
@@ -98,7 +99,7 @@ class LightningModelRunner:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, pool=self._pool):
             out, aux = layer(x, adapter_ids=ids)
-        self._graphs[key] = _Graph(g, x, out, aux, ids)
+        self._graphs[key] = _Graph(g, x, out, aux, ids, layer.adapters if adapters else None)
 
     @torch.inference_mode()
     def execute_model(self, input_ids: torch.Tensor | None,
@@ -112,6 +113,8 @@ class LightningModelRunner:
         h = hidden_states.reshape(-1, shape[-1])
         key = (h.shape[0], h.shape[1])
         gr = self._graphs.get(key if adapter_ids is None else (*key, True))
+        if gr is not None and gr.ids is not None and gr.adapters is not layer.adapters:
+            gr = None   # captured with adapters that the layer no longer has
         if gr is None:
             out, _ = layer(h, adapter_ids=adapter_ids)
             return out.view(shape).to(hidden_states.dtype)

@@ -168,6 +168,37 @@ def test_runner_serves_adapters():
     assert torch.equal(wk.execute_model(None, x, adapter_ids=ids), ref)
 
 
+def test_adapters_exchanged_behind_a_captured_graph():
+    from lightning_router.serving.model_runner import LightningModelRunner
+    from lightning_router.workloads import build_layer
+    w = _workload(tokens=16, d_model=256, d_ff=512)
+    layer, t = build_layer(w, device=DEV)
+    r = LightningModelRunner(dict(hidden_size=256, intermediate_size=512),
+                             dict(num_experts=8, num_experts_per_token=2), dict(group_size=128),
+                             {}, device="cuda:0")
+    r.load_model()
+    r.moe_layer.load_state_dict(layer.state_dict())
+    r.set_adapters(_adapters(layer, 4, 8, 6))
+    r.capture(16, adapters=True)
+    ids = torch.arange(16, device=DEV, dtype=torch.int32) % 4
+    x = torch.randn(16, 256, device=DEV).half()
+    old = r.execute_model(None, x, adapter_ids=ids)
+    r.moe_layer.adapters = _adapters(layer, 4, 8, 7)      # not through set_adapters
+    ref, _ = r.moe_layer(x, adapter_ids=ids)
+    assert torch.equal(r.execute_model(None, x, adapter_ids=ids), ref)
+    assert not torch.equal(old, ref)
+
+
+def test_serving_with_adapters_takes_states_that_require_a_gradient():
+    from lightning_router.workloads import build_layer
+    layer, t = build_layer(_workload(tokens=16, d_model=256, d_ff=256), device=DEV)
+    layer.adapters = _adapters(layer, 2, 8, 3)
+    ids = torch.zeros(16, dtype=torch.int32, device=DEV)
+    want, _ = layer(t.x, adapter_ids=ids)
+    got, _ = layer(t.x.clone().requires_grad_(), adapter_ids=ids)
+    assert torch.equal(got, want)
+
+
 # ---------------------------------------------------------------------------
 # training
 # ---------------------------------------------------------------------------
