@@ -117,7 +117,7 @@ LR_DEVICE void group_rows(Groups& s, const int32_t* __restrict__ index, long row
     const int t = u * 32 + lane;
     a[u] = -2;
     if (t < W && row0 + t < R) {
-      a[u] = __ldg(index + row0 + t);
+      a[u] = __ldcg(index + row0 + t);
       if (a[u] < -1 || a[u] >= n) {
         report(err, LR_DEVERR_BAD_ADAPTER);
         a[u] = -1;
@@ -353,8 +353,13 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   __shared__ int s_abort;
   __shared__ Groups s;
   __shared__ float s_fac[BANKS][W];
-  pdl_wait();
-  pdl_trigger();
+  // Only v comes from the launch before (shrink, which lets this one start after its
+  // own wait): index, base rows and weights are read ahead of that launch's end.
+  // A product's weights are its predecessor's, too.
+  if (MODE == kExpandProduct) {
+    pdl_wait();
+    pdl_trigger();
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   const long row0 = long(blockIdx.x) * W;
   const int nrows = int(min(long(W), p.R - row0));
@@ -420,6 +425,10 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   // (64 rows, rank 16: 17.7 -> 16.8 us a pass; SwiGLU and rank 64 lose more to spills).
   constexpr bool EARLY = MT == 1 && RV == 16 && MODE == kExpandAdd;
   if (EARLY) group_weights(cg0 + warp, 0);
+  if (MODE != kExpandProduct) {
+    pdl_wait();
+    pdl_trigger();
+  }
   {  // v: fp32 -> scaled (value, remainder) pairs in fragment order
     constexpr int LPR = kAdThreads / W;               // lanes of a row
     constexpr int EL = (RV / 2 + LPR - 1) / LPR;      // pairs of a lane
