@@ -394,8 +394,6 @@ static int launch_cluster(void (*kern)(KArgs...), dim3 grid, unsigned cluster, s
   return 0;
 }
 
-constexpr long kSmallRows = 256;  // up to here windows of 8 (shrink) and 16 rows (expand)
-
 // Blocks are made to fill one wave of two per SM: K is split over a cluster, and a
 // small batch's window over blocks of its groups.
 template <int RB>

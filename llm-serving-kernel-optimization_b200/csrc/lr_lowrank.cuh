@@ -61,6 +61,15 @@ LR_DEVICE uint4 ld_row(const uint4* p) {
   return v;
 }
 
+LR_DEVICE uint2 ld_row8(const __half* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];"
+               : "=r"(v.x), "=r"(v.y)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // Read-only loads that stay where they are issued (ahead of their use).
 LR_DEVICE uint4 ld_ahead16(const void* p) {
   uint4 v;
@@ -171,9 +180,7 @@ LR_DEVICE int warps_per_group(int g) { return g <= 1 ? 8 : g <= 2 ? 4 : g <= 4 ?
 // and one store each.
 // 16384 x 14336, rank 32: 182 us, 5.2 TB/s of base in and out (floor 143); the
 // instructions around 16 rows x 32 columns (16 of them mma, 44 to convert, add,
-// round) and the power cap's clock keep it from the rest.  64 rows x 14336 with 64
-// adapters of rank 16: 11 us (33 MB, floor 5).  128 rows of 64 SwiGLU adapter pairs:
-// 20 us (70 MB, floor 11).
+// round) and the power cap's clock keep it from the rest.
 // Largest sizes taken: row numbers plus a tile, and 64 rows' offsets, stay in 32 bits.
 constexpr int kMaxRows = 0x7fffffff - 1023;
 constexpr int kMaxColumns = 1 << 26;
@@ -210,13 +217,15 @@ struct RankTile {
   uint32_t w[kSteps][4][2];
 
   // Columns n0 + (g >> 1) * 8 + 2 j + (g & 1); bp points at (that column for j = 0, tq * kPer).
+  // With a distance of 1: columns n0 + 4 g + j.
+  template <int DISTANCE = 2>
   LR_DEVICE void load(const __half* __restrict__ bp, int ldb, bool ok, int tq) {
 #pragma unroll
     for (int b = 0; b < kLoads; ++b)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const bool in = ok && b * 32 + tq * kPer < ldb;
-        const __half* q = bp + (unsigned(2 * j) * unsigned(ldb) + b * 32);
+        const __half* q = bp + (unsigned(DISTANCE * j) * unsigned(ldb) + b * 32);
         if (RV == 16) {
           uint2 v = make_uint2(0, 0);
           if (in) v = ld_ahead8(q);
@@ -253,6 +262,28 @@ struct RankTile {
       for (int j = 0; j < 4; ++j) mma_f16(acc[j], a.x, a.y, a.z, a.w, w[t][j][0], w[t][j][1]);
     }
   }
+
+  // The weights as the A operand (32 columns) and 8 rows' terms as B: `v` holds
+  // [step][lane] of (value, value, remainder, remainder).
+  LR_DEVICE void multiply_rows(float (&acc)[2][4], const uint4* v) const {
+#pragma unroll
+    for (int t = 0; t < kSteps; ++t) {
+      const uint4 q = v[t * 32];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (t == 0)
+          mma_f16_first(acc[i], w[t][2 * i][0], w[t][2 * i + 1][0], w[t][2 * i][1],
+                        w[t][2 * i + 1][1], q.x, q.y);
+        else
+          mma_f16(acc[i], w[t][2 * i][0], w[t][2 * i + 1][0], w[t][2 * i][1],
+                  w[t][2 * i + 1][1], q.x, q.y);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        mma_f16(acc[i], w[t][2 * i][0], w[t][2 * i + 1][0], w[t][2 * i][1], w[t][2 * i + 1][1],
+                q.z, q.w);
+    }
+  }
 };
 
 // Place of rank values (c, c + 1), c even, of row t among a window's fragments
@@ -274,11 +305,10 @@ LR_DEVICE int fragment_word(int t, int c) {
   return ((m * (RV / 16) + step) * 32 + g * 4 + tq) * 4 + kh * 2 + h;
 }
 
-// Small batches: groups of a window whose weights are in flight together.
+// Windows of 16 rows: groups whose weights are in flight together.
 template <int RV, int MODE>
 constexpr int expand_ahead() {
   // as many as 64 registers hold; SwiGLU's two banks leave room for half of that
-  // (128 rows, rank 16, N 14336: 31 us a pass with 2 groups, 37 with 4)
   return MODE == kExpandSwiglu ? (RV == 16 ? 2 : 1) : RV <= 64 ? 128 / RV : 1;
 }
 
@@ -403,7 +433,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   };
   if (stream && warp == kProducer) produce(0, min(n_tiles, kTileStages));
 
-  // Small batches: the weights of groups [g0, g0 + S) for column group c.
+  // Windows of 16 rows: the weights of groups [g0, g0 + S) for column group c.
   constexpr int S = MT == 1 ? expand_ahead<RV, MODE>() : 1;
   const int n_groups = MODE == kExpandProduct ? 1 : s.n;
   RankTile<RV> wt[S][BANKS];
@@ -422,7 +452,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     }
   };
   // The first ones are in flight while v is prepared where the registers allow it
-  // (64 rows, rank 16: 17.7 -> 16.8 us a pass; SwiGLU and rank 64 lose more to spills).
+  // (SwiGLU and rank 64 lose more to spills).
   constexpr bool EARLY = MT == 1 && RV == 16 && MODE == kExpandAdd;
   if (EARLY) group_weights(cg0 + warp, 0);
   if (MODE != kExpandProduct) {
@@ -612,7 +642,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     return;
   }
 
-  // Small batches: a warp takes its column groups for all 16 rows.  The window's
+  // Windows of 16 rows: a warp takes its column groups for all of them.  The window's
   // groups come S at a time, all their weights in flight; each is multiplied with
   // every row and kept for its own, so the base rows are finished once, by all lanes.
   int gid[2];
@@ -672,6 +702,198 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   }
 }
 
+// Up to 256 rows: windows of 8 rows.  A block's (request, column group) pairs are
+// split evenly over its warps in that order, so a warp streams one adapter's columns
+// (or two's), the weights and base rows of the next S column groups in flight.  The
+// weights are the A operand (16 columns a tile), the window's rows B: half the
+// products of a tile of 16 rows, of which a request has one or two; rows of other
+// requests are multiplied too and not stored.  A lane ends with 4 neighbouring
+// columns of rows 2 tq and 2 tq + 1.  Against 16-row tiles with every group in
+// every warp, a pass with shrink: 64 rows of 64 adapters of rank 16, N 14336, 15.5
+// us (15.9), of rank 32 21.6 (27); 128 expert rows of SwiGLU pairs 31.5 (32.2), in
+// neighbouring pairs 25.3 (27.2); one token, 4096 x 4096, rank 64, 7.5 (8.6).
+// Powers of two of warps to a group left warps idle: 33.7 for the expert rows.
+// Column groups in flight: twice as many spill registers, half as many leave the
+// memory idle (decode batch 20 and 16.5 us against 15).
+template <int RV, int MODE>
+constexpr int expand_rows_ahead() {
+  constexpr int n = (MODE == kExpandSwiglu ? 32 : 64) / RV;
+  return n > 0 ? n : 1;
+}
+
+template <int RV, int MODE>
+constexpr int expand_rows_min_blocks() {
+  return RV <= (MODE == kExpandSwiglu ? 32 : 64) ? 2 : 1;
+}
+
+template <int RV, int MODE>
+__global__ void __launch_bounds__(kAdThreads, expand_rows_min_blocks<RV, MODE>())
+    expand_rows_kernel(ExpandArgs p) {
+  constexpr int W = 8, BANKS = MODE == kExpandSwiglu ? 2 : 1;
+  constexpr int S = expand_rows_ahead<RV, MODE>();
+  __shared__ uint4 s_v[BANKS][RV / 16][32];
+  __shared__ float s_fac[BANKS][W];
+  __shared__ Groups s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const long row0 = long(blockIdx.x) * W;
+  const int cg0 = blockIdx.y * p.groups_per_chunk;
+  const int cg1 = min(cg0 + p.groups_per_chunk, (p.N + 31) / 32);
+  // as in expand_kernel: only v comes from the launch before
+  if (warp == 0) group_rows<W>(s, p.index, row0, p.R, p.n, !p.in_place, nullptr);
+  __syncthreads();
+  // (group, column group) items in order, an eighth of them to each warp: a warp
+  // streams the columns of one or two groups
+  const int cols = cg1 - cg0;
+  const int first = s.n * cols * warp / kAdWarps, last = s.n * cols * (warp + 1) / kAdWarps;
+  RankTile<RV> wt[S][BANKS];
+  uint2 bs[S][BANKS][2];
+  const size_t row_off = size_t(row0 + 2 * tq) * p.N + 4 * g;
+  int left = last - first;                       // items to load
+  int lgrp = first / cols, lc = cg0 + first % cols;  // the next one
+  int lad = -1;
+  bool lmine[2] = {false, false};
+  const __half* wp[BANKS];
+  const __half* bp[BANKS];
+#pragma unroll
+  for (int bk = 0; bk < BANKS; ++bk) bp[bk] = p.base[bk] + row_off + lc * 32;
+  const auto enter = [&]() {
+    if (left > 0) {
+      lad = s.adapter[s.first[lgrp]];
+      lmine[0] = s.group[2 * tq] == lgrp;
+      lmine[1] = s.group[2 * tq + 1] == lgrp;
+    }
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk)
+      wp[bk] = p.b[bk] + (size_t(max(lad, 0)) * p.N + lc * 32 + 4 * g) * p.ldb +
+               tq * RankTile<RV>::kPer;
+  };
+  enter();
+  const unsigned wstep = 32u * unsigned(p.ldb);
+  const auto load = [&](RankTile<RV>(&w)[BANKS], uint2(&base)[BANKS][2]) {
+    const bool in = left > 0 && lc * 32 + 4 * g < p.N;
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk) {
+      w[bk].template load<1>(wp[bk], p.ldb, in && lad >= 0, tq);
+      wp[bk] += wstep;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (in && lmine[h]) base[bk][h] = ld_row8(bp[bk] + h * size_t(p.N));
+      bp[bk] += 32;
+    }
+    --left;
+    if (++lc == cg1) {
+      lc = cg0;
+      ++lgrp;
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk) bp[bk] -= cols * 32;
+      enter();
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < S; ++u) load(wt[u], bs[u]);  // in flight while v is prepared
+  pdl_wait();
+  pdl_trigger();
+  {  // v: a warp per row, fp32 -> scaled (value, remainder) pairs in fragment order
+    constexpr int EL = (RV / 2 + 31) / 32;  // pairs of a lane
+    const int ad = s.adapter[warp];  // of row `warp`
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk) {
+      const float* row = p.v + (size_t(bk) * p.R + row0 + warp) * p.r;
+      float val[EL][2];
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < EL; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int c = 2 * (i * 32 + lane) + e;
+          val[i][e] = ad >= 0 && c < p.r ? __ldcg(row + c) : 0.f;
+          const float a = fabsf(val[i][e]);
+          if (a < INFINITY) m = fmaxf(m, a);
+        }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      int ex = 0;
+      if (m > 0.f) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
+      const float up = __uint_as_float(unsigned(127 + ex) << 23);
+      const float down = __uint_as_float(unsigned(127 - ex) << 23);
+#pragma unroll
+      for (int i = 0; i < EL; ++i) {
+        const int c = 2 * (i * 32 + lane);
+        if (c < RV) {
+          __half h[2], l[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = val[i][e] * up;
+            h[e] = __float2half_rn(x);
+            const float hf = __half2float(h[e]);
+            l[e] = __float2half_rn(fabsf(hf) < INFINITY ? x - hf : 0.f);
+          }
+          const int step = RV == 16 ? 0 : (c >> 5) * 2 + ((c >> 2) & 1);
+          const int q = RV == 16 ? c >> 2 : (c >> 3) & 3;
+          uint32_t* to = reinterpret_cast<uint32_t*>(&s_v[bk][step][warp * 4 + q]) + ((c >> 1) & 1);
+          to[0] = __half_as_ushort(h[0]) | (uint32_t(__half_as_ushort(h[1])) << 16);
+          to[2] = __half_as_ushort(l[0]) | (uint32_t(__half_as_ushort(l[1])) << 16);
+        }
+      }
+      if (lane == 0)
+        s_fac[bk][warp] = ad >= 0 ? (p.scale[bk] ? __ldg(p.scale[bk] + ad) : 1.f) * down : 0.f;
+    }
+  }
+  __syncthreads();
+  float fac[2][BANKS];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int bk = 0; bk < BANKS; ++bk) fac[h][bk] = s_fac[bk][2 * tq + h];
+  const int gid[2] = {s.group[2 * tq], s.group[2 * tq + 1]};
+  const bool none[2] = {s.adapter[2 * tq] < 0, s.adapter[2 * tq + 1] < 0};
+  int i = first, grp = i / cols, c = cg0 + i % cols;
+  __half* out = p.out + row_off + c * 32;
+  while (i < last) {
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      if (i >= last) break;
+      float acc[BANKS][2][4];
+#pragma unroll
+      for (int bk = 0; bk < BANKS; ++bk) wt[u][bk].multiply_rows(acc[bk], &s_v[bk][0][lane]);
+      const bool cok = c * 32 + 4 * g < p.N;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float o[BANKS][4];
+#pragma unroll
+        for (int bk = 0; bk < BANKS; ++bk) {
+          const __half2* b2 = reinterpret_cast<const __half2*>(&bs[u][bk][h]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float2 f = __half22float2(b2[x]);
+            o[bk][2 * x] = fmaf(acc[bk][x][h], fac[h][bk], f.x);
+            o[bk][2 * x + 1] = fmaf(acc[bk][x][2 + h], fac[h][bk], f.y);
+          }
+        }
+        if (MODE == kExpandSwiglu) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[0][x] = silu_f32(o[0][x]) * o[BANKS - 1][x];
+        }
+        const __half2 lo = __floats2half2_rn(o[0][0], o[0][1]);
+        const __half2 hi = __floats2half2_rn(o[0][2], o[0][3]);
+        uint2 r = make_uint2(reinterpret_cast<const uint32_t&>(lo),
+                             reinterpret_cast<const uint32_t&>(hi));
+        if (MODE == kExpandAdd && none[h]) r = bs[u][0][h];
+        if (cok && gid[h] == grp)
+          *reinterpret_cast<uint2*>(out + h * size_t(p.N)) = r;
+      }
+      load(wt[u], bs[u]);
+      ++i;
+      out += 32;
+      if (++c == cg1) {
+        c = cg0;
+        ++grp;
+        out -= cols * 32;
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -702,6 +924,22 @@ static int launch_expand(ExpandArgs p, cudaStream_t stream) {
                     dim3(kAdThreads), smem, stream, p);
 }
 
+template <int RV, int MODE>
+static int launch_expand_rows(ExpandArgs p, cudaStream_t stream) {
+  if (p.N > kMaxColumns) return LR_ERR_INVALID_ARGUMENT;
+  const long windows = (p.R + 7) / 8;
+  const int cgs = (p.N + 31) / 32;
+  // one wave of two blocks per SM
+  const long fit = (windows * cgs + 2 * kTargetBlocks - 1) / (2 * kTargetBlocks);
+  const int gpc = int(fit < 4 ? 4 : fit > 128 ? 128 : fit);
+  p.groups_per_chunk = gpc;
+  if ((cgs + gpc - 1) / gpc > 65535) return LR_ERR_INVALID_ARGUMENT;
+  return launch_pdl(expand_rows_kernel<RV, MODE>, dim3(unsigned(windows), (cgs + gpc - 1) / gpc),
+                    dim3(kAdThreads), 0, stream, p);
+}
+
+constexpr long kSmallRows = 256;  // up to here windows of 8 rows
+
 // Row windows of 64 (32 for SwiGLU), or of 16 while the larger ones would leave
 // fewer than two blocks of 256 columns for an SM.
 template <int MODE>
@@ -709,6 +947,13 @@ static int run_expand(const ExpandArgs& p, cudaStream_t stream) {
   constexpr int MT = MODE == kExpandSwiglu ? 2 : 4;
   const long blocks = (p.R + 16 * MT - 1) / (16 * MT) * ((p.N + 255) / 256);
   const bool small = blocks < 2 * kTargetBlocks;
+  if constexpr (MODE != kExpandProduct) {
+    if (p.R <= kSmallRows)
+      return p.r <= 16   ? launch_expand_rows<16, MODE>(p, stream)
+             : p.r <= 32 ? launch_expand_rows<32, MODE>(p, stream)
+             : p.r <= 64 ? launch_expand_rows<64, MODE>(p, stream)
+                         : launch_expand_rows<128, MODE>(p, stream);
+  }
   if (p.r <= 16)
     return small ? launch_expand<16, 1, MODE>(p, stream) : launch_expand<16, MT, MODE>(p, stream);
   if (p.r <= 32)

@@ -81,7 +81,10 @@ SHAPES = [  # rows, requests, K, N, adapters, rank
     (4099, 11, 512, 512, 7, 32), (5000, 5000, 128, 64, 40, 16),
     # windows of 64 rows with streamed base rows: one, a few and many groups in a window
     (9600, 2, 64, 520, 2, 8), (4099, 11, 512, 1544, 7, 32), (3000, 40, 136, 1808, 33, 104),
-    (2500, 9, 1000, 2056, 6, 64), (5000, 5000, 128, 1032, 40, 16), (19137, 700, 72, 232, 64, 24)]
+    (2500, 9, 1000, 2056, 6, 64), (5000, 5000, 128, 1032, 40, 16), (19137, 700, 72, 232, 64, 24),
+    # windows of 8 rows with many column groups to a warp; windows of 16 rows
+    (256, 256, 64, 5000, 64, 16), (250, 1, 64, 9608, 2, 64), (129, 40, 72, 8200, 7, 32),
+    (256, 30, 64, 4104, 9, 120), (700, 700, 64, 264, 30, 16), (500, 60, 64, 264, 9, 104)]
 
 
 @pytest.mark.parametrize("R,requests,K,N,n,r", SHAPES)
@@ -197,7 +200,10 @@ def test_bad_adapter_numbers_are_flagged_and_taken_as_none():
     (100, 7, 256, 520, 4, 128), (257, 4, 512, 264, 8, 32), (1000, 20, 136, 96, 16, 48),
     # windows of 32 rows with streamed base rows
     (2001, 3, 256, 1288, 3, 16), (1500, 90, 136, 1800, 7, 24), (1100, 1100, 64, 2312, 40, 40),
-    (9000, 12, 520, 264, 5, 128)])
+    (9000, 12, 520, 264, 5, 128),
+    # windows of 8 rows with many column groups to a warp; windows of 16 rows
+    (200, 200, 64, 3208, 32, 16), (256, 100, 64, 4104, 7, 128), (255, 2, 64, 9608, 2, 32),
+    (400, 130, 64, 264, 9, 16), (300, 6, 64, 264, 3, 128)])
 def test_adapter_swiglu(R, requests, K, N, n, r):
     from lightning_router.kernels.adapters import adapter_swiglu
     g = _gen(R + K + N)
