@@ -197,6 +197,13 @@ LR_DEVICE bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, volatile int* a
   }
 }
 
+// The same by all 32 lanes of a warp, with one verdict: lanes that saw the phase
+// complete do not go on to warp-wide instructions without lanes that gave up.
+LR_DEVICE bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* err,
+                              uint64_t limit_ns) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, err, limit_ns)) != 0;
+}
+
 // ---------------------------------------------------------------------------
 // TMA
 // ---------------------------------------------------------------------------

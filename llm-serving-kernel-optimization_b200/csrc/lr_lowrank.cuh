@@ -40,7 +40,9 @@ LR_DEVICE uint32_t cluster_nctarank() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
+// Of every thread of the cluster; the barrier takes a warp's lanes together.
 LR_DEVICE void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;"
                ::: "memory");
 }
@@ -415,9 +417,8 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     for (int i = first; i < last; ++i) {
       const int st = i % kTileStages, round = i / kTileStages, cg = cg0 + i * kTileGroups;
       if (round > 0 &&
-          !mbar_wait_bounded(s_empty + st, (round - 1) & 1, &s_abort, p.err, kCopyWaitNs))
+          !mbar_wait_warp(s_empty + st, (round - 1) & 1, &s_abort, p.err, kCopyWaitNs))
         return;
-      __syncwarp();
       if (lane < kTileGroups * 4 && cg * 32 + lane * 8 < p.N) {
 #pragma unroll
         for (int bk = 0; bk < BANKS; ++bk) {
@@ -532,7 +533,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
 
     const auto arrived = [&]() {
       return MODE == kExpandProduct ||
-             mbar_wait_bounded(s_full + st, parity, &s_abort, p.err, kCopyWaitNs);
+             mbar_wait_warp(s_full + st, parity, &s_abort, p.err, kCopyWaitNs);
     };
     // One group's rows of the tile of column group c.  `whole`: the window is one
     // group and `grp` is not looked at; `last`: the tile is not read again.
