@@ -324,12 +324,14 @@ LR_DEVICE int rank_chunk(int e, bool valid, int E, int32_t* s_wcnt, int32_t* s_r
 }
 
 // Last-block tail: scans blk_counts over blocks per expert into blk_base,
-// writes offsets / kept_counts and the aux loss, resets the ticket.
+// writes offsets / kept_counts and the aux loss, resets the ticket.  The number of
+// warps is a constant: with blockDim.x the scan of 1M tokens' blocks was 13 us slower.
+template <int NW>
 LR_DEVICE void route_tail(const RouteWs& ws, int B, int E, int C, int num_slots, int T, int k,
                           float lbw, int32_t* offsets, int32_t* kept_counts, float* aux_loss,
                           double* prob_sums, int32_t* s_tot, double* s_P, double* s_f) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int e = warp; e < E; e += blockDim.x / 32) {
+  for (int e = warp; e < E; e += NW) {
     int carry = 0;
     double psum = 0.0;
     for (int b0 = 0; b0 < B; b0 += 32) {
@@ -354,7 +356,7 @@ LR_DEVICE void route_tail(const RouteWs& ws, int B, int E, int C, int num_slots,
   }
   __syncthreads();
   // a thread per expert divides; one thread then scans and sums in expert order
-  for (int e = tid; e < E; e += blockDim.x) {
+  for (int e = tid; e < E; e += NW * 32) {
     if (kept_counts) kept_counts[e] = min(s_tot[e], C);
     if (prob_sums) prob_sums[e] = s_P[e];
     if (aux_loss) {
@@ -545,14 +547,15 @@ __global__ void __launch_bounds__(kRouteThreads)
     }
   }
   if (!arrive_last(ws.ticket, num_blocks, &s_last)) return;
-  route_tail(ws, num_blocks, E, C, T * k, T, k, lbw, offsets, kept_counts, aux_loss, prob_sums,
-             s_tot, s_P, s_f);
+  route_tail<kWarps>(ws, num_blocks, E, C, T * k, T, k, lbw, offsets, kept_counts, aux_loss,
+                     prob_sums, s_tot, s_P, s_f);
 }
 
 // The same for more than 8 experts, bit for bit, with a token's logits spread over
 // LPT lanes (8 neighbouring experts each): the one-thread form above unrolls 64
 // experts times k selections into more instructions than the caches hold (777
-// tokens, 64 experts, top-6: 60 us).  The softmax denominator runs through the
+// tokens, 64 experts, top-6: 60 us).  Up to 32 experts the one-thread form takes
+// batches that fill the SMs several times over (see lr_topk_route).  The softmax denominator runs through the
 // lanes in expert order and the probability sums follow the shuffle tree of
 // warp_prob_sums, so sums keep their order; a NaN is selected where the scan of
 // topk_softmax would (as the first expert not yet taken).
@@ -743,8 +746,8 @@ __global__ void __launch_bounds__(route_lanes_threads<LPT>())
     }
   }
   if (!arrive_last(ws.ticket, num_blocks, &s_last)) return;
-  route_tail(ws, num_blocks, E, C, T * k, T, k, lbw, offsets, kept_counts, aux_loss, prob_sums,
-             s_tot, s_P, s_f);
+  route_tail<kThreads / 32>(ws, num_blocks, E, C, T * k, T, k, lbw, offsets, kept_counts, aux_loss,
+                            prob_sums, s_tot, s_P, s_f);
 }
 
 // ---------------------------------------------------------------------------
@@ -782,8 +785,8 @@ __global__ void __launch_bounds__(kRouteThreads)
   }
   for (int i = tid; i < E; i += kRouteThreads) ws.blk_counts[size_t(blockIdx.x) * E + i] = s_run[i];
   if (!arrive_last(ws.ticket, num_blocks, &s_last)) return;
-  route_tail(ws, num_blocks, E, C, S, 1, 1, 0.f, offsets, kept_counts, nullptr, nullptr, s_tot,
-             s_P, nullptr);
+  route_tail<kWarps>(ws, num_blocks, E, C, S, 1, 1, 0.f, offsets, kept_counts, nullptr, nullptr,
+                     s_tot, s_P, nullptr);
 }
 
 // ---------------------------------------------------------------------------
@@ -1411,8 +1414,18 @@ extern "C" int lr_topk_route(const float* logits, int T, int E, int k, int capac
   KERNEL<<<B, THREADS, 0, stream>>>(                                      \
       logits, T, E, k, capacity, load_balance_weight, expert_ids, gate_weights, token_indices, \
       slot_pos, offsets, kept_counts, aux_loss, prob_sums, ws, B)
+  // A block of lanes holds a quarter (E <= 32) or a half (E <= 16) of the tokens that
+  // one-thread blocks keep on an SM, and pays shuffles for each selection: past four
+  // blocks x selections per SM the one-thread form is ahead (262144 tokens, 24
+  // experts top-4: 114 against 140 us, 16 top-8: 91 against 107; 32768 tokens: 27
+  // against 25, 25 against 25; top-1 never: 32 experts, 262144 tokens, 126 against 121).
+  const bool one_thread = k > 1 && long(B) * k > 4 * 148;
   if (E <= 8)
     LR_ROUTE_CASE(topk_route_kernel<8>, kRouteThreads);
+  else if (E <= 16 && one_thread)
+    LR_ROUTE_CASE(topk_route_kernel<16>, kRouteThreads);
+  else if (E <= 32 && one_thread)
+    LR_ROUTE_CASE(topk_route_kernel<32>, kRouteThreads);
   else if (E <= 16)
     LR_ROUTE_CASE(topk_route_lanes_kernel<2>, route_lanes_threads<2>());
   else if (E <= 32)
