@@ -1362,12 +1362,25 @@ using namespace lr;
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Where the tiled kernel is ahead.  Rows shorter than 256 leave its ring nothing to
+// stream (20000 x 64, 32 experts: 9.3 us untiled, 12.4 tiled), except for up to 16
+// experts once every SM has a tile of 64 tokens (65536 x 64, 8 experts: 17 against
+// 10); 17 to 64 experts share one block per tile of tokens, which takes longer rows
+// to pay below 4096 tokens (2048 x 512, 64 experts: 8.3 untiled, 10.4 tiled; x 1024:
+// 12.4 both).
+static bool gate_tiled(int T, int d, int E) {
+  if (T < kGateTiledTokens) return false;
+  if (E <= 16) return d >= 256 || T >= 64 * 148;
+  if (E <= 64 && T < 4096) return d >= (E <= 32 ? 512 : 1024);
+  return d >= 256;
+}
+
 extern "C" int lr_gate_logits(const void* h, const void* wg, const float* bias, int T, int d, int E,
                               float* logits, lr_stream_t stream) {
   if (T < 0 || d <= 0 || d % 16 != 0 || E < 1 || E > 256) return LR_ERR_INVALID_ARGUMENT;
   if (T == 0) return LR_OK;
   if (!h || !wg || !logits) return LR_ERR_INVALID_ARGUMENT;
-  if (T >= kGateTiledTokens && aligned16(h) && aligned16(wg)) {
+  if (gate_tiled(T, d, E) && aligned16(h) && aligned16(wg)) {
     const __half* hp = static_cast<const __half*>(h);
     const __half* wp = static_cast<const __half*>(wg);
     // tiles of 32 tokens while tiles of 64 would leave SMs idle (3000 x 4096, 8
