@@ -403,22 +403,25 @@ void check_rows(const at::Tensor& t, const at::Tensor& x, int64_t N, const char*
               name, ": (", x.size(0), ", ", N, ") fp16 expected");
 }
 
-// The result tensor: a new one, or `out`, which may share memory with the rows
-// it is computed from only as the very same tensor.
-at::Tensor result_rows(const OptTensor& out, const at::Tensor& x, int64_t N,
-                       std::initializer_list<at::Tensor> reads) {
-  if (!given(out)) return at::empty({x.size(0), N}, x.options());
-  check_rows(*out, x, N, "out");
-  TORCH_CHECK(out->is_contiguous() && (reinterpret_cast<uintptr_t>(out->data_ptr()) & 15u) == 0,
+// A given result may share memory with the rows it is computed from only as the
+// very same tensor.
+void check_out(const at::Tensor& out, const at::Tensor& x, int64_t N,
+               std::initializer_list<at::Tensor> reads) {
+  check_rows(out, x, N, "out");
+  TORCH_CHECK(out.is_contiguous() && (reinterpret_cast<uintptr_t>(out.data_ptr()) & 15u) == 0,
               "out must be contiguous and 16-byte aligned");
-  const char* o0 = static_cast<const char*>(out->data_ptr());
-  const char* o1 = o0 + out->nbytes();
+  const char* o0 = static_cast<const char*>(out.data_ptr());
+  const char* o1 = o0 + out.nbytes();
   for (const at::Tensor& t : reads) {
     const char* t0 = static_cast<const char*>(t.data_ptr());
     const char* t1 = t0 + t.nbytes();
     TORCH_CHECK(t0 == o0 || t1 <= o0 || o1 <= t0, "out overlaps an input at another offset");
   }
-  return *out;
+}
+
+// Kernels write through raw pointers: a graph that saved `t` learns of it here.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 void check_index(const at::Tensor& index, const at::Tensor& x) {
@@ -427,15 +430,17 @@ void check_index(const at::Tensor& index, const at::Tensor& x) {
   check_int32(index, x, x.size(0), "index");
 }
 
-at::Tensor adapter_add(const at::Tensor& x_in, const at::Tensor& index, const at::Tensor& a,
-                       const at::Tensor& b, const OptTensor& scale, const at::Tensor& base_in,
-                       const OptTensor& out_in, const OptTensor& err) {
+at::Tensor adapter_add_rows(const at::Tensor& x_in, const at::Tensor& index, const at::Tensor& a,
+                            const at::Tensor& b, const OptTensor& scale,
+                            const at::Tensor& base_in, const OptTensor& out_in,
+                            const OptTensor& err) {
   check_index(index, x_in);
   const Bank k = check_bank(a, b, scale, x_in);
   check_rows(base_in, x_in, k.N, "base");
   c10::cuda::CUDAGuard g(x_in.device());
   const at::Tensor x = rows16(x_in, at::kHalf), base = rows16(base_in, at::kHalf);
-  at::Tensor out = result_rows(out_in, x, k.N, {base});
+  if (given(out_in)) check_out(*out_in, x, k.N, {base});
+  at::Tensor out = given(out_in) ? *out_in : at::empty({x.size(0), k.N}, x.options());
   const int64_t R = x.size(0);
   auto ws = workspace(lr_adapter_workspace_bytes(as_int(R), as_int(k.r), 1), x);
   check_status(lr_adapter_add(x.data_ptr(), as_int(R), as_int(k.K), index.data_ptr<int32_t>(),
@@ -446,11 +451,12 @@ at::Tensor adapter_add(const at::Tensor& x_in, const at::Tensor& index, const at
   return out;
 }
 
-at::Tensor adapter_swiglu(const at::Tensor& x_in, const at::Tensor& index, const at::Tensor& a_gate,
-                          const at::Tensor& b_gate, const OptTensor& scale_gate,
-                          const at::Tensor& a_up, const at::Tensor& b_up,
-                          const OptTensor& scale_up, const at::Tensor& gate_in,
-                          const at::Tensor& up_in, const OptTensor& out_in, const OptTensor& err) {
+at::Tensor adapter_swiglu_rows(const at::Tensor& x_in, const at::Tensor& index,
+                               const at::Tensor& a_gate, const at::Tensor& b_gate,
+                               const OptTensor& scale_gate, const at::Tensor& a_up,
+                               const at::Tensor& b_up, const OptTensor& scale_up,
+                               const at::Tensor& gate_in, const at::Tensor& up_in,
+                               const OptTensor& out_in, const OptTensor& err) {
   check_index(index, x_in);
   const Bank kg = check_bank(a_gate, b_gate, scale_gate, x_in);
   const Bank ku = check_bank(a_up, b_up, scale_up, x_in);
@@ -461,7 +467,8 @@ at::Tensor adapter_swiglu(const at::Tensor& x_in, const at::Tensor& index, const
   c10::cuda::CUDAGuard g(x_in.device());
   const at::Tensor x = rows16(x_in, at::kHalf), gate = rows16(gate_in, at::kHalf),
                    up = rows16(up_in, at::kHalf);
-  at::Tensor out = result_rows(out_in, x, kg.N, {gate, up});
+  if (given(out_in)) check_out(*out_in, x, kg.N, {gate, up});
+  at::Tensor out = given(out_in) ? *out_in : at::empty({x.size(0), kg.N}, x.options());
   const int64_t R = x.size(0);
   auto ws = workspace(lr_adapter_workspace_bytes(as_int(R), as_int(kg.r), 2), x);
   check_status(lr_adapter_swiglu(x.data_ptr(), as_int(R), as_int(kg.K), index.data_ptr<int32_t>(),
@@ -471,6 +478,38 @@ at::Tensor adapter_swiglu(const at::Tensor& x_in, const at::Tensor& index, const
                                  cur_stream()),
                "adapter_swiglu");
   return out;
+}
+
+at::Tensor adapter_add(const at::Tensor& x, const at::Tensor& index, const at::Tensor& a,
+                       const at::Tensor& b, const OptTensor& scale, const at::Tensor& base,
+                       const OptTensor& err) {
+  return adapter_add_rows(x, index, a, b, scale, base, {}, err);
+}
+
+void adapter_add_out(const at::Tensor& x, const at::Tensor& index, const at::Tensor& a,
+                     const at::Tensor& b, const OptTensor& scale, const at::Tensor& base,
+                     const at::Tensor& out, const OptTensor& err) {
+  adapter_add_rows(x, index, a, b, scale, base, out, err);
+  written(out);
+}
+
+at::Tensor adapter_swiglu(const at::Tensor& x, const at::Tensor& index, const at::Tensor& a_gate,
+                          const at::Tensor& b_gate, const OptTensor& scale_gate,
+                          const at::Tensor& a_up, const at::Tensor& b_up,
+                          const OptTensor& scale_up, const at::Tensor& gate,
+                          const at::Tensor& up, const OptTensor& err) {
+  return adapter_swiglu_rows(x, index, a_gate, b_gate, scale_gate, a_up, b_up, scale_up, gate, up,
+                             {}, err);
+}
+
+void adapter_swiglu_out(const at::Tensor& x, const at::Tensor& index, const at::Tensor& a_gate,
+                        const at::Tensor& b_gate, const OptTensor& scale_gate,
+                        const at::Tensor& a_up, const at::Tensor& b_up, const OptTensor& scale_up,
+                        const at::Tensor& gate, const at::Tensor& up, const at::Tensor& out,
+                        const OptTensor& err) {
+  adapter_swiglu_rows(x, index, a_gate, b_gate, scale_gate, a_up, b_up, scale_up, gate, up, out,
+                      err);
+  written(out);
 }
 
 at::Tensor adapter_rows(const at::Tensor& adapter_ids, const at::Tensor& source_idx,
@@ -505,11 +544,18 @@ TORCH_LIBRARY_FRAGMENT(lightning_router, m) {
       "kept_counts, int k) -> Tensor");
   m.def(
       "adapter_add(Tensor x, Tensor index, Tensor a, Tensor b, Tensor? scale, Tensor base, "
-      "Tensor? out, Tensor? err) -> Tensor");
+      "Tensor? err) -> Tensor");
+  m.def(
+      "adapter_add_out(Tensor x, Tensor index, Tensor a, Tensor b, Tensor? scale, Tensor base, "
+      "Tensor(a!) out, Tensor? err) -> ()");
   m.def(
       "adapter_swiglu(Tensor x, Tensor index, Tensor a_gate, Tensor b_gate, Tensor? scale_gate, "
-      "Tensor a_up, Tensor b_up, Tensor? scale_up, Tensor gate, Tensor up, Tensor? out, "
-      "Tensor? err) -> Tensor");
+      "Tensor a_up, Tensor b_up, Tensor? scale_up, Tensor gate, Tensor up, Tensor? err) -> "
+      "Tensor");
+  m.def(
+      "adapter_swiglu_out(Tensor x, Tensor index, Tensor a_gate, Tensor b_gate, Tensor? "
+      "scale_gate, Tensor a_up, Tensor b_up, Tensor? scale_up, Tensor gate, Tensor up, "
+      "Tensor(a!) out, Tensor? err) -> ()");
   m.def(
       "adapter_rows(Tensor adapter_ids, Tensor source_idx, Tensor offsets, Tensor kept_counts, "
       "int num_adapters, Tensor? err) -> Tensor");
@@ -522,7 +568,9 @@ TORCH_LIBRARY_IMPL(lightning_router, CUDA, m) {
   m.impl("dispatch_tokens", &dispatch_tokens);
   m.impl("combine_tokens", &combine_tokens);
   m.impl("adapter_add", &adapter_add);
+  m.impl("adapter_add_out", &adapter_add_out);
   m.impl("adapter_swiglu", &adapter_swiglu);
+  m.impl("adapter_swiglu_out", &adapter_swiglu_out);
   m.impl("adapter_rows", &adapter_rows);
 }
 

@@ -84,12 +84,17 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, bank: AdapterBank, index: t
     """``base + scale (x A^T) B^T`` with each row's adapter ``index`` (R,) integers, -1: none.
 
     ``x`` (R, K) and ``base`` (R, N) fp16.  ``out`` (contiguous) may be ``base`` itself; rows
-    without an adapter are then left as they are.  A number outside [-1, n) is taken as -1 and
+    without an adapter are then left as they are.  Writing to it counts as an in-place change:
+    a backward pass that needs its former values raises.  A number outside [-1, n) is taken as -1 and
     flagged (:func:`lightning_router._ext.check_device_errors`)."""
     _ext.require_cuda(base, x, index, *bank)
-    _no_grad("adapter_add", base, x, *bank)
-    return _ext.ops().adapter_add(x, adapter_index(index), bank.a, bank.b, bank.scale, base, out,
-                                  _ext.error_word(x.device.index))
+    _no_grad("adapter_add", base, x, *bank, out)
+    args = (x, adapter_index(index), bank.a, bank.b, bank.scale, base)
+    err = _ext.error_word(x.device.index)
+    if out is None:
+        return _ext.ops().adapter_add(*args, err)
+    _ext.ops().adapter_add_out(*args, out, err)
+    return out
 
 
 def adapter_swiglu(gate: torch.Tensor, up: torch.Tensor, x: torch.Tensor, gate_bank: AdapterBank,
@@ -98,10 +103,13 @@ def adapter_swiglu(gate: torch.Tensor, up: torch.Tensor, x: torch.Tensor, gate_b
     """``silu(gate + delta_gate) * (up + delta_up)`` with each row's adapters; see
     :func:`adapter_add`.  The banks have the same n, rank and sizes."""
     _ext.require_cuda(gate, up, x, index, *gate_bank, *up_bank)
-    _no_grad("adapter_swiglu", gate, up, x, *gate_bank, *up_bank)
-    return _ext.ops().adapter_swiglu(x, adapter_index(index), gate_bank.a, gate_bank.b, gate_bank.scale,
-                                     up_bank.a, up_bank.b, up_bank.scale, gate, up, out,
-                                     _ext.error_word(x.device.index))
+    _no_grad("adapter_swiglu", gate, up, x, *gate_bank, *up_bank, out)
+    args = (x, adapter_index(index), *gate_bank, *up_bank, gate, up)
+    err = _ext.error_word(x.device.index)
+    if out is None:
+        return _ext.ops().adapter_swiglu(*args, err)
+    _ext.ops().adapter_swiglu_out(*args, out, err)
+    return out
 
 
 def adapter_rows(adapter_ids: torch.Tensor, plan, num_adapters: int) -> torch.Tensor:
