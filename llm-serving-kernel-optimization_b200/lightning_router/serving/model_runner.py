@@ -31,6 +31,17 @@ class _Graph:
                  aux: torch.Tensor, ids: torch.Tensor | None = None, adapters=None):
         self.graph, self.x, self.out, self.aux = graph, x, out, aux
         self.ids, self.adapters = ids, adapters   # the adapters that the graph reads
+        # the memory it reads, kept for as long as the graph may be replayed
+        self.banks = [] if adapters is None else [b.detach() for b in adapters.buffers()]
+
+    def reads(self, adapters) -> bool:
+        """Whether these are the adapters captured, in the memory they had then."""
+        if adapters is not self.adapters:
+            return False
+        now = list(adapters.buffers())
+        return len(now) == len(self.banks) and all(
+            a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.dtype == b.dtype
+            and a.stride() == b.stride() for a, b in zip(now, self.banks))
 
 
 class LightningModelRunner:
@@ -113,8 +124,8 @@ class LightningModelRunner:
         h = hidden_states.reshape(-1, shape[-1])
         key = (h.shape[0], h.shape[1])
         gr = self._graphs.get(key if adapter_ids is None else (*key, True))
-        if gr is not None and gr.ids is not None and gr.adapters is not layer.adapters:
-            gr = None   # captured with adapters that the layer no longer has
+        if gr is not None and gr.ids is not None and not gr.reads(layer.adapters):
+            gr = None   # captured with adapters that the layer no longer has, or has elsewhere
         if gr is None:
             out, _ = layer(h, adapter_ids=adapter_ids)
             return out.view(shape).to(hidden_states.dtype)
