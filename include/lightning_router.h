@@ -293,6 +293,11 @@ size_t lr_gate_backward_workspace_bytes(int num_tokens, int d_model, int num_exp
 int lr_gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d, int E,
                      void* d_h, float* d_wg, float* d_bias, void* workspace,
                      size_t workspace_bytes, lr_stream_t stream);
+/* The same with d_h[T,d] in fp32, not rounded (hidden rows that were fp32 or bf16
+ * before lr_gate_logits: their gradients may leave the range of fp16).       */
+int lr_gate_backward_rows32(const void* h, const void* wg, const float* d_logits, int T, int d,
+                            int E, float* d_h, float* d_wg, float* d_bias, void* workspace,
+                            size_t workspace_bytes, lr_stream_t stream);
 
 /* Gradient of the row dispatch: d_x[t,:] = fp16(sum_j d_permuted[slot_pos[t*k+j],:])
  * over kept slots, fp32 in slot order.  d % 8 == 0.                           */

@@ -196,18 +196,25 @@ struct GateProjection : public torch::autograd::Function<GateProjection> {
     const bool need_h = need & 1, need_b = need & 4, need_w = need & 6;
     const auto fopt = dl.options();
     at::Tensor dh, dw, db;
-    if (need_h) dh = at::empty({T, d}, fopt.dtype(at::kHalf));
+    // hidden rows of other types than fp16 get the sums as they are, rounded once at the end
+    const bool rows32 = ctx->saved_data.find("h_type") != ctx->saved_data.end();
+    if (need_h) dh = at::empty({T, d}, fopt.dtype(rows32 ? at::kFloat : at::kHalf));
     if (need_w) dw = at::empty({E, d}, fopt);
     if (need_b) db = at::empty({E}, fopt);
     const size_t wsb = lr_gate_backward_workspace_bytes(as_int(T), as_int(d), as_int(E));
     at::Tensor ws;
     if (wsb) ws = workspace(wsb, dl);
-    check_status(lr_gate_backward(h.data_ptr(), w.data_ptr(), dl.data_ptr<float>(), as_int(T),
-                                  as_int(d), as_int(E), need_h ? dh.data_ptr() : nullptr,
-                                  need_w ? dw.data_ptr<float>() : nullptr,
-                                  need_b ? db.data_ptr<float>() : nullptr,
-                                  wsb ? ws.data_ptr() : nullptr, wsb, cur_stream()),
-                 "gate_projection (backward)");
+    const auto run = [&](auto entry, auto* dh_ptr) {
+      check_status(entry(h.data_ptr(), w.data_ptr(), dl.data_ptr<float>(), as_int(T), as_int(d),
+                         as_int(E), dh_ptr, need_w ? dw.data_ptr<float>() : nullptr,
+                         need_b ? db.data_ptr<float>() : nullptr, wsb ? ws.data_ptr() : nullptr,
+                         wsb, cur_stream()),
+                   "gate_projection (backward)");
+    };
+    if (rows32)
+      run(lr_gate_backward_rows32, need_h ? dh.data_ptr<float>() : nullptr);
+    else
+      run(lr_gate_backward, need_h ? dh.data_ptr() : nullptr);
     const auto cast = [&](at::Tensor& t, const char* key) {
       const auto it = ctx->saved_data.find(key);
       if (t.defined() && it != ctx->saved_data.end())

@@ -477,7 +477,7 @@ extern "C" int lr_adapter_add(const void* x, int R, int K, const int32_t* index,
                 static_cast<float*>(workspace), R, K, num_adapters, rank, err};
   if (const int rc = run_shrink(sp, 1, stream)) return rc;
   ExpandArgs ep{sp.v, {static_cast<const __half*>(b), nullptr}, {scale, nullptr}, index,
-                {static_cast<const __half*>(base), nullptr}, static_cast<__half*>(out), R, N,
+                {static_cast<const __half*>(base), nullptr}, out, R, N,
                 num_adapters, rank, rank, 0, base == out, err};
   return run_expand<kExpandAdd>(ep, stream);
 }
@@ -502,7 +502,7 @@ extern "C" int lr_adapter_swiglu(const void* x, int R, int K, const int32_t* ind
   ExpandArgs ep{sp.v, {static_cast<const __half*>(b_gate), static_cast<const __half*>(b_up)},
                 {scale_gate, scale_up}, index,
                 {static_cast<const __half*>(gate), static_cast<const __half*>(up)},
-                static_cast<__half*>(out), R, N, num_adapters, rank, rank, 0, false, err};
+                out, R, N, num_adapters, rank, rank, 0, false, err};
   return run_expand<kExpandSwiglu>(ep, stream);
 }
 

@@ -192,7 +192,12 @@ enum ExpandMode : int {
   kExpandAdd = 0,      // base + delta
   kExpandSwiglu = 1,   // silu(base + delta) * (base2 + delta2)
   kExpandProduct = 2,  // delta alone, every row with entry 0 of b (no index)
+  kExpandProduct32 = 3,  // the same, out in fp32
 };
+
+constexpr bool is_product(int mode) {
+  return mode == kExpandProduct || mode == kExpandProduct32;
+}
 
 struct ExpandArgs {
   const float* v;  // [bank][R][r]
@@ -200,7 +205,7 @@ struct ExpandArgs {
   const float* scale[2];
   const int32_t* index;
   const __half* base[2];  // the base rows; gate and up rows for SwiGLU
-  __half* out;
+  void* out;  // fp16; fp32 for kExpandProduct32
   long R;
   int N, n, r, ldb;
   int groups_per_chunk;  // 32-column groups of a block
@@ -321,7 +326,7 @@ constexpr int expand_ahead() {
 // parts.)  Without base rows all eight warps consume.
 template <int MODE>
 constexpr int consumers() {
-  return MODE == kExpandProduct ? kAdWarps : kAdWarps - 1;
+  return is_product(MODE) ? kAdWarps : kAdWarps - 1;
 }
 constexpr int kTilePitch = (kAdWarps - 1) * 64;  // bytes, 64 mod 128: neighbouring rows in
                                                  // different banks
@@ -332,7 +337,7 @@ constexpr int tile_stages() {
 
 template <int RV, int MT, int MODE>
 constexpr int expand_base_bytes() {
-  return MODE == kExpandProduct || MT == 1
+  return is_product(MODE) || MT == 1
              ? 0
              : tile_stages<MODE>() * (MODE == kExpandSwiglu ? 2 : 1) * MT * 16 * kTilePitch;
 }
@@ -348,6 +353,26 @@ constexpr int expand_min_blocks() {
   return RV <= (MODE == kExpandSwiglu ? (MT == 1 ? 32 : 16) : 64) ? 2 : 1;
 }
 
+template <int MODE>
+struct ExpandOut {
+  using type = __half;
+};
+template <>
+struct ExpandOut<kExpandProduct32> {
+  using type = float;
+};
+
+// Eight results of a row of the fp32 product, unrounded.
+LR_DEVICE void store_product32(float* to, const float (&acc)[1][4][4], int h, float fac) {
+  float4 o[2];
+  o[0] = make_float4(acc[0][0][2 * h] * fac, acc[0][0][2 * h + 1] * fac, acc[0][1][2 * h] * fac,
+                     acc[0][1][2 * h + 1] * fac);
+  o[1] = make_float4(acc[0][2][2 * h] * fac, acc[0][2][2 * h + 1] * fac, acc[0][3][2 * h] * fac,
+                     acc[0][3][2 * h + 1] * fac);
+  reinterpret_cast<float4*>(to)[0] = o[0];
+  reinterpret_cast<float4*>(to)[1] = o[1];
+}
+
 // Eight results of a row: base (and base2) with the scaled sums of both banks.
 template <int MODE, int BANKS>
 LR_DEVICE uint4 expand_epilogue(const float (&acc)[BANKS][4][4], int h, const float (&fac)[BANKS],
@@ -358,7 +383,7 @@ LR_DEVICE uint4 expand_epilogue(const float (&acc)[BANKS][4][4], int h, const fl
     const __half2* bh = reinterpret_cast<const __half2*>(&base[bk]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 b2 = MODE == kExpandProduct ? make_float2(0.f, 0.f) : __half22float2(bh[j]);
+      const float2 b2 = is_product(MODE) ? make_float2(0.f, 0.f) : __half22float2(bh[j]);
       o[bk][2 * j] = fmaf(acc[bk][j][2 * h], fac[bk], b2.x);
       o[bk][2 * j + 1] = fmaf(acc[bk][j][2 * h + 1], fac[bk], b2.y);
     }
@@ -388,7 +413,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   // Only v comes from the launch before (shrink, which lets this one start after its
   // own wait): index, base rows and weights are read ahead of that launch's end.
   // A product's weights are its predecessor's, too.
-  if (MODE == kExpandProduct) {
+  if (is_product(MODE)) {
     pdl_wait();
     pdl_trigger();
   }
@@ -397,9 +422,9 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   const int nrows = int(min(long(W), p.R - row0));
   const int cg0 = blockIdx.y * p.groups_per_chunk;
   const int cg1 = min(cg0 + p.groups_per_chunk, (p.N + 31) / 32);
-  if (MODE != kExpandProduct && warp == 0)
+  if (!is_product(MODE) && warp == 0)
     group_rows<W>(s, p.index, row0, p.R, p.n, !p.in_place, nullptr);
-  if (MT > 1 && MODE != kExpandProduct && threadIdx.x == 32) {
+  if (MT > 1 && !is_product(MODE) && threadIdx.x == 32) {
     for (int i = 0; i < kTileStages; ++i) {
       mbar_init(s_full + i, 32);  // the producer's lanes
       mbar_init(s_empty + i, kTileGroups);
@@ -408,7 +433,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     fence_mbarrier_init();
   }
   __syncthreads();
-  const bool stream = MT > 1 && MODE != kExpandProduct && s.n > 0;
+  const bool stream = MT > 1 && !is_product(MODE) && s.n > 0;
 
   // Producer: tiles [first, last) of the base rows, each as soon as its stage has
   // been read.  The first stages start ahead of everything else.
@@ -436,13 +461,13 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
 
   // Windows of 16 rows: the weights of groups [g0, g0 + S) for column group c.
   constexpr int S = MT == 1 ? expand_ahead<RV, MODE>() : 1;
-  const int n_groups = MODE == kExpandProduct ? 1 : s.n;
+  const int n_groups = is_product(MODE) ? 1 : s.n;
   RankTile<RV> wt[S][BANKS];
   const auto group_weights = [&](int c, int g0) {
     const int nr = c * 32 + (g >> 1) * 8;
 #pragma unroll
     for (int u = 0; u < S; ++u) {
-      const int ad = MODE == kExpandProduct ? 0
+      const int ad = is_product(MODE) ? 0
                      : g0 + u < n_groups    ? s.adapter[s.first[g0 + u]]
                                             : -1;
 #pragma unroll
@@ -456,7 +481,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   // (SwiGLU and rank 64 lose more to spills).
   constexpr bool EARLY = MT == 1 && RV == 16 && MODE == kExpandAdd;
   if (EARLY) group_weights(cg0 + warp, 0);
-  if (MODE != kExpandProduct) {
+  if (!is_product(MODE)) {
     pdl_wait();
     pdl_trigger();
   }
@@ -464,7 +489,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     constexpr int LPR = kAdThreads / W;               // lanes of a row
     constexpr int EL = (RV / 2 + LPR - 1) / LPR;      // pairs of a lane
     const int t = threadIdx.x / LPR, q = threadIdx.x % LPR;
-    const int ad = MODE == kExpandProduct ? (t < nrows ? 0 : -1) : s.adapter[t];
+    const int ad = is_product(MODE) ? (t < nrows ? 0 : -1) : s.adapter[t];
 #pragma unroll
     for (int bk = 0; bk < BANKS; ++bk) {
       const float* row = p.v + (size_t(bk) * p.R + row0 + t) * p.r;
@@ -516,7 +541,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
   if (MT > 1) {
     // Every consumer takes its 32 of a tile's columns for all rows: a window's groups
     // one after the other (one for a prompt), each on its own row tiles.
-    if (MODE != kExpandProduct && warp == kProducer) {
+    if (!is_product(MODE) && warp == kProducer) {
       if (stream) produce(min(n_tiles, kTileStages), n_tiles);
       cp_async_wait_all();  // leave no copy behind
       return;
@@ -526,13 +551,14 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     for (int i = 0; i < 2 * MT; ++i)
 #pragma unroll
       for (int bk = 0; bk < BANKS; ++bk) fac[i][bk] = s_fac[bk][g + 8 * i];
-    __half* out = p.out + size_t(row0 + g) * p.N + (cg0 + warp) * 32 + tq * 8;
+    using Out = typename ExpandOut<MODE>::type;
+    Out* out = static_cast<Out*>(p.out) + size_t(row0 + g) * p.N + (cg0 + warp) * 32 + tq * 8;
     const unsigned char* bp = s_dyn + g * kTilePitch + warp * 64 + tq * 16;
     const uint4* vp = s_v + lane;
     unsigned st = 0, parity = 0;
 
     const auto arrived = [&]() {
-      return MODE == kExpandProduct ||
+      return is_product(MODE) ||
              mbar_wait_warp(s_full + st, parity, &s_abort, p.err, kCopyWaitNs);
     };
     // One group's rows of the tile of column group c.  `whole`: the window is one
@@ -552,10 +578,10 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int bk = 0; bk < BANKS; ++bk)
-            if (MODE != kExpandProduct)
+            if (!is_product(MODE))
               bs[h][bk] = *reinterpret_cast<const uint4*>(
                   bp + ((st * BANKS + bk) * W + 16 * m + 8 * h) * kTilePitch);
-        if (m == MT - 1 && MODE != kExpandProduct && last) {
+        if (m == MT - 1 && !is_product(MODE) && last) {
           __syncwarp();
           if (lane == 0) mbar_arrive(s_empty + st);
         }
@@ -568,9 +594,14 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint4 o = expand_epilogue<MODE, BANKS>(acc, h, fac[2 * m + h], bs[h]);
-          if (cok && mine[h])
-            *reinterpret_cast<uint4*>(out + size_t(unsigned(2 * m + h) * n8)) = o;
+          if constexpr (MODE == kExpandProduct32) {
+            if (cok && mine[h])
+              store_product32(out + size_t(unsigned(2 * m + h) * n8), acc, h, fac[2 * m + h][0]);
+          } else {
+            const uint4 o = expand_epilogue<MODE, BANKS>(acc, h, fac[2 * m + h], bs[h]);
+            if (cok && mine[h])
+              *reinterpret_cast<uint4*>(out + size_t(unsigned(2 * m + h) * n8)) = o;
+          }
         }
       }
     };
@@ -583,8 +614,8 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     };
     const int end = cg0 + warp + n_tiles * kTileGroups;
     int c = cg0 + warp;
-    if (MODE == kExpandProduct || s.uniform) {
-      const int ad = MODE == kExpandProduct ? 0 : s.adapter[0];
+    if (is_product(MODE) || s.uniform) {
+      const int ad = is_product(MODE) ? 0 : s.adapter[0];
       const __half* wp[BANKS];
 #pragma unroll
       for (int bk = 0; bk < BANKS; ++bk)
@@ -600,7 +631,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
       };
       // the next column group's weights load while one is multiplied
       RankTile<RV> w0[BANKS], w1[BANKS];
-      if (RV <= (MODE == kExpandProduct ? 32 : 64) && MODE != kExpandSwiglu) {
+      if (RV <= (is_product(MODE) ? 32 : 64) && MODE != kExpandSwiglu) {
         weights(w0, c);
         while (true) {
           weights(w1, c + kTileGroups);
@@ -652,8 +683,8 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int t = g + 8 * h;
-    gid[h] = MODE == kExpandProduct ? (t < nrows ? 0 : -1) : s.group[t];
-    none[h] = MODE != kExpandProduct && s.adapter[t] < 0;
+    gid[h] = is_product(MODE) ? (t < nrows ? 0 : -1) : s.group[t];
+    none[h] = !is_product(MODE) && s.adapter[t] < 0;
 #pragma unroll
     for (int bk = 0; bk < BANKS; ++bk) fac[h][bk] = s_fac[bk][t];
   }
@@ -666,7 +697,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int bk = 0; bk < BANKS; ++bk)
-        if (MODE != kExpandProduct && cok && gid[h] >= 0)
+        if (!is_product(MODE) && cok && gid[h] >= 0)
           bs[h][bk] = ld_row(reinterpret_cast<const uint4*>(p.base[bk] + off + h * n8));
     float acc[BANKS][4][4];
 #pragma unroll
@@ -696,9 +727,13 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (!cok || gid[h] < 0) continue;
-      uint4 o = expand_epilogue<MODE, BANKS>(acc, h, fac[h], bs[h]);
-      if (MODE == kExpandAdd && none[h]) o = bs[h][0];
-      *reinterpret_cast<uint4*>(p.out + off + h * n8) = o;
+      if constexpr (MODE == kExpandProduct32) {
+        store_product32(static_cast<float*>(p.out) + off + h * n8, acc, h, fac[h][0]);
+      } else {
+        uint4 o = expand_epilogue<MODE, BANKS>(acc, h, fac[h], bs[h]);
+        if (MODE == kExpandAdd && none[h]) o = bs[h][0];
+        *reinterpret_cast<uint4*>(static_cast<__half*>(p.out) + off + h * n8) = o;
+      }
     }
   }
 }
@@ -849,7 +884,7 @@ __global__ void __launch_bounds__(kAdThreads, expand_rows_min_blocks<RV, MODE>()
   const int gid[2] = {s.group[2 * tq], s.group[2 * tq + 1]};
   const bool none[2] = {s.adapter[2 * tq] < 0, s.adapter[2 * tq + 1] < 0};
   int i = first, grp = i / cols, c = cg0 + i % cols;
-  __half* out = p.out + row_off + c * 32;
+  __half* out = static_cast<__half*>(p.out) + row_off + c * 32;
   while (i < last) {
 #pragma unroll
     for (int u = 0; u < S; ++u) {
@@ -911,7 +946,7 @@ static int launch_expand(ExpandArgs p, cudaStream_t stream) {
   const long windows = (p.R + W - 1) / W;
   const int cgs = (p.N + 31) / 32;
   int gpc = consumers<MODE>();
-  if (MT == 1 || MODE == kExpandProduct) {
+  if (MT == 1 || is_product(MODE)) {
     // one wave of two blocks per SM where that leaves a warp 1 to 16 groups
     const long per = (windows * cgs + 2 * kTargetBlocks * 8 - 1) / (2 * kTargetBlocks * 8);
     gpc = int(per < 1 ? 1 : per > 16 ? 16 : per) * 8;
@@ -948,7 +983,7 @@ static int run_expand(const ExpandArgs& p, cudaStream_t stream) {
   constexpr int MT = MODE == kExpandSwiglu ? 2 : 4;
   const long blocks = (p.R + 16 * MT - 1) / (16 * MT) * ((p.N + 255) / 256);
   const bool small = blocks < 2 * kTargetBlocks;
-  if constexpr (MODE != kExpandProduct) {
+  if constexpr (!is_product(MODE)) {
     if (p.R <= kSmallRows)
       return p.r <= 16   ? launch_expand_rows<16, MODE>(p, stream)
              : p.r <= 32 ? launch_expand_rows<32, MODE>(p, stream)

@@ -10,6 +10,8 @@
 //   dl_e   = p_e (dp_e - sum_i p_i dp_i)              (f is a constant, as in the loss)
 //   dW     = dl^T h,  dh = dl W,  db = sum_t dl
 //   dy_row = w dout_t,  dw = <dout_t, y_row>,  dx_t = sum_j dpermuted[row_j]
+#include <type_traits>
+
 #include "lr_lowrank.cuh"
 
 namespace lr {
@@ -687,14 +689,25 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dh[T,d] = dl W, fp16 out, for more experts than the low-rank kernel takes (128).
+// A row gradient: rounded to fp16, or fp32 as it is.
+LR_DEVICE void store_dh(__half* to, float v) { *to = __float2half_rn(v); }
+LR_DEVICE void store_dh(float* to, float v) { *to = v; }
+LR_DEVICE void store_dh8(__half* to, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(to) = pack_half8(v);
+}
+LR_DEVICE void store_dh8(float* to, const float (&v)[8]) {
+  reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// dh[T,d] = dl W for more experts than the low-rank kernel takes (128).
 // fp32 gradients go in as two tf32 terms.  A warp owns MT*16 tokens x 64 columns; experts are
 // the k axis.  n-tile j takes column g*8 + j of the lane's 16-byte weight load,
 // so a lane ends with 16 neighbouring columns of its rows.
-template <int MT>
+template <int MT, typename DH>
 __global__ void __launch_bounds__(256)
     gate_dh_kernel(const float* __restrict__ dl, const __half* __restrict__ wg, int T, int d, int E,
-                   __half* __restrict__ dh) {
+                   DH* __restrict__ dh) {
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
@@ -746,7 +759,7 @@ __global__ void __launch_bounds__(256)
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = acc[m][j][2 * r + half_i];
-        if (c < d) *reinterpret_cast<uint4*>(dh + size_t(t) * d + c) = pack_half8(v);
+        if (c < d) store_dh8(dh + size_t(t) * d + c, v);
       }
     }
 }
@@ -758,10 +771,11 @@ __global__ void __launch_bounds__(256)
 constexpr int kSmallGateTokens = 256;
 constexpr int kSmallGateExperts = 64;
 
+template <typename DH>
 __global__ void __launch_bounds__(256)
     gate_backward_small_kernel(const __half* __restrict__ h, const __half* __restrict__ wg,
                                const float* __restrict__ dl, int T, int d, int E,
-                               __half* __restrict__ dh, float* __restrict__ dw,
+                               DH* __restrict__ dh, float* __restrict__ dw,
                                float* __restrict__ db) {
   extern __shared__ __align__(128) unsigned char s_dyn[];
   const int EP = (E + 3) & ~3;                       // zeros past E
@@ -798,7 +812,7 @@ __global__ void __launch_bounds__(256)
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (t0 + 4 * u < T) dh[size_t(t0 + 4 * u) * d + col] = __float2half_rn(acc[u]);
+        if (t0 + 4 * u < T) store_dh(dh + size_t(t0 + 4 * u) * d + col, acc[u]);
     }
   }
   if (dw && col < d) {
@@ -1086,9 +1100,11 @@ extern "C" size_t lr_gate_backward_workspace_bytes(int num_tokens, int d_model, 
   return gate_plan(num_tokens, d_model, num_experts).bytes;
 }
 
-extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d,
-                                int E, void* d_h, float* d_wg, float* d_bias, void* workspace,
-                                size_t workspace_bytes, lr_stream_t stream) {
+// DH: the type of d_h.
+template <typename DH>
+static int gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d, int E,
+                         void* d_h, float* d_wg, float* d_bias, void* workspace,
+                         size_t workspace_bytes, lr_stream_t stream) {
   if (T < 0 || T > kMaxRows || d <= 0 || d % 16 != 0 || d > kMaxColumns || E < 1 ||
       E > 256)
     return LR_ERR_INVALID_ARGUMENT;
@@ -1106,13 +1122,13 @@ extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_lo
     const int ep = (E + 3) & ~3;
     static unsigned long long configured = 0;
     if (const int rc = set_dyn_smem_once(
-            gate_backward_small_kernel,
+            gate_backward_small_kernel<DH>,
             (kSmallGateTokens + 64) * kSmallGateExperts * int(sizeof(float)), configured))
       return rc;
-    return launch_pdl(gate_backward_small_kernel, dim3((d + 63) / 64), dim3(256),
+    return launch_pdl(gate_backward_small_kernel<DH>, dim3((d + 63) / 64), dim3(256),
                       size_t(T + 64) * ep * sizeof(float), stream,
                       static_cast<const __half*>(h), static_cast<const __half*>(wg), d_logits, T,
-                      d, E, static_cast<__half*>(d_h), d_wg, d_bias);
+                      d, E, static_cast<DH*>(d_h), d_wg, d_bias);
   }
   const GatePlan gp = gate_plan(T, d, E);
   if (!workspace || !aligned16(workspace) || workspace_bytes < gp.bytes) return LR_ERR_WORKSPACE;
@@ -1141,19 +1157,20 @@ extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_lo
       ExpandArgs ep{};
       ep.v = d_logits;
       ep.b[0] = sp.wt;
-      ep.out = static_cast<__half*>(d_h);
+      ep.out = d_h;
       ep.R = T;
       ep.N = d;
       ep.n = 1;
       ep.r = E;
       ep.ldb = gp.E8;
-      if (const int rc = run_expand<kExpandProduct>(ep, stream)) return rc;
+      constexpr int kMode = std::is_same<DH, float>::value ? kExpandProduct32 : kExpandProduct;
+      if (const int rc = run_expand<kMode>(ep, stream)) return rc;
     } else {
       constexpr int MT = 2;
       const dim3 grid((T + 16 * MT - 1) / (16 * MT), (d + 511) / 512);
-      if (const int rc = launch_pdl(gate_dh_kernel<MT>, grid, dim3(256), 0, stream, d_logits,
+      if (const int rc = launch_pdl(gate_dh_kernel<MT, DH>, grid, dim3(256), 0, stream, d_logits,
                                     static_cast<const __half*>(wg), T, d, E,
-                                    static_cast<__half*>(d_h)))
+                                    static_cast<DH*>(d_h)))
         return rc;
     }
   }
@@ -1173,6 +1190,21 @@ extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_lo
                         static_cast<const float*>(sp.colsum), gp.chunks, E, gp.E8, d_bias);
   }
   return LR_OK;
+}
+
+extern "C" int lr_gate_backward(const void* h, const void* wg, const float* d_logits, int T, int d,
+                                int E, void* d_h, float* d_wg, float* d_bias, void* workspace,
+                                size_t workspace_bytes, lr_stream_t stream) {
+  return gate_backward<__half>(h, wg, d_logits, T, d, E, d_h, d_wg, d_bias, workspace,
+                               workspace_bytes, stream);
+}
+
+extern "C" int lr_gate_backward_rows32(const void* h, const void* wg, const float* d_logits, int T,
+                                       int d, int E, float* d_h, float* d_wg, float* d_bias,
+                                       void* workspace, size_t workspace_bytes,
+                                       lr_stream_t stream) {
+  return gate_backward<float>(h, wg, d_logits, T, d, E, d_h, d_wg, d_bias, workspace,
+                              workspace_bytes, stream);
 }
 
 extern "C" int lr_combine_backward(const void* d_out, const void* y, const float* gate_weights,

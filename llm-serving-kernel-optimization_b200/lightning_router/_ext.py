@@ -33,6 +33,7 @@ C_ABI_SYMBOLS = (
     "lr_grouped_w4a16_gemm", "lr_quantized_matmul",
     "lr_balanced_gating_workspace_bytes", "lr_balanced_gating", "lr_balanced_gating_backward",
     "lr_round_half", "lr_gate_backward_workspace_bytes", "lr_gate_backward",
+    "lr_gate_backward_rows32",
     "lr_dispatch_backward", "lr_combine_backward",
     "lr_adapter_workspace_bytes", "lr_adapter_add", "lr_adapter_swiglu", "lr_adapter_rows",
     "lr_ep_plan_size", "lr_ep_plan", "lr_ep_plan_tokens", "lr_ep_publish", "lr_ep_plan_wait",

@@ -13,9 +13,10 @@ kernels without atomics (the same inputs give the same bits).
 * :func:`combine_tokens` -- :func:`combine` with gradients for the experts' rows and the weights.
 
 Gradients follow the formulas of a loss in which the selection and the slot counts are
-constants, as in the Switch balance loss.  Row gradients are fp16 like the rows: scale the
-loss so that they stay in range.  Logit, weight and bias gradients are fp32.  Each function
-is differentiable once (``create_graph=True`` raises).
+constants, as in the Switch balance loss.  Gradients of fp16 rows are fp16: scale the loss so
+that they stay in range.  The gate's gradient of fp32 or bf16 hidden rows is rounded to their
+type alone.  Logit, weight and bias gradients are fp32.  Each function is differentiable once
+(``create_graph=True`` raises).
 """
 
 from __future__ import annotations
@@ -69,7 +70,8 @@ def gate_projection(hidden: torch.Tensor, gate_weight: torch.Tensor,
                     bias: torch.Tensor | None = None) -> torch.Tensor:
     """fp32 logits ``hidden @ gate_weight.T (+ bias)`` from operands rounded to fp16,
     differentiable in all three.  ``hidden`` (T, d) and ``gate_weight`` (E, d) of any
-    floating type (a gradient has its tensor's type); ``d % 16 == 0``, ``E <= 256``."""
+    floating type (a gradient has its tensor's type, rounded once from fp32 sums);
+    ``d % 16 == 0``, ``E <= 256``."""
     _ext.require_cuda(hidden, gate_weight, bias)
     return _ext.ops().gate_projection(hidden, gate_weight, bias)
 
