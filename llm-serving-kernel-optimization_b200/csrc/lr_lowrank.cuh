@@ -169,6 +169,15 @@ LR_DEVICE void group_rows(Groups& s, const int32_t* __restrict__ index, long row
 // Warps per group (a power of two) when g groups share the block's warps.
 LR_DEVICE int warps_per_group(int g) { return g <= 1 ? 8 : g <= 2 ? 4 : g <= 4 ? 2 : 1; }
 
+// Powers of two that take a largest finite value m into [2^14, 2^15) and back, both
+// normal numbers: 2^-113 to 2^126.  Below 2^-112 m stays under 2^14; two fp16 terms
+// then leave 2^-25 of 2^-126 over, less than fp32's own spacing.
+LR_DEVICE void half_range_scale(float m, float& up, float& down) {
+  const int ex = m > 0.f ? min(126, 141 - int(__float_as_uint(m) >> 23)) : 0;
+  up = __uint_as_float(unsigned(127 + ex) << 23);
+  down = __uint_as_float(unsigned(127 - ex) << 23);
+}
+
 // ---------------------------------------------------------------------------
 // expand: out[row] = base[row] + s_a v[row] . B_a^T   (or the SwiGLU of two)
 // ---------------------------------------------------------------------------
@@ -506,12 +515,8 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
         }
 #pragma unroll
       for (int o = 1; o < LPR; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      // 2^ex takes the row's largest finite value into [2^14, 2^15); both powers are
-      // normal numbers
-      int ex = 0;
-      if (m > 0.f) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
-      const float up = __uint_as_float(unsigned(127 + ex) << 23);
-      const float down = __uint_as_float(unsigned(127 - ex) << 23);
+      float up, down;
+      half_range_scale(m, up, down);
       uint32_t* hi = reinterpret_cast<uint32_t*>(s_v + 2 * bk * kTerm);
       uint32_t* lo = hi + 4 * kTerm;
 #pragma unroll
@@ -848,10 +853,8 @@ __global__ void __launch_bounds__(kAdThreads, expand_rows_min_blocks<RV, MODE>()
         }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      int ex = 0;
-      if (m > 0.f) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
-      const float up = __uint_as_float(unsigned(127 + ex) << 23);
-      const float down = __uint_as_float(unsigned(127 - ex) << 23);
+      float up, down;
+      half_range_scale(m, up, down);
 #pragma unroll
       for (int i = 0; i < EL; ++i) {
         const int c = 2 * (i * 32 + lane);

@@ -494,10 +494,9 @@ __global__ void __launch_bounds__(256) gate_split_kernel(SplitArgs p) {
     __syncthreads();
     if (q == 0) {
       m = fmaxf(fmaxf(s_red[0][e], s_red[1][e]), fmaxf(s_red[2][e], s_red[3][e]));
-      int ex = 0;
-      if (m > 0.f) ex = max(-100, min(100, 141 - int(__float_as_uint(m) >> 23)));
-      s_up[e] = __uint_as_float(unsigned(127 + ex) << 23);
-      if (e < ne8) p.down[size_t(chunk) * p.E8 + e0 + e] = __uint_as_float(unsigned(127 - ex) << 23);
+      float down;
+      half_range_scale(m, s_up[e], down);
+      if (e < ne8) p.down[size_t(chunk) * p.E8 + e0 + e] = down;
     }
     __syncthreads();
     s_red[q][e] = sum;
