@@ -308,7 +308,7 @@ int lr_dispatch_backward(const void* d_permuted, const int32_t* slot_pos, int T,
  * d_y[slot_pos[s],:] = fp16(gate_weights[s] * d_out[t,:]), d_weights[s] =
  * <d_out[t,:], y[slot_pos[s],:]> in fp32 (0 for a dropped slot); the rows of
  * d_y that no slot keeps (past kept_counts in each segment of offsets) are
- * zero.  d % 8 == 0.                                                        */
+ * zero.  d_y and d_weights are each nullable.  d % 8 == 0.                   */
 int lr_combine_backward(const void* d_out, const void* y, const float* gate_weights,
                         const int32_t* slot_pos, const int32_t* offsets,
                         const int32_t* kept_counts, int T, int k, int d, int E, void* d_y,

@@ -276,14 +276,14 @@ struct DispatchTokens : public torch::autograd::Function<DispatchTokens> {
     const int64_t k = ctx->saved_data["k"].toInt(), d = ctx->saved_data["d"].toInt();
     const double lbw = ctx->saved_data["lbw"].toDouble();
     at::Tensor dx, dl;
-    if (grads[2].defined()) {
+    if (grads[2].defined() && ctx->needs_input_grad(0)) {
       const at::Tensor dp = rows16(grads[2], at::kHalf);
       dx = at::empty({T, d}, dp.options());
       check_status(lr_dispatch_backward(dp.data_ptr(), saved[3].data_ptr<int32_t>(), as_int(T),
                                         as_int(k), as_int(d), dx.data_ptr(), cur_stream()),
                    "dispatch_tokens (backward)");
     }
-    if (grads[0].defined() || grads[1].defined()) {
+    if ((grads[0].defined() || grads[1].defined()) && ctx->needs_input_grad(1)) {
       const at::Tensor dw = grads[0].defined() ? grads[0].contiguous() : grads[0];
       const at::Tensor da = grads[1].defined() ? grads[1].contiguous() : grads[1];
       dl = at::empty_like(logits);
@@ -349,15 +349,18 @@ struct CombineTokens : public torch::autograd::Function<CombineTokens> {
     const int64_t k = ctx->saved_data["k"].toInt();
     const int64_t S = y.size(0), d = y.size(1), E = saved[4].numel();
     const at::Tensor dout = rows16(grads[0], at::kHalf);
-    auto dy = at::empty({S, d}, y.options());
-    auto dw = at::empty({S}, w.options());
+    const bool need_y = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    at::Tensor dy, dw;
+    if (need_y) dy = at::empty({S, d}, y.options());
+    if (need_w) dw = at::empty({S}, w.options());
     check_status(lr_combine_backward(dout.data_ptr(), y.data_ptr(), w.data_ptr<float>(),
                                      saved[2].data_ptr<int32_t>(), saved[3].data_ptr<int32_t>(),
                                      saved[4].data_ptr<int32_t>(), as_int(S / k), as_int(k),
-                                     as_int(d), as_int(E), dy.data_ptr(), dw.data_ptr<float>(),
-                                     cur_stream()),
+                                     as_int(d), as_int(E), need_y ? dy.data_ptr() : nullptr,
+                                     need_w ? dw.data_ptr<float>() : nullptr, cur_stream()),
                  "combine_tokens (backward)");
-    return {dy, dw.view(w.sizes()), {}, {}, {}, {}};
+    if (need_w) dw = dw.view(w.sizes());
+    return {dy, dw, {}, {}, {}, {}};
   }
 };
 

@@ -910,8 +910,9 @@ static int launch_dw(const __half* h, const uint4* frag, const float* down, int 
 // WPT warps share a token's row: the row of dout is read once, each kept slot's
 // y row once, dy written once; the dot products are summed over lanes and warps
 // in a fixed order.  Rows no slot keeps (the tail of an over-full expert's
-// segment) are zero-filled by the warps of the tokens with the same numbers.
-template <int WPT>
+// segment) are zero-filled by the warps of the tokens with the same numbers.  With
+// one of the two gradients alone (frozen experts: DW) the other's bytes stay away.
+template <int WPT, bool DY, bool DW>
 __global__ void __launch_bounds__(256)
     combine_backward_kernel(const uint4* __restrict__ dout, const uint4* __restrict__ y,
                             const float* __restrict__ gate_w, const int32_t* __restrict__ slot_pos,
@@ -956,7 +957,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const int c = c0 + u * 32 + lane;
-            if (c < d8) v[u] = ld_stream(y + size_t(pos[j]) * d8 + c);
+            if (DW && c < d8) v[u] = ld_stream(y + size_t(pos[j]) * d8 + c);
           }
 #pragma unroll
           for (int u = 0; u < U; ++u) {
@@ -967,20 +968,23 @@ __global__ void __launch_bounds__(256)
               float o[8];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float2 a = __half22float2(gh[i]), b = __half22float2(vh[i]);
-                dot[j] = fmaf(a.x, b.x, dot[j]);
-                dot[j] = fmaf(a.y, b.y, dot[j]);
+                const float2 a = __half22float2(gh[i]);
+                if (DW) {
+                  const float2 b = __half22float2(vh[i]);
+                  dot[j] = fmaf(a.x, b.x, dot[j]);
+                  dot[j] = fmaf(a.y, b.y, dot[j]);
+                }
                 o[2 * i] = w[j] * a.x;
                 o[2 * i + 1] = w[j] * a.y;
               }
-              dy[size_t(pos[j]) * d8 + c] = pack_half8(o);
+              if (DY) dy[size_t(pos[j]) * d8 + c] = pack_half8(o);
             }
           }
         }
       }
     }
     // rows that no slot keeps
-    for (int j = 0; j < k; ++j) {
+    for (int j = 0; DY && j < k; ++j) {
       const long r = t * k + j;
       bool drop = false;
       for (int e = lane; e < E; e += 32)
@@ -992,6 +996,7 @@ __global__ void __launch_bounds__(256)
       }
     }
   }
+  if (!DW) return;
 #pragma unroll
   for (int j = 0; j < kMaxTopK; ++j) {
     if (j < k) {
@@ -1213,7 +1218,7 @@ extern "C" int lr_combine_backward(const void* d_out, const void* y, const float
   if (T < 0 || k < 1 || k > kMaxTopK || long(T) * k > kMaxRows || d <= 0 || d % 8 != 0 || E < 1)
     return LR_ERR_INVALID_ARGUMENT;
   if (T == 0) return LR_OK;
-  if (!d_out || !y || !gate_weights || !slot_pos || !offsets || !kept_counts || !d_y || !d_weights)
+  if (!d_out || !y || !gate_weights || !slot_pos || !offsets || !kept_counts)
     return LR_ERR_INVALID_ARGUMENT;
   if (!aligned16(d_out) || !aligned16(y) || !aligned16(d_y)) return LR_ERR_INVALID_ARGUMENT;
   const int d8 = d / 8;
@@ -1224,5 +1229,13 @@ extern "C" int lr_combine_backward(const void* d_out, const void* y, const float
                       slot_pos, offsets, kept_counts, E, T, k, d8, static_cast<uint4*>(d_y),
                       d_weights);
   };
-  return T < 2368 ? run(combine_backward_kernel<8>, 8) : run(combine_backward_kernel<1>, 1);
+  if (!d_y && !d_weights) return LR_OK;
+  if (!d_y)
+    return T < 2368 ? run(combine_backward_kernel<8, false, true>, 8)
+                    : run(combine_backward_kernel<1, false, true>, 1);
+  if (!d_weights)
+    return T < 2368 ? run(combine_backward_kernel<8, true, false>, 8)
+                    : run(combine_backward_kernel<1, true, false>, 1);
+  return T < 2368 ? run(combine_backward_kernel<8, true, true>, 8)
+                  : run(combine_backward_kernel<1, true, true>, 1);
 }
