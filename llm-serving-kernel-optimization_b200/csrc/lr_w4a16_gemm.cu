@@ -54,6 +54,12 @@ constexpr int kGemmThreads = (kMmaWarp + 1) * 32;
 // accumulator takes MT * WN TMEM columns; it is double buffered when two fit
 // in the 512 columns of an SM, otherwise the epilogue of a tile and the main
 // loop of the next one take turns.
+constexpr int least_common_multiple(int a, int b) {
+  int m = a;
+  while (m % b != 0) m += a;
+  return m;
+}
+
 template <int TOKROWS_, int MT_, int WN_, int STAGES_, int DSTAGES_, int DGROUPS_>
 struct GemmShape {
   static constexpr int TOKROWS = TOKROWS_, MT = MT_, WN = WN_, STAGES = STAGES_,
@@ -74,7 +80,12 @@ struct GemmShape {
   static constexpr int offB = offA + STAGES * kAStage;
   static constexpr int offW = offB + DSTAGES * kBBuf;
   static constexpr int offBar = offW + STAGES * kWStage;
-  static constexpr int kNumBars = 4 * STAGES + DSTAGES + 4 + 1;
+  // "Words loaded" barriers: k-step it uses it % WBARS, so that one dequant group sees
+  // every phase of a barrier.  With one per stage, a stage passes from group to group
+  // (3 stages, 2 groups), and a group whose own words landed before the other's could
+  // ask for a phase while the one before was incomplete: its parity reads as complete.
+  static constexpr int WBARS = least_common_multiple(STAGES, DGROUPS);
+  static constexpr int kNumBars = 3 * STAGES + WBARS + DSTAGES + 4 + 1;
   static constexpr int offMisc = offBar + kNumBars * 8;
   static constexpr int offTab = offMisc + 8 * 4;
   static constexpr int kTabBytes = (kMaxGemmExperts * 4 + 1) * 4;
@@ -117,8 +128,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   uint32_t* sW = reinterpret_cast<uint32_t*>(smem + S::offW);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::offBar);  // token stage loaded
   uint64_t* empty = full + STAGES;    // token stage released by the MMA
-  uint64_t* wfull = empty + STAGES;   // packed-weight stage loaded
-  uint64_t* wempty = wfull + STAGES;  // packed-weight stage read by its dequant group
+  uint64_t* wfull = empty + STAGES;   // packed-weight stage loaded (WBARS of them)
+  uint64_t* wempty = wfull + S::WBARS;  // packed-weight stage read by its dequant group
   uint64_t* dfull = wempty + STAGES;
   uint64_t* tfull = dfull + DSTAGES;
   uint64_t* tempty = tfull + 2;
@@ -139,9 +150,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
-      mbar_init(&wfull[i], 1);
       mbar_init(&wempty[i], kDeqWarps / DGROUPS);
     }
+    for (int i = 0; i < S::WBARS; ++i) mbar_init(&wfull[i], 1);
     for (int i = 0; i < DSTAGES; ++i) mbar_init(&dfull[i], kDeqWarps / DGROUPS);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
@@ -233,10 +244,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&wfull[s], uint32_t(S::kWStage));
+          uint64_t* loaded = &wfull[it % S::WBARS];
+          mbar_arrive_expect_tx(loaded, uint32_t(S::kWStage));
           uint32_t* w = sW + s * (S::kWStage / 4);
-          tma_load_2d(w, wmap0, &wfull[s], n0 / 8, kb * kBK);
-          if (kGLU) tma_load_2d(w + S::kWStage / 8, wmap1, &wfull[s], n0 / 8, kb * kBK);
+          tma_load_2d(w, wmap0, loaded, n0 / 8, kb * kBK);
+          if (kGLU) tma_load_2d(w + S::kWStage / 8, wmap1, loaded, n0 / 8, kb * kBK);
         }
       }
       // Weight stages are released by ordinary arrivals of the dequant warps,
@@ -245,7 +257,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       // CTA exits.
       (void)ok;
       const int first = it - STAGES < 0 ? 0 : it - STAGES;
-      for (int i = first; i < it; ++i) wait_drain(&wfull[i % STAGES], (i / STAGES) & 1);
+      for (int i = first; i < it; ++i) wait_drain(&wfull[i % S::WBARS], (i / S::WBARS) & 1);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ MMA issue
@@ -395,10 +407,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         uint32_t zw_next = zw;
         if (kb + DGROUPS < KB) load_params(kb + DGROUPS, sc_next, zw_next);
         const int s = it % STAGES;
-        const uint32_t ph = (it / STAGES) & 1;
         const int q = it % DSTAGES;
         const int prev = it - DSTAGES;  // last k-step that used buffer q
-        if (!wait_any(&wfull[s], ph, s_abort, err) ||
+        if (!wait_any(&wfull[it % S::WBARS], (it / S::WBARS) & 1, s_abort, err) ||
             (prev >= 0 &&
              !wait_any(&empty[prev % STAGES], (prev / STAGES) & 1, s_abort, err))) {
           ok = false;
