@@ -409,12 +409,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int s = it % STAGES;
         const int q = it % DSTAGES;
         const int prev = it - DSTAGES;  // last k-step that used buffer q
-        if (!wait_any(&wfull[it % S::WBARS], (it / S::WBARS) & 1, s_abort, err) ||
-            (prev >= 0 &&
-             !wait_any(&empty[prev % STAGES], (prev / STAGES) & 1, s_abort, err))) {
-          ok = false;
-          break;
-        }
+        // Lanes may differ in whether they saw a phase complete or the abort first: one
+        // whose wait ran out stays in step with its warp to the end of the tile, and waits
+        // and (lane 0) arrives no more.  The tile is then as wrong as the error word says.
+        ok = ok && wait_any(&wfull[it % S::WBARS], (it / S::WBARS) & 1, s_abort, err) &&
+             (prev < 0 || wait_any(&empty[prev % STAGES], (prev / STAGES) & 1, s_abort, err));
         const uint32_t* w = sW + s * (S::kWStage / 4);
         DeqParams P;
         deq_params(zw, sc, P);
@@ -441,13 +440,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         // every packed word of the stage has been read and used: release it
         // to the weight producer before the operand buffer is published
         __syncwarp();
-        if (lane == 0) mbar_arrive(&wempty[s]);
+        if (lane == 0 && ok) mbar_arrive(&wempty[s]);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&dfull[q]);
+        if (lane == 0 && ok) mbar_arrive(&dfull[q]);
         sc = sc_next;
         zw = zw_next;
       }
+      ok = __all_sync(0xffffffffu, ok) != 0;  // the warp leaves together
     }
   } else {
     // ------------------------------------------------------------ epilogue

@@ -366,18 +366,23 @@ __global__ void __maxnreg__(112)
     if (nx_group < n_groups) load_params(nx_group, nx_sc, nx_zw);
   };
 
+  // Lanes may differ in whether they saw a stage arrive or the abort first: one whose
+  // wait ran out (at k-step `stop`) stays in step with its warp to the end, waits and
+  // refills no more, and the CTA's result is dropped.  (4096 x 4096, groups of 32: 1
+  // to 8 rows 39.8 us, 39.6 when such lanes left alone; 64 rows 50.5, 49.6; a vote of
+  // the warp at every wait 41.1 and 50.1; lane 0 waiting for its warp 44.0 and 55.1.)
   bool ok = true;
-  int kb = 0;
+  int stop = KB;
   // The k loop, specialised on the live token tiles (fixed for the CTA) and on
   // whether a stage lies in one group (group size >= 64), so that a stage's
   // slices are straight-line code the compiler can interleave.
   auto main_loop = [&](auto ntu_c, auto one_group_c) {
     constexpr bool kOneGroup = decltype(one_group_c)::value;
-    for (; kb < KB; ++kb) {
+    for (int kb = 0; kb < KB; ++kb) {
       const int s = kb % STAGES;
-      if (!wait_any(&full[s], (kb / STAGES) & 1, s_abort, err)) {
+      if (ok && !wait_any(&full[s], (kb / STAGES) & 1, s_abort, err)) {
         ok = false;
-        break;
+        stop = kb;
       }
       const uint32_t base = smem_u32(smem + s * S::kStageBytes);
       if (kOneGroup) enter_group((4 * kb) >> gsh);
@@ -388,7 +393,7 @@ __global__ void __maxnreg__(112)
       }
       // the last warp done with this slot refills it with the stage STAGES ahead
       __syncwarp();
-      if (lane == 0) {
+      if (lane == 0 && ok) {
         if (atom_add_acq_rel(&done[s], 1u) == uint32_t(S::kConsumers - 1)) {
           done[s] = 0;
           if (kb + STAGES < KB) {
@@ -411,7 +416,8 @@ __global__ void __maxnreg__(112)
   if (!ok && lane == 0) {
     // a wait ran out: let the copies in flight on this warp's slots land before exit
     const int last = *reinterpret_cast<volatile int*>(s_issued);
-    for (int i = kb; i < last && i < kb + STAGES; ++i) wait_drain(&full[i % STAGES], (i / STAGES) & 1);
+    for (int i = stop; i < last && i < stop + STAGES; ++i)
+      wait_drain(&full[i % STAGES], (i / STAGES) & 1);
   }
 
   // ---------------------------------------------------------------- epilogue

@@ -47,3 +47,17 @@ def test_whole_warp_waits_use_it(name):
 def test_cluster_barrier_gathers_the_warp():
     body = _body(_code("lr_lowrank.cuh"), "void cluster_sync()")
     assert body.index("__syncwarp()") < body.index("barrier.cluster.arrive")
+
+
+@pytest.mark.parametrize("name,loop", [("lr_w4a16_gemm.cu", "for (; kb < KB; kb += DGROUPS)"),
+                                       ("lr_w4a16_skinny.cu", "for (int kb = 0; kb < KB; ++kb) {")])
+def test_gemm_lanes_stay_in_step(name, loop):
+    """The loops of whole warps in the GEMMs take no vote at each wait: a lane whose wait ran out
+    goes on to the end with the others, so none leaves ahead of mma.sync or __syncwarp, and its
+    warp's lane 0 arrives only while its own waits held."""
+    code = _code(name)
+    body = _body(code, loop)
+    assert "wait_any(" in body and "__syncwarp" in body
+    assert "break" not in body and "return" not in body
+    assert len(re.findall(r"if \(lane == 0\)", body)) == 0
+    assert "if (lane == 0 && ok)" in body
