@@ -63,3 +63,69 @@ def test_concurrent_products(M):
         torch.cuda.synchronize()
         for n, o in enumerate(got):
             assert torch.equal(o, want[(i + n) % 3]), (i, n)
+
+
+@pytest.mark.parametrize("R,requests,K,N,n,r", [
+    (9600, 2, 256, 1544, 2, 8), (4099, 11, 512, 2056, 7, 32), (1111, 9, 2048, 1408, 6, 64),
+    (200, 50, 520, 4104, 33, 16), (700, 700, 264, 264, 30, 128)])
+def test_concurrent_adapters(R, requests, K, N, n, r):
+    from lightning_router import _ext
+    from lightning_router.kernels.adapters import AdapterBank, adapter_add, adapter_swiglu
+    g = torch.Generator(device=DEV).manual_seed(R)
+
+    def half(*s, std=1.0):
+        return (torch.randn(*s, generator=g, device=DEV) * std).half()
+    bank = AdapterBank(half(n, r, K, std=K ** -0.5), half(n, N, r, std=0.2))
+    sets = []
+    for _ in range(3):
+        ids = torch.randint(-1, n, (requests,), generator=g, device=DEV, dtype=torch.int32)
+        sets.append((half(R, N), half(R, N), half(R, K),
+                     ids.repeat_interleave(-(-R // requests))[:R].contiguous()))
+
+    def both(base, up, x, ids):
+        return (adapter_add(base, x, bank, ids),
+                adapter_swiglu(base, up, x, bank, bank, ids))
+    want = []
+    for s in sets:
+        want.append(both(*s))
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(60):
+        got = []
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append(both(*sets[(i + k) % 3]))
+        torch.cuda.synchronize()
+        for k, o in enumerate(got):
+            assert all(torch.equal(a, b) for a, b in zip(o, want[(i + k) % 3])), (i, k)
+    _ext.check_device_errors()
+
+
+@pytest.mark.parametrize("T,d,E,k", [(64, 256, 8, 2), (777, 2048, 64, 6), (4000, 1024, 24, 4)])
+def test_concurrent_training_steps(T, d, E, k):
+    from lightning_router.kernels.routing_grad import (balanced_gating, combine_tokens,
+                                                       dispatch_tokens, gate_projection)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    w = torch.randn(E, d, generator=g, device=DEV) * 0.05
+    sets = [torch.randn(T, d, generator=g, device=DEV).half() for _ in range(3)]
+
+    def step(x):
+        leaf, weight = x.clone().requires_grad_(), w.clone().requires_grad_()
+        logits = gate_projection(leaf, weight)
+        plan = dispatch_tokens(leaf, logits, k, 0.9)
+        out = combine_tokens(plan.permuted, plan.gate_weights, plan)
+        loss = (out.float() ** 2).sum() / T + plan.aux_loss + balanced_gating(logits, k).aux_loss
+        return torch.autograd.grad(loss, (leaf, weight))
+    want = []
+    for x in sets:
+        want.append(step(x))
+        torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(30):
+        got = []
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append(step(sets[(i + n) % 3]))
+        torch.cuda.synchronize()
+        for n, o in enumerate(got):
+            assert all(torch.equal(a, b) for a, b in zip(o, want[(i + n) % 3])), (i, n)
