@@ -72,10 +72,13 @@ def adapter_index(index: torch.Tensor) -> torch.Tensor:
     """Adapter numbers of any integer type as contiguous int32."""
     if index.dtype == torch.int32 and index.dim() == 1 and index.is_contiguous():
         return index
-    if index.dtype.is_floating_point or index.dtype == torch.bool:
+    if index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
         raise ValueError(f"adapter numbers must be integers, got {index.dtype}")
     if index.dtype in (torch.int64, torch.uint32, torch.uint64):
-        index = index.to(torch.int64).clamp(-2, 2**31 - 1)  # out of range stays out of range
+        wide = index.to(torch.int64)
+        if index.dtype == torch.uint64:     # from 2^63 on: negative now, and not "none"
+            wide = torch.where(wide < 0, 2**31 - 1, wide)
+        index = wide.clamp(-2, 2**31 - 1)   # out of range stays out of range
     return index.reshape(-1).to(torch.int32).contiguous()
 
 
