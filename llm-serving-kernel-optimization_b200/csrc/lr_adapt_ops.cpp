@@ -429,11 +429,6 @@ void check_out(const at::Tensor& out, const at::Tensor& x, int64_t N,
   }
 }
 
-// Kernels write through raw pointers: a graph that saved `t` learns of it here.
-void written(const at::Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
 void check_index(const at::Tensor& index, const at::Tensor& x) {
   TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.scalar_type() == at::kHalf,
               "x: a CUDA tensor (R,K) fp16 expected");

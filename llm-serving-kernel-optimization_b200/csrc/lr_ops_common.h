@@ -41,4 +41,9 @@ inline at::Tensor workspace(size_t bytes, const at::Tensor& like) {
                    like.options().dtype(at::kByte));
 }
 
+// Kernels write through raw pointers: a graph that saved `t` learns of it here.
+inline void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 }  // namespace lr_ops

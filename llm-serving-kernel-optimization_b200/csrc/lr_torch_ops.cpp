@@ -359,6 +359,7 @@ at::Tensor grouped_w4a16_gemm(const at::Tensor& table, int64_t num_experts, int6
                                      wsb ? ws.data_ptr() : nullptr, wsb, err_ptr(err),
                                      cur_stream()),
                "grouped_w4a16_gemm");
+  if (out.has_value() && out->defined()) written(C);
   return C;
 }
 
@@ -562,7 +563,7 @@ TORCH_LIBRARY(lightning_router, m) {
       "num_experts, int d_model, int d_ff, int group_size, bool gated) -> Tensor");
   m.def(
       "grouped_w4a16_gemm(Tensor table, int num_experts, int mode, int mat, Tensor A, int N, "
-      "int group_size, Tensor? seg_start, Tensor? seg_len, int max_rows, Tensor? out, "
+      "int group_size, Tensor? seg_start, Tensor? seg_len, int max_rows, Tensor(a!)? out, "
       "Tensor? err, bool int8_operands=True) -> Tensor");
   m.def(
       "route_rows(Tensor expert_ids, Tensor gate_weights, Tensor row_offsets, Tensor(a!) "
