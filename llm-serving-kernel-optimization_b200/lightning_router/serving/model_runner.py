@@ -97,19 +97,20 @@ class LightningModelRunner:
         key = (num_tokens, d, True) if adapters else (num_tokens, d)
         ids = torch.full((num_tokens,), -1, dtype=torch.int32, device=self.device) \
             if adapters else None
+        kw = {} if ids is None else {"adapter_ids": ids}   # a layer may know of none
         x = torch.zeros(num_tokens, d, dtype=torch.float16, device=self.device)
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(side):
             for _ in range(max(1, warmup)):
-                layer(x, adapter_ids=ids)
+                layer(x, **kw)
         torch.cuda.current_stream(self.device).wait_stream(side)
         torch.cuda.synchronize(self.device)
         if self._pool is None:
             self._pool = torch.cuda.graph_pool_handle()
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g, pool=self._pool):
-            out, aux = layer(x, adapter_ids=ids)
+            out, aux = layer(x, **kw)
         self._graphs[key] = _Graph(g, x, out, aux, ids, layer.adapters if adapters else None)
 
     @torch.inference_mode()
@@ -127,7 +128,7 @@ class LightningModelRunner:
         if gr is not None and gr.ids is not None and not gr.reads(layer.adapters):
             gr = None   # captured with adapters that the layer no longer has, or has elsewhere
         if gr is None:
-            out, _ = layer(h, adapter_ids=adapter_ids)
+            out, _ = layer(h) if adapter_ids is None else layer(h, adapter_ids=adapter_ids)
             return out.view(shape).to(hidden_states.dtype)
         if adapter_ids is not None:
             from lightning_router.kernels.adapters import adapter_index
