@@ -264,7 +264,7 @@ int lr_quantized_matmul(const void* device_table, const void* A, int M, int K, i
  * token_mask[T] (nullable; bytes, 0 = padding): a padded token keeps valid ids,
  * gets weight 0 and enters neither counts nor loss, whatever its logits hold
  * (NaN included).  n = 0 gives a loss of 0.  T = 0 is accepted.
- * Limits: E <= 64, 1 <= k <= min(E, 8).                                    */
+ * Limits: E <= 64, 1 <= k <= min(E, 8); workspace 16-byte aligned.           */
 size_t lr_balanced_gating_workspace_bytes(int num_tokens, int num_experts);
 int lr_balanced_gating(const float* logits, const uint8_t* token_mask, int T, int E, int k,
                        float load_balance_weight, int32_t* expert_ids, float* gate_weights,
@@ -324,8 +324,8 @@ int lr_combine_backward(const void* d_out, const void* y, const float* gate_weig
  *   swiglu: out = silu(gate + delta_gate) * (up + delta_up)
  * out may be base (gate or up) itself: rows without an adapter are then left
  * alone by add.  A row's result depends on its own adapter only.
- * Limits: K, N and rank multiples of 8, rank <= 128; x, a, b, base, gate, up
- * and out 16-byte aligned.  num_banks is 1 for add and 2 for swiglu.          */
+ * Limits: K, N and rank multiples of 8, rank <= 128; x, a, b, base, gate, up,
+ * out and workspace 16-byte aligned.  num_banks is 1 for add and 2 for swiglu.          */
 size_t lr_adapter_workspace_bytes(int num_rows, int rank, int num_banks);
 int lr_adapter_add(const void* x, int R, int K, const int32_t* index, int num_adapters,
                    const void* a, const void* b, const float* scale, int rank, int N,

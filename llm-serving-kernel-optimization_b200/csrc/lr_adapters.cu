@@ -473,6 +473,7 @@ extern "C" int lr_adapter_add(const void* x, int R, int K, const int32_t* index,
     return LR_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < lr_adapter_workspace_bytes(R, rank, 1))
     return LR_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return LR_ERR_INVALID_ARGUMENT;
   ShrinkArgs sp{static_cast<const __half*>(x), {static_cast<const __half*>(a), nullptr}, index,
                 static_cast<float*>(workspace), R, K, num_adapters, rank, err};
   if (const int rc = run_shrink(sp, 1, stream)) return rc;
@@ -495,6 +496,7 @@ extern "C" int lr_adapter_swiglu(const void* x, int R, int K, const int32_t* ind
     return LR_ERR_INVALID_ARGUMENT;
   if (!workspace || workspace_bytes < lr_adapter_workspace_bytes(R, rank, 2))
     return LR_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return LR_ERR_INVALID_ARGUMENT;
   ShrinkArgs sp{static_cast<const __half*>(x),
                 {static_cast<const __half*>(a_gate), static_cast<const __half*>(a_up)}, index,
                 static_cast<float*>(workspace), R, K, num_adapters, rank, err};

@@ -1048,6 +1048,7 @@ extern "C" int lr_balanced_gating(const float* logits, const uint8_t* token_mask
   if (B > 1) {
     if (!workspace || workspace_bytes < lr_balanced_gating_workspace_bytes(T, E))
       return LR_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return LR_ERR_INVALID_ARGUMENT;  // it starts with doubles
     parts.psum = static_cast<double*>(workspace);
     parts.count = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) +
                                              align256(size_t(B) * E * sizeof(double)));
