@@ -9,9 +9,8 @@
 // window's rows are grouped by adapter inside the block (no sort of the batch,
 // no host involvement), and the block's 8 warps are dealt out to its groups:
 // one group (a prompt's rows) gets all warps, eight groups (decode) a warp each.
-// Work is bound by memory: a row costs 2 (K + 2N) bytes and 2 r (K + N)
-// operations, so mma.sync with fragments loaded straight into registers keeps
-// up and needs no staging through shared memory.
+// The floor is memory: a row costs 2 (K + 2N) bytes and 2 r (K + N) operations.
+// mma.sync keeps up with that (its pipe is 22 to 32 % busy in the large batches).
 #include "lr_lowrank.cuh"
 
 namespace lr {
@@ -191,10 +190,11 @@ __global__ void __launch_bounds__(kAdThreads) adapter_shrink_kernel(ShrinkArgs p
 // The groups of a window that up to three requests share go to the two blocks of
 // the grid's z (one of them leaves at once otherwise: its slot is free while the
 // others stream); a window of more groups takes its halves through shrink_groups.
-// 16384 x 4096, rank 32: 44 us (x alone is 21 us of HBM; A, read again by every
-// window, is half as much from L2); 49 us where requests meet inside windows.
-// Bulk copies of these 256-byte rows took 127 us: the copy engine needs 25 to 30 ns
-// for each, whatever its size.
+// 16384 x 4096, rank 32: 36 to 44 us (x alone is 21 us of HBM; A, read again by every
+// window, is half as much from L2); 49 us where requests meet inside windows.  A bulk
+// copy for each of these 256-byte rows took 127 us; a tensor map that moves a whole
+// tile was not tried.  Registers (128, a few bytes spilled) and 256 working blocks on
+// 296 places hold it where it is: HBM at 48 %, issue slots at 40 %.
 constexpr int kTileK = 128;
 constexpr int kTileKPitch = kTileK * 2 + 64;  // bytes; neighbouring rows in different banks
 

@@ -189,9 +189,9 @@ LR_DEVICE void half_range_scale(float m, float& up, float& down) {
 // stands for output column (c >> 1) * 8 + 2 j + (c & 1) of the warp's 32: a lane
 // ends with 8 neighbouring columns of its two rows, one 16-byte read of the base
 // and one store each.
-// 16384 x 14336, rank 32: 182 us, 5.2 TB/s of base in and out (floor 143); the
-// instructions around 16 rows x 32 columns (16 of them mma, 44 to convert, add,
-// round) and the power cap's clock keep it from the rest.
+// 16384 x 14336, rank 32: 175 to 190 us, 5 TB/s of base in and out (floor 143), HBM
+// 64 % and the tensor pipe 32 % busy; of the 126 instructions around 16 rows x 32
+// columns 16 are mma and 44 convert, add and round, under the power cap's clock.
 // Largest sizes taken: row numbers plus a tile, and 64 rows' offsets, stay in 32 bits.
 constexpr int kMaxRows = 0x7fffffff - 1023;
 constexpr int kMaxColumns = 1 << 26;
@@ -750,7 +750,8 @@ __global__ void __launch_bounds__(kAdThreads, expand_min_blocks<RV, MT, MODE>())
 // products of a tile of 16 rows, of which a request has one or two; rows of other
 // requests are multiplied too and not stored.  A lane ends with 4 neighbouring
 // columns of rows 2 tq and 2 tq + 1.  Against 16-row tiles with every group in
-// every warp, a pass with shrink: 64 rows of 64 adapters of rank 16, N 14336, 15.5
+// every warp, a pass with shrink outside graphs (in a captured one, whose launches
+// carry no programmatic edge, 17 and 33 us): 64 rows of 64 adapters of rank 16, N 14336, 15.5
 // us (15.9), of rank 32 21.6 (27); 128 expert rows of SwiGLU pairs 31.5 (32.2), in
 // neighbouring pairs 25.3 (27.2); one token, 4096 x 4096, rank 64, 7.5 (8.6).
 // Powers of two of warps to a group left warps idle: 33.7 for the expert rows.

@@ -25,9 +25,9 @@ namespace lr {
 // first) keys.  Probability sums and counts stay in registers over a lane's
 // tokens, go through shuffles and shared memory to one partial per block and
 // expert, and are summed over blocks in double in block order: no atomics.
-// Latency bounds it: 262144 tokens x 8 experts take 10 us (12.6 MB, 2 us of HBM)
-// and 8192 x 64 top-6 takes 8, of which the selection's shuffles are most; one
-// thread per token with 64 experts in registers took 60 at 777 tokens.
+// 262144 tokens x 8 experts take 10 us (12.6 MB, 2 us of HBM: a warp has no loads in
+// flight ahead of its next round, of which it has one or two) and 8192 x 64 top-6
+// takes 8; one thread per token with 64 experts in registers took 60 at 777 tokens.
 constexpr int kGateThreads = 512;
 constexpr int kGateBlocksMax = 296;  // 2 per SM
 
@@ -538,9 +538,11 @@ LR_DEVICE void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t saddr) {
 
 // A block: 256 columns of h, up to 64 experts (blockIdx.z), a range of chunks.
 // Stages of 64 tokens (rows of h and dl fragments) come in by cp.async, three
-// deep.  Reading h bounds it with 8 experts (16384 x 4096: 24 us, 5.5 TB/s), the
-// shared-memory reads of 2 x 64 gradient rows with 64 (8111 x 2048: 21 us).  tf32
-// products of the unsplit gradients took 38 and 117 us.
+// deep.  Reading h bounds it with 8 experts (16384 x 4096: 24 us, 5.5 TB/s).  With 64
+// (8111 x 2048: 21 us, 5 of HBM) 252 registers leave 8 warps on an SM, each of which
+// reads all fragments of the 2 x 64 gradient rows from shared memory; the tensor pipe
+// is 34 % busy.  tcgen05 (M = 128 fits) was not tried.  tf32 products of the unsplit
+// gradients took 38 and 117 us.
 template <int MTL>
 __global__ void __launch_bounds__(256)
     gate_dw_kernel(const __half* __restrict__ h, const uint4* __restrict__ frag,
@@ -906,7 +908,8 @@ static int launch_dw(const __half* h, const uint4* frag, const float* down, int 
 // ---------------------------------------------------------------------------
 // weighted combine: gradients
 // ---------------------------------------------------------------------------
-// HBM bounds it: 16384 tokens x 2 slots x 4096 in 107 us, 6.3 TB/s.
+// HBM bounds it: 16384 tokens x 2 slots x 4096 in 107 us, 6.3 TB/s; the weights'
+// gradient alone 70 us.
 // WPT warps share a token's row: the row of dout is read once, each kept slot's
 // y row once, dy written once; the dot products are summed over lanes and warps
 // in a fixed order.  Rows no slot keeps (the tail of an over-full expert's

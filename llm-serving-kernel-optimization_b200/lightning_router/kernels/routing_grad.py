@@ -1,8 +1,11 @@
 """The routing path with gradients: train the router, over frozen INT4 experts or with plain ones.
 
 Differentiable counterparts of the functions in :mod:`lightning_router.kernels.expert_routing`.
-Their forward results are those of the inference functions; the backward passes are sm_100a
-kernels without atomics (the same inputs give the same bits).
+``gate_projection``, ``dispatch_tokens`` and ``combine_tokens`` give the inference functions' bits.
+``balanced_gating`` selects the same experts, except that a NaN logit of a live token comes last
+here and is taken by the inference scan where it leads; its weights and loss may differ in the
+last bits (sums in another order).  The backward passes are sm_100a kernels without atomics (the
+same inputs give the same bits).
 
 * :func:`balanced_gating` -- top-k softmax weights, per-expert counts and the balance loss
   from logits, without a dispatch; a token mask keeps padding out.

@@ -194,7 +194,7 @@ class ExpertGroup(nn.Module):
         """:meth:`forward_segments` with low-rank adapters (:class:`ExpertAdapters`) beside
         every projection; ``index`` holds each row's bank entry (:func:`adapter_rows`).  The
         projections are rounded to fp16 before their adapters are added (SwiGLU is taken in
-        fp32 from there)."""
+        fp32 from there; the SiLU of non-gated experts is a pass of its own over fp16 rows)."""
         if not self.quantized:
             raise RuntimeError("forward_segments_adapted requires quantized experts")
         n, f = self.num_experts, self.intermediate_size

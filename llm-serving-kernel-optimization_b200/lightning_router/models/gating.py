@@ -13,8 +13,9 @@ load-balancing loss ``lbw * E * sum_e f_e P_e`` with the uncapped slot fraction
 added to the logits, used by the skewed-routing workload.
 
 With ``trainable=True`` and gradients enabled, weights and loss are differentiable
-in ``gate_proj.weight`` (fp32 or fp16) and in the hidden states: the same values
-from :func:`gate_projection` and :func:`balanced_gating`, whose token mask keeps
+in ``gate_proj.weight`` (fp32 or fp16) and in the hidden states: from
+:func:`gate_projection` (the same logits) and :func:`balanced_gating` (the same
+selection; weights and loss up to the order of fp32 sums), whose token mask keeps
 padding out of the loss.
 """
 

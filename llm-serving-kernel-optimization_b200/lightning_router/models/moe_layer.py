@@ -21,11 +21,14 @@ Two optional uses:
 
 * **adapters**: with ``layer.adapters`` (:class:`ExpertAdapters`) set,
   ``forward(h, adapter_ids=ids)`` adds each token's low-rank adapter to its
-  experts' projections (INT4 experts); tokens with id -1 go without.
+  experts' projections (INT4 experts); tokens with id -1 go without.  A call with
+  ids leaves the fused SwiGLU product for all tokens (gate and up are written,
+  rounded to fp16, and read again), also where every id is -1: pass ``None`` then.
 * **training** (``MoEConfig.trainable``, gradients enabled): the output and the
   balance loss carry gradients.  INT4 experts are frozen: the router's weight
   learns from their rows, which are constants, and hidden states must not
-  require a gradient.  Plain experts (``QuantizationConfig(enabled=False)``)
+  require a gradient.  With a ``token_mask`` the loss is :func:`balanced_gating`'s.
+  Plain experts (``QuantizationConfig(enabled=False)``)
   train with the router, gradients reach the hidden states.  Row gradients are
   fp16: scale the loss.
 """
