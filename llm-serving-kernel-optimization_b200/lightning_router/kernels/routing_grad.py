@@ -74,7 +74,8 @@ def gate_projection(hidden: torch.Tensor, gate_weight: torch.Tensor,
     """fp32 logits ``hidden @ gate_weight.T (+ bias)`` from operands rounded to fp16,
     differentiable in all three.  ``hidden`` (T, d) and ``gate_weight`` (E, d) of any
     floating type (a gradient has its tensor's type, rounded once from fp32 sums);
-    ``d % 16 == 0``, ``E <= 256``."""
+    ``d % 16 == 0``, ``E <= 256``.  As in any product, a hidden row that is not finite leaves
+    the weight's gradient not finite, also where the row's own logits have no gradient."""
     _ext.require_cuda(hidden, gate_weight, bias)
     return _ext.ops().gate_projection(hidden, gate_weight, bias)
 

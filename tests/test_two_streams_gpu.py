@@ -42,24 +42,28 @@ def test_concurrent_layers(name, kw, rounds):
     _ext.check_device_errors()
 
 
-@pytest.mark.parametrize("M", [33, 64, 65, 128, 129, 600])
-def test_concurrent_products(M):
+@pytest.mark.parametrize("K,N,group", [
+    (4096, 2048, 128),      # tcgen05
+    (2048, 1024, 32),       # mma.sync with a ring
+    (1024, 520, 64)])       # CUDA cores
+@pytest.mark.parametrize("M", [1, 16, 33, 64, 65, 128, 129, 600])
+def test_concurrent_products(M, K, N, group):
     from lightning_router.kernels.quantized_matmul import quantized_matmul
     from lightning_router.quantization.pack_weights import quantize_tensor
-    K, N = 4096, 2048
     g = torch.Generator().manual_seed(M)
-    q, s, z = (v.to(DEV) for v in quantize_tensor(torch.randn(K, N, generator=g) * 0.02, 128))
+    q, s, z = (v.to(DEV) for v in quantize_tensor(torch.randn(K, N, generator=g) * 0.02, group))
     xs = [torch.randn(M, K, generator=g).half().to(DEV) for _ in range(3)]
     want = []
     for x in xs:
-        want.append(quantized_matmul(x, q, s, z, N))
+        want.append(quantized_matmul(x, q, s, z, N, group))
         torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(3)]
     for i in range(60):
         got = []
         for n, st in enumerate(streams):
             with torch.cuda.stream(st):
-                got.append([quantized_matmul(xs[(i + n) % 3], q, s, z, N) for _ in range(3)][-1])
+                got.append([quantized_matmul(xs[(i + n) % 3], q, s, z, N, group)
+                            for _ in range(3)][-1])
         torch.cuda.synchronize()
         for n, o in enumerate(got):
             assert torch.equal(o, want[(i + n) % 3]), (i, n)
